@@ -107,7 +107,8 @@ vk_status vk_pool_create_in(const vk_pool_cfg* cfg, void* device_mem, size_t byt
  * with a page format; cfg->page_bytes must be 0. */
 vk_status vk_pool_create_fmt(const vk_pool_cfg* cfg, int32_t kv_format, void* device_mem, size_t bytes,
                              vk_pool** out_pool);
-/* VK_KV_FP16 or VK_KV_FP8; -1 for a byte-page pool or NULL. */
+/* VK_KV_FP16, VK_KV_FP8 or (latent pools, below) VK_KV_LATENT_*; -1 for a
+ * byte-page pool or NULL. */
 int32_t   vk_pool_kv_format(const vk_pool* pool);
 
 vk_status vk_pool_destroy(vk_pool* pool);
@@ -362,6 +363,132 @@ vk_status vk_oproj_pack_weight(const float* w, int32_t ldw, int32_t k_rows, int3
                                void* stream);
 vk_status vk_oproj_pack_weight_t16(const void* w_t, int32_t ldw, int32_t n, int32_t k_rows,
                                    void* w_packed, void* stream);
+
+/* ---- element types of the entry points below ------------------------------- */
+#define VK_F16  0
+#define VK_BF16 1
+#define VK_F32  2
+
+/* ---- rotary positions -------------------------------------------------------
+ * The rotation as an operator of its own, for models whose rotary form is not
+ * the one that vk_set_rope fuses (interleaved pairs over the whole head,
+ * unscaled frequencies; the reference's cuda/rope.cu:34-60):
+ *   y[a_i] = x[a_i] cos - x[b_i] sin,  y[b_i] = x[a_i] sin + x[b_i] cos,
+ *   angle = position * f_i,  f_i = theta_base^(-2i / rotary_dim)
+ * with pairs (a_i, b_i) = (2i, 2i+1) (VK_ROTARY_INTERLEAVED) or
+ * (i, i + rotary_dim/2) (VK_ROTARY_HALF) of the leading rotary_dim elements of
+ * each head; the elements behind them are copied (not touched in place).  To
+ * rotate another part of a head, pass a view that starts there.
+ * Scalings of f_i for contexts longer than original_len:
+ *   VK_ROTARY_LINEAR         f_i / factor
+ *   VK_ROTARY_BY_PARTS       pairs that make more than `high` turns within
+ *       original_len keep f_i, pairs that make fewer than `low` get
+ *       f_i / factor, with a linear ramp over the pair index between;
+ *       cos and sin are multiplied by 0.1 ln(factor) + 1 for factor > 1
+ *   VK_ROTARY_BY_WAVELENGTH  the same two ends with
+ *       t = original_len * f_i / (2 pi) turns: a blend (t - low) / (high - low)
+ * magnitude > 0 replaces the factor on cos and sin (0: the scaling's own, 1
+ * unless said above).  Angles are exact to fp32 at any int32 position. */
+#define VK_ROTARY_INTERLEAVED 0
+#define VK_ROTARY_HALF        1
+#define VK_ROTARY_PLAIN         0
+#define VK_ROTARY_LINEAR        1
+#define VK_ROTARY_BY_PARTS      2
+#define VK_ROTARY_BY_WAVELENGTH 3
+
+typedef struct vk_rotary_cfg {
+    int32_t rotary_dim;    /* even, 2..256                                      */
+    int32_t layout;        /* VK_ROTARY_INTERLEAVED or VK_ROTARY_HALF           */
+    int32_t scaling;       /* VK_ROTARY_PLAIN, ...                              */
+    int32_t device;        /* CUDA device that vk_rotary_apply runs on          */
+    double  theta_base;    /* > 1                                               */
+    double  factor, original_len, low, high, magnitude;
+} vk_rotary_cfg;
+
+/* One tensor: element (token, head, d) is x[token*x_token + head*x_head + d]
+ * (strides in elements); the result goes to y likewise.  y may be x with equal
+ * strides (in place), and may not overlap x otherwise. */
+typedef struct vk_rotary_view {
+    const void* x;
+    void*       y;
+    int64_t     x_token, x_head, y_token, y_head;
+    int32_t     heads;
+} vk_rotary_view;
+
+typedef struct vk_rotary vk_rotary;
+/* Host only: the handle holds a table that launches pass by value. */
+vk_status vk_rotary_create(const vk_rotary_cfg* cfg, vk_rotary** out);
+vk_status vk_rotary_destroy(vk_rotary* r);
+/* The scaled f_i (rotary_dim/2 values) and the magnitude of a configuration. */
+vk_status vk_rotary_frequencies(const vk_rotary_cfg* cfg, double* out, double* magnitude);
+/* Rotates q, and k unless NULL, of `tokens` tokens in one launch, on the cfg's
+ * device.  dtype: VK_F16, VK_BF16 or VK_F32 of x and y; positions: int32
+ * [tokens] device array, any sign.  fp32 arithmetic, one rounding. */
+vk_status vk_rotary_apply(const vk_rotary* r, int32_t dtype, const vk_rotary_view* q, const vk_rotary_view* k,
+                          int32_t head_dim, const int32_t* positions, int32_t tokens, void* stream);
+
+/* ---- latent cache: one shared vector a token instead of keys and values ------
+ * For attention whose keys and values are all linear in one latent vector c of
+ * a token (plus one rotary key part r shared by the heads):
+ *   k_h = [W_k,h c | r],  v_h = W_v,h c
+ * A latent pool caches only the row [c | r], latent_dim + rope_dim elements:
+ *   row (layer, page, slot) at base + ((layer*num_pages + page)*page_tokens
+ *                                      + slot) * (latent_dim + rope_dim) * 2
+ * Limits: latent_dim 128, 256, 384 or 512; rope_dim 16, 32, 48 or 64;
+ * page_tokens 16, 32 or 64 (64 fetches a tile of the attention in the fewest
+ * copies); dtype VK_F16 or VK_BF16.  The allocator, copy, remap, compaction and
+ * swap entry points take latent pools; the entry points of K/V pages refuse
+ * them.  device_mem NULL: the library allocates and zero-fills; else the pool
+ * lives in caller-owned memory (256-byte aligned, left as it is). */
+#define VK_KV_LATENT_F16  2   /* vk_pool_kv_format() of a latent pool */
+#define VK_KV_LATENT_BF16 3
+
+typedef struct vk_latent_cfg {
+    int32_t num_layers, latent_dim, rope_dim, page_tokens, num_pages, device, dtype;
+} vk_latent_cfg;
+
+vk_status vk_latent_pool_create(const vk_latent_cfg* cfg, void* device_mem, size_t bytes, vk_pool** out_pool);
+
+/* Appends `tokens` new tokens of `batch` sequences.  Token rows come
+ * concatenated; offsets (int32 [batch+1], device) gives sequence b the rows
+ * offsets[b]..offsets[b+1]-1 (rows behind offsets[batch] are ignored); NULL:
+ * tokens / batch rows each.  Row offsets[b]+i is written to position
+ * positions[b]+i of sequence b.
+ * latent, k_rope: the pool's type, row strides in elements (two views of one
+ * down-projection's output).  norm_weight (latent_dim elements of the pool's
+ * type; NULL: no norm): the latent is stored as c / sqrt(mean(c^2) + eps) *
+ * norm_weight.  rotary (NULL: none; its rotary_dim must be rope_dim): k_rope is
+ * rotated at the token's position.  fp32 arithmetic, one rounding.
+ * Rows 16-byte aligned (strides multiples of 8). */
+vk_status vk_latent_append(vk_pool* pool, int32_t layer, const void* latent, int64_t latent_stride,
+                           const void* k_rope, int64_t rope_stride, const void* norm_weight, float eps,
+                           const vk_rotary* rotary, const int32_t* block_tables, int32_t bt_stride,
+                           const int32_t* positions, const int32_t* offsets, int32_t batch, int32_t tokens,
+                           void* stream);
+
+/* Attention in the absorbed form, for decode steps and a few drafted tokens:
+ * the query is already in the latent space (q_latent = W_k,h^T q_h), and
+ *   s_j = scale * (q_latent . c_j + q_rope . r_j),  out = sum_j softmax(s)_j c_j
+ * over the sequence's cached rows (out goes through W_v,h afterwards).
+ * Query token t of tokens_per_seq (T) sees the first seq_lens[b] - (T-1-t)
+ * rows: seq_lens (device) counts all T tokens, appended before the call.  A row
+ * that sees nothing gives zeros and an lse of -inf.
+ * Element (b, t, h, d) of q_latent: [(b*T + t)*ql_token_stride +
+ * h*ql_head_stride + d], q_rope (rotated already) likewise; out: [batch, T,
+ * num_heads, latent_dim], lse (optional): [batch, T, num_heads] fp32, the natural
+ * log of the sum of exp(s), to join outputs over other keys.  Pool's type;
+ * 16-byte aligned, strides multiples of 8.  scale must be given (> 0).  A length
+ * below 0 or beyond the table's capacity records VK_ERR_SEQ_LEN and counts as 0.
+ * Lengths are read on the device, so a captured call replays with new ones.
+ * workspace: vk_latent_decode_workspace_size() bytes, 16-byte aligned; needs no
+ * initial value; calls that may overlap on the GPU need one each. */
+size_t    vk_latent_decode_workspace_size(const vk_pool* pool, int32_t batch, int32_t tokens_per_seq,
+                                          int32_t num_heads);
+vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* q_latent, int64_t ql_token_stride,
+                           int64_t ql_head_stride, const void* q_rope, int64_t qr_token_stride,
+                           int64_t qr_head_stride, void* out, float* lse, const int32_t* block_tables,
+                           int32_t bt_stride, const int32_t* seq_lens, int32_t batch, int32_t tokens_per_seq,
+                           int32_t num_heads, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- K3: chunked prefill -------------------------------------------------
  * The prefill use of launch_attention (src/transformer.cpp:136-189 with

@@ -30,6 +30,22 @@ class VkPoolCfg(ctypes.Structure):
                 ("page_bytes", c_u64)]
 
 
+class VkRotaryCfg(ctypes.Structure):
+    _fields_ = [("rotary_dim", c_i32), ("layout", c_i32), ("scaling", c_i32), ("device", c_i32),
+                ("theta_base", ctypes.c_double), ("factor", ctypes.c_double), ("original_len", ctypes.c_double),
+                ("low", ctypes.c_double), ("high", ctypes.c_double), ("magnitude", ctypes.c_double)]
+
+
+class VkRotaryView(ctypes.Structure):
+    _fields_ = [("x", vp), ("y", vp), ("x_token", c_i64), ("x_head", c_i64), ("y_token", c_i64),
+                ("y_head", c_i64), ("heads", c_i32)]
+
+
+class VkLatentCfg(ctypes.Structure):
+    _fields_ = [("num_layers", c_i32), ("latent_dim", c_i32), ("rope_dim", c_i32), ("page_tokens", c_i32),
+                ("num_pages", c_i32), ("device", c_i32), ("dtype", c_i32)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "vk_pool_create": (c_i32, [ctypes.POINTER(VkPoolCfg), ctypes.POINTER(vp)]),
@@ -96,6 +112,18 @@ SIGNATURES = {
     "vk_swap_in": (c_i32, [vp, vp, c_i32, i32p, vp]),
     "vk_swap_in_to": (c_i32, [vp, vp, i32p, c_i32, vp]),
     "vk_attention_f32": (c_i32, [vp, vp, vp, vp, c_i32, c_i32, c_i32, c_i32, vp]),
+    "vk_rotary_create": (c_i32, [ctypes.POINTER(VkRotaryCfg), ctypes.POINTER(vp)]),
+    "vk_rotary_destroy": (c_i32, [vp]),
+    "vk_rotary_frequencies": (c_i32, [ctypes.POINTER(VkRotaryCfg), ctypes.POINTER(ctypes.c_double),
+                                      ctypes.POINTER(ctypes.c_double)]),
+    "vk_rotary_apply": (c_i32, [vp, c_i32, ctypes.POINTER(VkRotaryView), ctypes.POINTER(VkRotaryView), c_i32, vp,
+                                c_i32, vp]),
+    "vk_latent_pool_create": (c_i32, [ctypes.POINTER(VkLatentCfg), vp, c_sz, ctypes.POINTER(vp)]),
+    "vk_latent_append": (c_i32, [vp, c_i32, vp, c_i64, vp, c_i64, vp, c_f32, vp, vp, c_i32, vp, vp, c_i32, c_i32,
+                                 vp]),
+    "vk_latent_decode_workspace_size": (c_sz, [vp, c_i32, c_i32, c_i32]),
+    "vk_latent_decode": (c_i32, [vp, c_i32, vp, c_i64, c_i64, vp, c_i64, c_i64, vp, vp, vp, c_i32, vp, c_i32, c_i32,
+                                 c_i32, c_f32, vp, c_sz, vp]),
     "vk_last_error_string": (ctypes.c_char_p, []),
     "vk_status_string": (ctypes.c_char_p, [c_i32]),
     "vk_version": (c_i32, []),

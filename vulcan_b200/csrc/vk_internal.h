@@ -57,6 +57,8 @@ struct vk_pool {
     int32_t plan_workers = 0;        // cap on planned-decode workers (0 = resident warps)
     float rope_theta = 0.f;          // fused RoPE base (0 = off)
     float* rope_freq = nullptr;      // device [head_dim/2] frequencies when RoPE is on
+    int latent_dim = 0;              // latent pools (kv_format VK_KV_LATENT_*): latent and rotary
+    int rope_dim = 0;                // elements of a token's row
     int32_t num_sms = vk::kNumSmsDefault;
     vk::Allocator alloc;
 };
@@ -79,6 +81,11 @@ struct DeviceGuard {
         if (prev >= 0) cudaSetDevice(prev);
     }
 };
+
+// A latent pool: kv is false, so every entry point of K/V pages refuses it.
+inline bool is_latent(const vk_pool* p) {
+    return p->kv_format == VK_KV_LATENT_F16 || p->kv_format == VK_KV_LATENT_BF16;
+}
 
 // cuTensorMapEncodeTiled from the driver (NULL when unavailable).
 PFN_cuTensorMapEncodeTiled_v12000 tmap_encode_fn();
@@ -111,6 +118,8 @@ struct GatherView {
 bool gather_view(const vk_gather* g, GatherView* v);
 int gather_device(const vk_gather* g);
 uint32_t gather_next_epoch(vk_gather* g);
+struct RotaryTable;
+const RotaryTable* rotary_table(const vk_rotary* r);
 vk_status prefill_tc(vk_pool* pool, int layer, const void* q, void* out, const int32_t* bt, int bt_stride,
                      const int32_t* positions, int B, int T, int Hq, float scale, cudaStream_t st);
 

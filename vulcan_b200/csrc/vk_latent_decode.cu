@@ -1,0 +1,709 @@
+// Latent attention, absorbed form (vk_latent_decode): every query row of a
+// sequence (its T new tokens x H heads) attends the cached rows x_j = [c_j | r_j]
+//
+//   s_j = scale * (ql . c_j + qr . r_j),  out = sum_j softmax(s)_j c_j
+//
+// so the cache row is key and value at once and is read from HBM once for up to
+// 64 rows.  Floor: (latent + rope) * 2 bytes a cached token; 2 * (2 latent +
+// rope) flop a token and row, which 64 rows keep below the memory time.
+//
+// One persistent CTA per SM.  The cached tokens of all units (sequence, group
+// of 64 rows) are cut into 64-key tiles, laid end to end and dealt in equal
+// contiguous ranges, from the device's own lengths (no host plan: a captured
+// graph replays with other lengths).  A unit that several CTAs share leaves
+// fp32 partials (O, m, l) that latent_merge_kernel joins.
+//
+//  * warp 4 streams tiles with 2-D TMA boxes (64 elements x one page's rows,
+//    128-byte swizzle) into a ring of as many stages as fit (2 at 512 + 64);
+//  * warp 5, one thread, issues tcgen05.mma:  S[64 rows x 64 keys] = Q K^T (M 64,
+//    K-major both), then  O^T[latent x 64 rows] += V^T P^T  as M = 128 blocks of
+//    latent elements.  The transposed output keeps all 128 lanes at work with 64
+//    rows (O itself would be M = 64 at half the rate) and needs 256 TMEM columns
+//    instead of 512, so S has two buffers beside it: S of tile i+1 is issued
+//    before O of tile i and the tensor core works through the softmax.  V^T is
+//    the K tile itself read MN-major, P^T is P read K-major: nothing is copied;
+//  * warps 0-3: softmax with running maximum and sum.  Row r of S lies in lane
+//    (r/16)*32 + r%16 of TMEM (M = 64 fills 16 lanes of each warp), so the upper
+//    16 lanes take the second half of each row's keys by shuffle.  O is rescaled
+//    only when a row's maximum grows by more than 2^8 (all warps vote).
+//
+// P is rounded to the cache's 16-bit type for the second product: relative
+// error 2^-9 (bf16) or 2^-12 (fp16) a weight, below the output's own rounding;
+// the sum of the weights is taken from the unrounded fp32 values.
+//
+// Rows of the last tile behind the sequence are zeroed in shared memory before
+// the second product (0 * NaN is NaN), and keys that only some of the T tokens
+// may see have non-finite elements cleared there: a row that does see such a
+// key gets its NaN through S.
+#include "vk_internal.h"
+#include "vk_latent.cuh"
+#include "vk_ptx.cuh"
+#include "vk_rotary.cuh"
+#include "vk_tc.cuh"
+
+namespace vk {
+
+constexpr int kLdKeys = 64;       // keys of a tile
+constexpr int kLdThreads = 192;   // 4 softmax warps, TMA warp, MMA warp
+constexpr int kLdMaxStages = 8;
+constexpr int kLdChunk = kLdKeys * 128;  // 64 keys x 64 elements, 128-byte rows
+constexpr int kLdAux = 1024;             // barriers, alpha, 1/l, schedule
+constexpr int kLdSmemMax = 232448;
+// A unit's prologue and epilogue (q load, output) in tiles, for the deal.
+constexpr int kLdUnitCost = 2;
+// Least cost of a CTA's range: fewer, longer pieces when there is little work
+constexpr int kLdMinRange = 4;
+
+struct LdParams {
+    const char* ql;
+    const char* qr;
+    int64_t ql_token, ql_head, qr_token, qr_head;  // strides in elements
+    char* out;
+    float* lse;
+    const int32_t* bt;
+    const int32_t* lens;
+    uint32_t* err;
+    float* ws_o;     // [2 * CTAs][64][latent]
+    float2* ws_ml;   // [2 * CTAs][64]: maximum (log2 domain), sum
+    int2* ws_unit;   // [units]: first and last CTA of a split unit, or (-1, -1)
+    int bt_stride, B, T, H, groups, layer, num_pages, P, latent, rope, nch, stages;
+    float scale_log2;
+};
+
+__device__ __forceinline__ int ld_len(const LdParams& p, int b) {
+    const int len = __ldg(p.lens + b);
+    return len < 0 || len > static_cast<int64_t>(p.bt_stride) * p.P ? 0 : len;
+}
+
+struct LdPiece {
+    int b, g, t0, t1, tiles, len;
+    int64_t unit_start;
+    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == tiles; }
+};
+
+// The pieces of one CTA's range [v, v1) of the laid-out units; a unit spans its
+// tiles, then kLdUnitCost.
+struct LdWalk {
+    int64_t v, v1, unit_start;
+    int b, g, len, tiles;
+
+    __device__ __forceinline__ bool next(const LdParams& p, LdPiece& o) {
+        while (v < v1) {
+            const int64_t unit_end = unit_start + tiles + kLdUnitCost;
+            const int64_t ve = v1 < unit_end ? v1 : unit_end;
+            o.b = b;
+            o.g = g;
+            o.len = len;
+            o.tiles = tiles;
+            o.unit_start = unit_start;
+            o.t0 = static_cast<int>(v - unit_start);
+            o.t1 = static_cast<int>(ve - unit_start < tiles ? ve - unit_start : tiles);
+            v = ve;
+            if (v == unit_end) {
+                unit_start = unit_end;
+                if (++g == p.groups) {
+                    g = 0;
+                    ++b;
+                    len = b < p.B ? ld_len(p, b) : 0;
+                    tiles = (len + kLdKeys - 1) / kLdKeys;
+                }
+            }
+            if (o.t0 < o.t1 || (o.t0 == 0 && o.tiles == 0)) return true;  // an empty unit: its rows are zeros
+        }
+        return false;
+    }
+    __device__ __forceinline__ bool next_real(const LdParams& p, LdPiece& o) {
+        while (next(p, o))
+            if (o.t0 < o.t1) return true;
+        return false;
+    }
+};
+
+__device__ __forceinline__ void bar_softmax() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool bar_softmax_or(bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(static_cast<uint32_t>(x))
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+// 0 in the place of each non-finite 16-bit element of a word.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_word(uint32_t w) {
+    constexpr uint32_t e = Elem<T>::kBf16 ? 0x7f80u : 0x7c00u;
+    if ((w & e) == e) w &= 0xffff0000u;
+    if ((w & (e << 16)) == (e << 16)) w &= 0x0000ffffu;
+    return w;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __grid_constant__ CUtensorMap tmap,
+                                                                      const __grid_constant__ LdParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_u32(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t stage_bytes = p.nch * kLdChunk;
+    const uint32_t s_q = sbase + p.stages * stage_bytes, s_p = s_q + stage_bytes;
+    uint8_t* aux = smem + (p.stages + 1) * stage_bytes + kLdChunk;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(aux);
+    uint64_t* k_full = bars;                    // [stages] tile landed
+    uint64_t* k_empty = bars + kLdMaxStages;    // [stages] both products have read it
+    uint64_t* s_full = bars + 2 * kLdMaxStages;  // [2]
+    uint64_t* p_full = s_full + 2;              // P written, O rescaled, last piece's O read
+    uint64_t* pv_done = s_full + 3;
+    uint64_t* q_full = s_full + 4;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 5);
+    float* alpha = reinterpret_cast<float*>(aux + 256);   // [64] rescale factors
+    float* inv_l = reinterpret_cast<float*>(aux + 512);   // [64]
+    int64_t* sched = reinterpret_cast<int64_t*>(aux + 768);  // total, first b, its start; then warp sums
+    int64_t* wsum = sched + 4;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // ---- the deal: cost of every sequence from the device's lengths, a block scan, this CTA's start
+    const int per = (p.B + kLdThreads - 1) / kLdThreads;
+    const int b_lo = threadIdx.x * per, b_hi = min(p.B, b_lo + per);
+    int64_t mine = 0;
+    for (int b = b_lo; b < b_hi; ++b) {
+        const int len = ld_len(p, b);
+        mine += static_cast<int64_t>(p.groups) * ((len + kLdKeys - 1) / kLdKeys + kLdUnitCost);
+        if (blockIdx.x == 0 && len != __ldg(p.lens + b)) atomicOr(p.err, VK_ERR_SEQ_LEN);
+    }
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) {
+            mbar_init(smem_u32(&k_full[i]), 1);
+            mbar_init(smem_u32(&k_empty[i]), 1);
+        }
+        mbar_init(smem_u32(&s_full[0]), 1);
+        mbar_init(smem_u32(&s_full[1]), 1);
+        mbar_init(smem_u32(p_full), 4);
+        mbar_init(smem_u32(pv_done), 1);
+        mbar_init(smem_u32(q_full), 4);
+        mbar_fence_init();
+    }
+    __syncthreads();
+    int64_t total = 0, before = incl - mine;
+    for (int w = 0; w < kLdThreads / 32; ++w) {
+        total += wsum[w];
+        if (w < warp) before += wsum[w];
+    }
+    const int64_t n = min(static_cast<int64_t>(gridDim.x), (total + kLdMinRange - 1) / kLdMinRange);
+    if (blockIdx.x >= n) return;  // the whole CTA: nothing allocated yet
+    LdWalk walk0;
+    walk0.v = blockIdx.x * total / n;
+    walk0.v1 = (blockIdx.x + 1) * total / n;
+    if (walk0.v >= before && walk0.v < before + mine) {  // one thread: it finds the first unit
+        int64_t at = before;
+        int b = b_lo;
+        for (;; ++b) {
+            const int64_t c = static_cast<int64_t>(p.groups) * ((ld_len(p, b) + kLdKeys - 1) / kLdKeys + kLdUnitCost);
+            if (walk0.v < at + c) break;
+            at += c;
+        }
+        sched[0] = b;
+        sched[1] = at;
+    }
+    if (warp == 5) {
+        tmem_alloc(smem_u32(tmem_slot), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    walk0.b = static_cast<int>(sched[0]);
+    walk0.len = ld_len(p, walk0.b);
+    walk0.tiles = (walk0.len + kLdKeys - 1) / kLdKeys;
+    {
+        const int64_t span = walk0.tiles + kLdUnitCost;
+        walk0.g = static_cast<int>((walk0.v - sched[1]) / span);
+        walk0.unit_start = sched[1] + walk0.g * span;
+    }
+    const int rows = p.T * p.H;
+
+    if (warp == 4) {
+        // ------------------------------------------------------------ TMA producer
+        LdWalk w = walk0;
+        LdPiece c;
+        int it = 0;
+        bool ok = true;
+        if (lane == 0) prefetch_tmap(&tmap);
+        const uint64_t pol = p.groups > 1 ? l2_evict_last_policy() : l2_evict_first_policy();
+        const int ppt = kLdKeys / p.P;  // pages of a full tile
+        while (ok && w.next_real(p, c)) {
+            const int32_t* row = p.bt + static_cast<int64_t>(c.b) * p.bt_stride;
+            const int npages = (c.len + p.P - 1) / p.P;
+            int win = -32, entry = 0;  // block-table entries win..win+31, one a lane
+            for (int t = c.t0; t < c.t1 && ok; ++t, ++it) {
+                const int first = t * ppt, cnt = min(ppt, npages - first);
+                if (first + cnt > win + 32) {
+                    win = first;
+                    entry = win + lane < npages ? __ldg(row + win + lane) : 0;
+                    if (entry < 0 || entry >= p.num_pages) {
+                        atomicOr(p.err, VK_ERR_PAGE_ID);
+                        entry = 0;
+                    }
+                }
+                const int st = it % p.stages;
+                if (it >= p.stages) ok = wait_all(smem_u32(&k_empty[st]), (it / p.stages - 1) & 1, p.err);
+                if (!ok) break;
+                const uint32_t bar = smem_u32(&k_full[st]);
+                if (lane == 0) mbar_expect_tx(bar, cnt * p.nch * p.P * 128);
+                __syncwarp();
+                const uint32_t dst = sbase + st * stage_bytes;
+                for (int k0 = 0; k0 < cnt * p.nch; k0 += 32) {
+                    const int k = k0 + lane, i = min(k / p.nch, cnt - 1), ch = k % p.nch;
+                    const int page = __shfl_sync(0xffffffffu, entry, first - win + i);
+                    if (k < cnt * p.nch)
+                        tma_load_2d(dst + ch * kLdChunk + i * p.P * 128, &tmap, ch * 64, (p.layer * p.num_pages + page) * p.P,
+                                    bar, pol);
+                }
+            }
+        }
+    } else if (warp == 5) {
+        // ------------------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            LdWalk w = walk0;
+            LdPiece c;
+            int it = 0, piece = 0;
+            bool ok = true;
+            constexpr uint32_t id_s = idesc_16(Elem<T>::kBf16, 64, 64, 0, 0);
+            constexpr uint32_t id_pv = idesc_16(Elem<T>::kBf16, 128, 64, 1, 0);
+            const uint64_t dq = umma_desc_sw128(s_q, 16, 1024);
+            const uint64_t dp = umma_desc_sw128(s_p, 16, 1024);
+            const int lch = p.latent >> 6, rsteps = p.rope >> 4;
+            auto issue_s = [&](int i) {
+                const int st = i % p.stages;
+                ok = ok && mbar_wait(smem_u32(&k_full[st]), (i / p.stages) & 1, p.err);
+                if (!ok) return;
+                tc_fence_after();
+                const uint64_t dk = umma_desc_sw128(sbase + st * stage_bytes, 16, 1024);
+                const uint32_t d = tmem + 256 + (i & 1) * 64;
+                for (int ch = 0; ch < lch; ++ch)
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        const uint64_t off = static_cast<uint64_t>((ch * kLdChunk + ks * 32) >> 4);
+                        umma_ss(d, dq + off, dk + off, id_s, (ch | ks) != 0);
+                    }
+                for (int ks = 0; ks < rsteps; ++ks) {
+                    const uint64_t off = static_cast<uint64_t>((lch * kLdChunk + ks * 32) >> 4);
+                    umma_ss(d, dq + off, dk + off, id_s, 1);
+                }
+                umma_commit(smem_u32(&s_full[i & 1]));
+            };
+            while (ok && w.next_real(p, c)) {
+                const int nt = c.t1 - c.t0;
+                ok = mbar_wait(smem_u32(q_full), piece & 1, p.err);
+                ++piece;
+                if (!ok) break;
+                issue_s(it);
+                for (int j = 0; j < nt && ok; ++j, ++it) {
+                    if (j + 1 < nt) issue_s(it + 1);
+                    ok = ok && mbar_wait(smem_u32(p_full), it & 1, p.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const int st = it % p.stages;
+                    const uint64_t dv = umma_desc_sw128(sbase + st * stage_bytes, kLdChunk, 1024);
+                    for (int mb = 0; mb < (p.latent >> 7); ++mb)
+#pragma unroll
+                        for (int ks = 0; ks < kLdKeys / 16; ++ks)
+                            umma_ss(tmem + mb * 64, dv + static_cast<uint64_t>((mb * 2 * kLdChunk + ks * 2048) >> 4),
+                                    dp + static_cast<uint64_t>((ks * 32) >> 4), id_pv, (j | ks) != 0);
+                    umma_commit(smem_u32(pv_done));
+                    umma_commit(smem_u32(&k_empty[st]));
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ softmax and output
+        LdWalk w = walk0;
+        LdPiece c, nx;
+        const int r = warp * 16 + (lane & 15), hi = lane >> 4;  // row of the group; which half of a tile's keys
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+        const int width8 = (p.latent + p.rope) >> 3, lat8 = p.latent >> 3;
+
+        // next piece with tiles; rows of empty units are written on the way
+        auto advance = [&](LdPiece& o) -> bool {
+            while (w.next(p, o)) {
+                if (o.t0 < o.t1) return true;
+                const int live = min(64, rows - o.g * 64);
+                const int64_t row0 = static_cast<int64_t>(o.b) * rows + o.g * 64;
+                uint4* dst = reinterpret_cast<uint4*>(p.out + 2 * row0 * p.latent);
+                for (int i = threadIdx.x; i < live * lat8; i += 128) dst[i] = make_uint4(0, 0, 0, 0);
+                if (p.lse && threadIdx.x < live) p.lse[row0 + threadIdx.x] = -INFINITY;
+                if (threadIdx.x == 0) p.ws_unit[static_cast<int64_t>(o.b) * p.groups + o.g] = make_int2(-1, -1);
+            }
+            return false;
+        };
+        auto load_q = [&](const LdPiece& o) {
+            for (int k = warp; k < 64; k += 4) {
+                const int rr = o.g * 64 + k;
+                const bool live = rr < rows;
+                const int t = live ? rr / p.H : 0, h = live ? rr % p.H : 0;
+                const int64_t tok = static_cast<int64_t>(o.b) * p.T + t;
+                const char* ql = p.ql + 2 * (tok * p.ql_token + h * p.ql_head);
+                const char* qr = p.qr + 2 * (tok * p.qr_token + h * p.qr_head);
+                for (int v = lane; v < width8; v += 32)
+                    cp_async16(s_q + (v >> 3) * kLdChunk + swz128(k, v & 7), v < lat8 ? ql + v * 16 : qr + (v - lat8) * 16, live);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(q_full));
+        };
+
+        int it = 0;
+        bool fail = false;
+        bool have = advance(c);
+        if (have) load_q(c);
+        while (have) {
+            float m = -INFINITY, l = 0.f;  // log2 domain; l: this lane's half of the keys
+            const int row = c.g * 64 + r;
+            const int tq = row < rows ? row / p.H : p.T - 1;
+            const int lim = c.len - (p.T - 1 - tq);   // this row's keys
+            const int lim0 = c.len - (p.T - 1);       // keys that every token sees
+            for (int t = c.t0; t < c.t1; ++t, ++it) {
+                const int key0 = t * kLdKeys;
+                fail = !wait_all(smem_u32(&s_full[it & 1]), (it >> 1) & 1, p.err) || fail;
+                tc_fence_after();
+                float a[32], bq[32];
+                tmem_ld32(lane_base + 256 + (it & 1) * 64, a);
+                tmem_ld32(lane_base + 256 + (it & 1) * 64 + 32, bq);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float x = __shfl_sync(0xffffffffu, bq[i], lane & 15);
+                    if (hi) a[i] = x;
+                }
+                const bool tail = key0 + kLdKeys > lim0;
+                if (tail) {
+                    const int left = lim - key0 - 32 * hi;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (i >= left) a[i] = -INFINITY;
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    mx[0] = fmaxf(mx[0], a[i]);
+                    mx[1] = fmaxf(mx[1], a[i + 1]);
+                    mx[2] = fmaxf(mx[2], a[i + 2]);
+                    mx[3] = fmaxf(mx[3], a[i + 3]);
+                }
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                float al = 1.f;
+                if (top > m + 8.f || m == -INFINITY) {
+                    const float mn = fmaxf(m, top);
+                    al = m == -INFINITY ? 0.f : ex2(m - mn);
+                    m = mn;
+                }
+                // before the unit's first product O holds nothing to rescale
+                const bool resc = t > c.t0 && al != 1.f && row < rows;
+                const bool any = bar_softmax_or(resc || fail);
+                if (any && bar_softmax_or(fail)) goto done;
+                const float mneg = m == -INFINITY ? 0.f : -m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t pk[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float e0 = ex2(fmaf(a[i], p.scale_log2, mneg)), e1 = ex2(fmaf(a[i + 1], p.scale_log2, mneg));
+                    sum[(i >> 1) & 3] += e0 + e1;
+                    pk[i >> 1] = Elem<T>::pack(e0, e1);
+                }
+                l = l * al + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                if (tail) {  // V rows: zeros behind the sequence, finite where some token may not look
+                    const int st = it % p.stages;
+                    const int lo = max(0, lim0 - key0), nrow = kLdKeys - lo;
+                    for (int i = threadIdx.x; i < nrow * lat8; i += 128) {
+                        const int kr = lo + i / lat8, v = i % lat8;
+                        const uint32_t addr = sbase + st * stage_bytes + (v >> 3) * kLdChunk + swz128(kr, v & 7);
+                        uint4 x = make_uint4(0, 0, 0, 0);
+                        if (key0 + kr < c.len) {
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                                         : "r"(addr));
+                            x = make_uint4(finite_word<T>(x.x), finite_word<T>(x.y), finite_word<T>(x.z), finite_word<T>(x.w));
+                        }
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
+                                     : "memory");
+                    }
+                }
+                // P's buffer is free, and O complete, once the previous tile's product is done
+                if (it > 0) fail = !wait_all(smem_u32(pv_done), (it - 1) & 1, p.err) || fail;
+                if (any) {
+                    tc_fence_after();
+                    if (!hi) alpha[r] = resc ? al : 1.f;
+                    bar_softmax();
+                    for (int col = 0; col < (p.latent >> 1); col += 32) {
+                        float o[32];
+                        tmem_ld32(lane_base + col, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] *= alpha[(col & 32) + i];
+                        tmem_st32(lane_base + col, o);
+                    }
+                    tmem_wait_st();
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s_p + swz128(r, hi * 4 + k)), "r"(pk[4 * k]),
+                                 "r"(pk[4 * k + 1]), "r"(pk[4 * k + 2]), "r"(pk[4 * k + 3])
+                                 : "memory");
+                fence_async_smem();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(p_full));
+            }
+            // the last S of this piece has been read: the next piece's queries may land
+            have = advance(nx);
+            if (have) load_q(nx);
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
+            const bool whole = c.whole();
+            const int64_t row0 = static_cast<int64_t>(c.b) * rows + c.g * 64;
+            const int slot = 2 * blockIdx.x + (c.t0 == 0 ? 1 : 0);
+            if (!hi) {
+                inv_l[r] = l > 0.f || l != l ? 1.f / l : 0.f;
+                if (whole) {
+                    if (p.lse && row < rows) p.lse[row0 + r] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+                } else {
+                    p.ws_ml[slot * 64 + r] = make_float2(m, l);
+                }
+            }
+            if (threadIdx.x == 0 && c.t0 == 0) {
+                int2 u = make_int2(-1, -1);
+                if (!whole)  // CTA of the unit's last tile: the largest i with i * total / n <= its position
+                    u = make_int2(blockIdx.x, static_cast<int>(((c.unit_start + c.tiles) * n - 1) / total));
+                p.ws_unit[static_cast<int64_t>(c.b) * p.groups + c.g] = u;
+            }
+            fail = !wait_all(smem_u32(pv_done), (it - 1) & 1, p.err) || fail;
+            if (bar_softmax_or(fail)) goto done;
+            tc_fence_after();
+            const int live = min(64, rows - c.g * 64);
+            for (int mb = 0; mb < (p.latent >> 7); ++mb)
+#pragma unroll
+                for (int hc = 0; hc < 2; ++hc) {
+                    if (hc * 32 >= live) break;
+                    float o[32];
+                    tmem_ld32(lane_base + mb * 64 + hc * 32, o);
+                    tmem_wait_ld();
+                    const int d = mb * 128 + warp * 32 + lane;
+                    if (whole) {
+                        // neighbouring lanes hold neighbouring elements: they trade so that each
+                        // stores two elements of one row
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float i0 = inv_l[hc * 32 + i], i1 = inv_l[hc * 32 + i + 1];
+                            const float x0 = i0 == 0.f ? 0.f : o[i] * i0, x1 = i1 == 0.f ? 0.f : o[i + 1] * i1;
+                            const float got = __shfl_xor_sync(0xffffffffu, lane & 1 ? x0 : x1, 1);
+                            const int rr = hc * 32 + i + (lane & 1);
+                            const uint32_t wv = lane & 1 ? Elem<T>::pack(got, x1) : Elem<T>::pack(x0, got);
+                            if (rr < live)
+                                *reinterpret_cast<uint32_t*>(p.out + 2 * ((row0 + rr) * p.latent + (d & ~1))) = wv;
+                        }
+                    } else {
+                        float* dst = p.ws_o + (static_cast<int64_t>(slot) * 64 + hc * 32) * p.latent + d;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (hc * 32 + i < live) dst[static_cast<int64_t>(i) * p.latent] = o[i];
+                    }
+                }
+            tc_fence_before();
+            c = nx;
+        }
+    done:;
+    }
+    __syncthreads();
+    if (warp == 5) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the partials of units that several CTAs share.  Block (row, unit):
+// its warps take the unit's pieces in turn, then meet in shared memory; the
+// order of the sums is fixed by the pieces, so results repeat bit for bit.
+template <typename T>
+__global__ void latent_merge_kernel(const LdParams p) {
+    extern __shared__ float part[];  // [warps][latent]
+    __shared__ float lsum[32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int64_t unit = blockIdx.x;
+    const int b = static_cast<int>(unit / p.groups), g = static_cast<int>(unit % p.groups);
+    const int r = blockIdx.y, rows = p.T * p.H;
+    if (g * 64 + r >= rows) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int2 u = p.ws_unit[unit];
+    if (u.x < 0) return;
+    // piece i of CTA u.x + i: the first tile's piece in the odd slot, the others in even ones
+    auto slot_of = [&](int i) { return 2 * (u.x + i) + (i == 0 ? 1 : 0); };
+    const int pieces = u.y - u.x + 1;
+    float m = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) m = fmaxf(m, p.ws_ml[slot_of(i) * 64 + r].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float mref = m == -INFINITY ? 0.f : m;
+    const int nv = p.latent >> 7;  // float4 a lane
+    float4 acc[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll 4
+    for (int i = warp; i < pieces; i += warps) {
+        const int slot = slot_of(i);
+        const float2 ml = p.ws_ml[slot * 64 + r];
+        const float f = ex2(ml.x - mref);
+        const float4* src = reinterpret_cast<const float4*>(p.ws_o + (static_cast<int64_t>(slot) * 64 + r) * p.latent);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < nv) {
+                const float4 x = src[k * 32 + lane];
+                // a piece whose keys this row may not see has f = l = 0
+                acc[k].x = fmaf(f, x.x, acc[k].x);
+                acc[k].y = fmaf(f, x.y, acc[k].y);
+                acc[k].z = fmaf(f, x.z, acc[k].z);
+                acc[k].w = fmaf(f, x.w, acc[k].w);
+            }
+        l = fmaf(f, ml.y, l);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (k < nv) *reinterpret_cast<float4*>(part + warp * p.latent + (k * 32 + lane) * 4) = acc[k];
+    if (lane == 0) lsum[warp] = l;
+    __syncthreads();
+    float lt = 0.f;
+    for (int w = 0; w < warps; ++w) lt += lsum[w];
+    const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
+    const int64_t row = static_cast<int64_t>(b) * rows + g * 64 + r;
+    for (int d = threadIdx.x * 2; d < p.latent; d += blockDim.x * 2) {
+        float2 x = make_float2(0.f, 0.f);
+        for (int w = 0; w < warps; ++w) {
+            const float2 y = *reinterpret_cast<const float2*>(part + w * p.latent + d);
+            x.x += y.x;
+            x.y += y.y;
+        }
+        *reinterpret_cast<uint32_t*>(p.out + 2 * (row * p.latent + d)) =
+            Elem<T>::pack(inv == 0.f ? 0.f : x.x * inv, inv == 0.f ? 0.f : x.y * inv);
+    }
+    if (p.lse && threadIdx.x == 0) p.lse[row] = lt == 0.f ? -INFINITY : (m + log2f(lt)) * 0.69314718055994531f;
+}
+
+static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+template <typename T>
+static vk_status launch_latent_decode(vk_pool* pool, const LdParams& p, cudaStream_t st) {
+    static uint64_t attr_set = 0;
+    const uint64_t bit = 1ull << (pool->device & 63);
+    const size_t smem = static_cast<size_t>(p.stages + 1) * p.nch * kLdChunk + kLdChunk + kLdAux + 1024;
+    if (!(attr_set & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(latent_decode_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLdSmemMax);
+        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(latent_decode)");
+        attr_set |= bit;
+    }
+    latent_decode_kernel<T><<<pool->num_sms, kLdThreads, smem, st>>>(pool->tmap16, p);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "latent_decode_kernel launch");
+    // few rows: many pieces each, so more warps share a row's pieces
+    const int64_t units = static_cast<int64_t>(p.B) * p.groups;
+    const int rows = min(64, p.T * p.H);
+    const int warps = units * rows <= 4 * pool->num_sms ? 16 : 4;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(rows));
+    cfg.blockDim = dim3(warps * 32);
+    cfg.dynamicSmemBytes = static_cast<size_t>(warps) * p.latent * 4;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, latent_merge_kernel<T>, p);
+    return e == cudaSuccess ? VK_OK : cuda_fail(e, "latent_merge_kernel launch");
+}
+
+}  // namespace vk
+
+using namespace vk;
+
+extern "C" size_t vk_latent_decode_workspace_size(const vk_pool* pool, int32_t batch, int32_t tokens_per_seq,
+                                                  int32_t num_heads) {
+    if (!pool || !is_latent(pool) || batch <= 0 || tokens_per_seq <= 0 || num_heads <= 0) return 0;
+    const int64_t rows = static_cast<int64_t>(tokens_per_seq) * num_heads, units = batch * ((rows + 63) / 64);
+    if (rows > (1 << 20) || units > (1 << 24)) return 0;
+    const size_t slots = 2 * static_cast<size_t>(pool->num_sms);
+    return align256(slots * 64 * pool->latent_dim * 4) + align256(slots * 64 * 8) + align256(static_cast<size_t>(units) * 8);
+}
+
+extern "C" vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* q_latent, int64_t ql_token_stride,
+                                      int64_t ql_head_stride, const void* q_rope, int64_t qr_token_stride,
+                                      int64_t qr_head_stride, void* out, float* lse, const int32_t* block_tables,
+                                      int32_t bt_stride, const int32_t* seq_lens, int32_t batch, int32_t tokens_per_seq,
+                                      int32_t num_heads, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!pool) return fail(VK_INVALID_ARG, "pool is NULL");
+    if (!is_latent(pool)) return fail(VK_UNSUPPORTED, "latent decode needs a latent pool");
+    if (layer < 0 || layer >= pool->cfg.num_layers) return fail(VK_INVALID_ARG, "layer out of range");
+    if (batch < 0 || tokens_per_seq < 0 || num_heads <= 0 || bt_stride <= 0) return fail(VK_INVALID_ARG, "bad batch/tokens/heads/bt_stride");
+    if (!(scale > 0.f) || scale > 3.0e38f) return fail(VK_INVALID_ARG, "scale must be > 0 and finite");
+    if (batch == 0 || tokens_per_seq == 0) return VK_OK;
+    if (!q_latent || !q_rope || !out || !block_tables || !seq_lens) return fail(VK_INVALID_ARG, "NULL array");
+    if (((reinterpret_cast<uintptr_t>(q_latent) | reinterpret_cast<uintptr_t>(q_rope) | reinterpret_cast<uintptr_t>(out)) & 15) ||
+        ql_token_stride % 8 || ql_head_stride % 8 || qr_token_stride % 8 || qr_head_stride % 8)
+        return fail(VK_INVALID_ARG, "q_latent, q_rope and out must be 16-byte aligned, strides multiples of 8");
+    const size_t need = vk_latent_decode_workspace_size(pool, batch, tokens_per_seq, num_heads);
+    if (need == 0) return fail(VK_INVALID_ARG, "too many rows: tokens_per_seq * num_heads <= 2^20, batch * ceil(rows/64) <= 2^24");
+    if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
+        return fail(VK_INVALID_ARG, "workspace missing, too small or not 16-byte aligned");
+    LdParams p;
+    p.ql = static_cast<const char*>(q_latent);
+    p.qr = static_cast<const char*>(q_rope);
+    p.ql_token = ql_token_stride;
+    p.ql_head = ql_head_stride;
+    p.qr_token = qr_token_stride;
+    p.qr_head = qr_head_stride;
+    p.out = static_cast<char*>(out);
+    p.lse = lse;
+    p.bt = block_tables;
+    p.lens = seq_lens;
+    p.err = pool->d_err;
+    p.bt_stride = bt_stride;
+    p.B = batch;
+    p.T = tokens_per_seq;
+    p.H = num_heads;
+    p.groups = (tokens_per_seq * num_heads + 63) / 64;
+    p.layer = layer;
+    p.num_pages = pool->num_pages;
+    p.P = pool->cfg.page_tokens;
+    p.latent = pool->latent_dim;
+    p.rope = pool->rope_dim;
+    p.nch = p.latent / 64 + 1;
+    const int stage = p.nch * kLdChunk;
+    p.stages = (kLdSmemMax - 1024 - kLdAux - kLdChunk - stage) / stage;
+    if (p.stages > kLdMaxStages) p.stages = kLdMaxStages;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    const size_t slots = 2 * static_cast<size_t>(pool->num_sms);
+    char* ws = static_cast<char*>(workspace);
+    p.ws_o = reinterpret_cast<float*>(ws);
+    ws += align256(slots * 64 * p.latent * 4);
+    p.ws_ml = reinterpret_cast<float2*>(ws);
+    ws += align256(slots * 64 * 8);
+    p.ws_unit = reinterpret_cast<int2*>(ws);
+    DeviceGuard g(pool->device);
+    return pool->kv_format == VK_KV_LATENT_BF16 ? launch_latent_decode<__nv_bfloat16>(pool, p, as_stream(stream))
+                                                : launch_latent_decode<__half>(pool, p, as_stream(stream));
+}

@@ -15,6 +15,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 
 #include "vk_internal.h"
 #include "vk_fp8.cuh"
@@ -167,6 +168,32 @@ static void set_geometry(vk_pool* p) {
     }
 }
 
+// Latent pools: rows of latent_dim + rope_dim elements, page_tokens rows per
+// (layer, page); a TMA box is 64 elements (128 bytes, 128-byte swizzle) of one
+// page's rows.  Elements behind the row (rope_dim < 64) read as zeros.
+static vk_status make_latent_tmap(vk_pool* p) {
+    const uint64_t rows = static_cast<uint64_t>(p->num_pages) * p->cfg.num_layers * p->cfg.page_tokens;
+    if (rows >= (1ull << 31)) return fail(VK_UNSUPPORTED, "latent pool too large for 32-bit TMA row coordinates");
+    auto encode = tmap_encode_fn();
+    if (!encode) return fail(VK_CUDA_ERROR, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t width = static_cast<cuuint64_t>(p->latent_dim + p->rope_dim);
+    cuuint64_t dims[2] = {width, rows};
+    cuuint64_t strides[1] = {width * 2};
+    cuuint32_t box[2] = {64, static_cast<cuuint32_t>(p->cfg.page_tokens)};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = encode(&p->tmap16,
+                        p->kv_format == VK_KV_LATENT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        2, p->base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        char buf[96];
+        std::snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+        return fail(VK_CUDA_ERROR, buf);
+    }
+    p->tmap_ok = true;
+    return VK_OK;
+}
+
 static vk_status finish_create(vk_pool* p, vk_pool** out) {
     cudaError_t e = cudaMalloc(&p->d_err, sizeof(uint32_t));
     if (e != cudaSuccess) return cuda_fail(e, "cudaMalloc(error word)");
@@ -178,6 +205,10 @@ static vk_status finish_create(vk_pool* p, vk_pool** out) {
         p->num_sms = sms;
     if (p->kv && p->kv_format == VK_KV_FP16) {  // FP8 blocks are fetched with untiled bulk copies
         vk_status s = make_tmap(p);
+        if (s != VK_OK) return s;
+    }
+    if (is_latent(p)) {
+        vk_status s = make_latent_tmap(p);
         if (s != VK_OK) return s;
     }
     p->alloc.reset(p->num_pages);
@@ -281,7 +312,65 @@ vk_status vk_pool_create_fmt(const vk_pool_cfg* cfg, int32_t kv_format, void* de
                       : pool_create_owned(cfg, kv_format, out_pool);
 }
 
-int32_t vk_pool_kv_format(const vk_pool* pool) { return pool && pool->kv ? pool->kv_format : -1; }
+vk_status vk_latent_pool_create(const vk_latent_cfg* c, void* device_mem, size_t bytes, vk_pool** out_pool) {
+    if (!out_pool) return fail(VK_INVALID_ARG, "out_pool is NULL");
+    *out_pool = nullptr;
+    if (!c) return fail(VK_INVALID_ARG, "cfg is NULL");
+    if (c->num_pages <= 0 || c->num_layers <= 0) return fail(VK_INVALID_ARG, "num_layers and num_pages must be > 0");
+    if (c->dtype != VK_F16 && c->dtype != VK_BF16) return fail(VK_INVALID_ARG, "latent pages are VK_F16 or VK_BF16");
+    if (c->latent_dim <= 0 || c->latent_dim % 128 || c->latent_dim > 512)
+        return fail(VK_UNSUPPORTED, "latent_dim must be 128, 256, 384 or 512");
+    if (c->rope_dim <= 0 || c->rope_dim % 16 || c->rope_dim > 64)
+        return fail(VK_UNSUPPORTED, "rope_dim must be 16, 32, 48 or 64");
+    if (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64)
+        return fail(VK_UNSUPPORTED, "page_tokens must be 16, 32 or 64");
+    const uint64_t seg = 2ull * c->page_tokens * (c->latent_dim + c->rope_dim);
+    const uint64_t total = seg * static_cast<uint64_t>(c->num_layers) * static_cast<uint64_t>(c->num_pages);
+    if (static_cast<uint64_t>(c->num_layers) * static_cast<uint64_t>(c->num_pages) * c->page_tokens >= (1ull << 31))
+        return fail(VK_UNSUPPORTED, "latent pool too large for 32-bit TMA row coordinates");
+    if (device_mem && ((reinterpret_cast<uintptr_t>(device_mem) & 255) || bytes < total))
+        return fail(VK_INVALID_ARG, "device_mem must be 256-byte aligned and hold num_pages * page_bytes");
+    DeviceGuard g(c->device);
+    auto* p = new (std::nothrow) vk_pool();
+    if (!p) return fail(VK_INVALID_ARG, "out of host memory");
+    p->cfg.num_layers = c->num_layers;
+    p->cfg.num_kv_heads = 1;
+    p->cfg.head_dim = c->latent_dim + c->rope_dim;
+    p->cfg.page_tokens = c->page_tokens;
+    p->cfg.num_pages = c->num_pages;
+    p->cfg.device = c->device;
+    p->kv_format = c->dtype == VK_BF16 ? VK_KV_LATENT_BF16 : VK_KV_LATENT_F16;
+    p->latent_dim = c->latent_dim;
+    p->rope_dim = c->rope_dim;
+    p->device = c->device;
+    p->num_pages = c->num_pages;
+    p->page_bytes = seg * c->num_layers;
+    p->head_bytes = p->seg_bytes = seg;
+    p->nseg = c->num_layers;
+    p->seg_stride = seg * static_cast<uint64_t>(c->num_pages);
+    p->base = static_cast<char*>(device_mem);
+    vk_status s = VK_OK;
+    if (!device_mem) {
+        cudaError_t e = cudaMalloc(&p->base, total);
+        if (e == cudaSuccess) {
+            p->owns_mem = true;
+            e = cudaMemset(p->base, 0, total);
+        }
+        if (e != cudaSuccess) s = cuda_fail(e, "cudaMalloc(latent pool)");
+    }
+    if (s == VK_OK) s = finish_create(p, out_pool);
+    if (s != VK_OK) {
+        if (p->d_err) cudaFree(p->d_err);
+        if (p->owns_mem) cudaFree(p->base);
+        delete p;
+        *out_pool = nullptr;
+    }
+    return s;
+}
+
+int32_t vk_pool_kv_format(const vk_pool* pool) {
+    return pool && (pool->kv || is_latent(pool)) ? pool->kv_format : -1;
+}
 
 vk_status vk_pool_destroy(vk_pool* pool) {
     if (!pool) return VK_OK;

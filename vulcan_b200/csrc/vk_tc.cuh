@@ -114,4 +114,10 @@ __device__ __forceinline__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) 
     return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
+// Instruction descriptor, kind::f16, fp32 accumulate, M x N: 16-bit type of A
+// and B (bf16 or fp16), each K-major (mn = 0) or MN-major (mn = 1).
+__device__ __forceinline__ constexpr uint32_t idesc_16(bool bf16, uint32_t m, uint32_t n, uint32_t a_mn, uint32_t b_mn) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn << 15) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
 }  // namespace vk

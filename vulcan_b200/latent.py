@@ -1,0 +1,273 @@
+"""Rotary positions and the latent cache over the C ABI (include/vk_paged_kv.h).
+
+* ``RotaryEmbedding`` — vk_rotary: q and k rotated in one launch, interleaved or
+  half layout, the leading part of a head, frequencies scaled for long contexts.
+* ``LatentKVPool`` — vk_latent: a paged cache of one latent vector and one shared
+  rotary key part a token, its append (norm and rotation fused) and its
+  attention in the absorbed form (decode).  The page operations
+  of ``PagedKVPool`` (alloc, free, copy, compaction, swap) work on it unchanged.
+
+No reference counterpart: the reference has neither.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import List, Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import check
+from .paged_kv import PAGE_TOKENS, PagedKVPool
+
+DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # VK_F16, VK_BF16, VK_F32
+LAYOUTS = {"interleaved": 0, "half": 1}
+SCALINGS = {None: 0, "linear": 1, "by_parts": 2, "by_wavelength": 3}
+
+
+def _device(device) -> torch.device:
+    if isinstance(device, torch.device) and device.index is not None:
+        return device
+    return torch.device("cuda", torch.cuda.current_device() if device is None or isinstance(device, torch.device)
+                        else int(device))
+
+
+def _stream_of(stream, device: torch.device) -> int:
+    if stream is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
+
+
+def _empty(shape, dtype, device: torch.device, stream) -> torch.Tensor:
+    """Memory for a call on ``stream``: allocated on that stream, so the caching allocator hands it out again only
+    behind the call (and a captured call keeps its own)."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), device=device)
+    with torch.cuda.stream(s):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _on(t: torch.Tensor, dtype, name: str, device: torch.device) -> None:
+    if t.dtype != dtype:
+        raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
+    if t.device != device:
+        raise ValueError("%s must be on %s, got %s" % (name, device, t.device))
+
+
+def _i32(t: torch.Tensor, name: str, device: torch.device, numel: int) -> int:
+    _on(t, torch.int32, name, device)
+    if not t.is_contiguous() or t.numel() != numel:
+        raise ValueError("%s must be contiguous with %d elements" % (name, numel))
+    return t.data_ptr()
+
+
+def _tables(t: torch.Tensor, device: torch.device) -> int:
+    """Rows of the block tables; returns the batch."""
+    _on(t, torch.int32, "block_tables", device)
+    if t.dim() != 2 or not t.is_contiguous():
+        raise ValueError("block_tables must be a contiguous [batch, width] tensor")
+    return t.shape[0]
+
+
+def _token_head(t: torch.Tensor, name: str) -> Tuple[int, int]:
+    """(token, head) strides of [tokens, heads, d] or [batch, tokens, heads, d] with unit stride along d and, in
+    the second form, batches that follow one another."""
+    s, n = t.stride(), t.dim()
+    if n not in (3, 4) or (s[-1] != 1 and t.shape[-1] > 1):
+        raise ValueError("%s must be [tokens, heads, d] or [batch, tokens, heads, d] with unit stride along d" % name)
+    if n == 4 and t.shape[0] > 1 and t.shape[1] > 1 and s[0] != s[1] * t.shape[1]:
+        raise ValueError("%s: the batches of a 4-D view must follow one another (stride 0 = stride 1 * tokens)" % name)
+    return (s[0] if n == 4 and t.shape[1] == 1 else s[-3]), s[-2]
+
+
+class RotaryEmbedding:
+    """Rotary positions (vk_rotary, see the C header for the scalings).
+
+    ``rotary_dim`` leading elements of each head turn by position * f_i, with
+    pairs (2i, 2i+1) (``layout="interleaved"``) or (i, i + rotary_dim/2)
+    (``"half"``)."""
+
+    def __init__(self, rotary_dim: int, theta: float = 10000.0, layout: str = "interleaved", scaling: Optional[str] = None,
+                 factor: float = 1.0, original_len: float = 0.0, low: float = 1.0, high: float = 32.0,
+                 magnitude: float = 0.0, device=None):
+        if layout not in LAYOUTS:
+            raise ValueError("layout must be one of %s" % sorted(LAYOUTS))
+        if scaling not in SCALINGS:
+            raise ValueError("scaling must be one of %s" % list(SCALINGS))
+        self._lib = _lib.load()
+        self.rotary_dim, self.layout, self.scaling = rotary_dim, layout, scaling
+        # frequencies alone need no GPU: the device is looked up by the first apply
+        self._cfg = _lib.VkRotaryCfg(rotary_dim, LAYOUTS[layout], SCALINGS[scaling], 0, theta, factor, original_len, low,
+                                     high, magnitude)
+        self.frequencies()
+        self.handle = ctypes.c_void_p()
+        self.device = _device(device) if torch.cuda.is_available() else torch.device("cpu")
+        self._cfg.device = self.device.index or 0
+        check(self._lib.vk_rotary_create(ctypes.byref(self._cfg), ctypes.byref(self.handle)), "vk_rotary_create")
+
+    def frequencies(self) -> Tuple[List[float], float]:
+        """(radians per position of each pair, factor on cos and sin), scaled, in double precision."""
+        f = (ctypes.c_double * max(1, self.rotary_dim // 2))()
+        m = ctypes.c_double()
+        check(self._lib.vk_rotary_frequencies(ctypes.byref(self._cfg), f, ctypes.byref(m)), "vk_rotary_frequencies")
+        return list(f), m.value
+
+    def apply(self, q: torch.Tensor, positions: torch.Tensor, k: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, out_k: Optional[torch.Tensor] = None, stream=None):
+        """q, k: [tokens, heads, D] (or [batch, tokens, heads, D]) fp16, bf16 or fp32, strided views allowed;
+        positions: int32, one per token.  Returns the rotated q, or (q, k).  ``out``/``out_k`` may be q/k
+        themselves: rotated in place."""
+        dev = self.device
+        if q.dtype not in DTYPES:
+            raise TypeError("q must be fp16, bf16 or fp32, got %s" % q.dtype)
+        d, tokens = q.shape[-1], q.numel() // max(1, q.shape[-1] * q.shape[-2]) if q.dim() > 2 else -1
+        got, views = [], []
+        for x, y, name in ((q, out, "q"), (k, out_k, "k")):
+            if x is None:
+                continue
+            v = _lib.VkRotaryView()
+            _on(x, q.dtype, name, dev)
+            v.x_token, v.x_head = _token_head(x, name)
+            if x.shape[-1] != d or x.shape[:-2] != q.shape[:-2]:
+                raise ValueError("q and k must have the same tokens and head dimension")
+            if y is None:
+                y = _empty(x.shape, x.dtype, dev, stream)
+            else:
+                _on(y, q.dtype, "out", dev)
+                if y.shape != x.shape:
+                    raise ValueError("out must have the shape of its input")
+            v.y_token, v.y_head = _token_head(y, "out")
+            v.x, v.y, v.heads = x.data_ptr(), y.data_ptr(), x.shape[-2]
+            got.append(y)
+            views.append(v)
+        check(self._lib.vk_rotary_apply(self.handle, DTYPES[q.dtype], views[0], views[1] if k is not None else None, d,
+                                        _i32(positions, "positions", dev, tokens), tokens, _stream_of(stream, dev)),
+              "vk_rotary_apply")
+        return got[0] if k is None else tuple(got)
+
+    def close(self) -> None:
+        if getattr(self, "handle", None) is not None and self.handle.value:
+            self._lib.vk_rotary_destroy(self.handle)
+            self.handle = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class LatentKVPool(PagedKVPool):
+    """A paged cache of rows [latent | rotary key part] (vk_latent_pool_create).
+
+    Storage: ``[num_layers, num_pages, page_tokens, latent_dim + rope_dim]`` of
+    ``dtype`` (fp16 or bf16): a torch allocation, ``storage`` when given (a
+    contiguous CUDA tensor of that size), or the library's own memory with
+    ``own_memory``."""
+
+    def __init__(self, num_layers: int, latent_dim: int, rope_dim: int, num_pages: int, page_tokens: int = PAGE_TOKENS,
+                 dtype: torch.dtype = torch.float16, device=None, own_memory: bool = False, zero: bool = True,
+                 storage: Optional[torch.Tensor] = None):
+        self._lib = _lib.load()
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError("dtype must be torch.float16 or torch.bfloat16")
+        self.handle = None
+        self.device = storage.device if storage is not None else _device(device)
+        self.num_layers, self.num_pages, self.page_tokens, self.dtype = num_layers, num_pages, page_tokens, dtype
+        self.latent_dim, self.rope_dim, self.width = latent_dim, rope_dim, latent_dim + rope_dim
+        self.num_kv_heads, self.head_dim, self.kv, self.kv_format = 1, self.width, False, "latent"
+        self.block_bytes = 2 * page_tokens * self.width
+        self.page_bytes = num_layers * self.block_bytes
+        total = self.page_bytes * num_pages
+        if storage is not None:
+            if not storage.is_cuda or not storage.is_contiguous() or storage.numel() * storage.element_size() != total:
+                raise ValueError("storage must be a contiguous CUDA tensor of %d bytes" % total)
+            self.storage = storage
+        elif own_memory:
+            self.storage = None
+        else:
+            self.storage = (torch.zeros if zero else torch.empty)(max(0, total), dtype=torch.uint8, device=self.device)
+        cfg = _lib.VkLatentCfg(num_layers, latent_dim, rope_dim, page_tokens, num_pages, self.device.index, DTYPES[dtype])
+        handle = ctypes.c_void_p()
+        check(self._lib.vk_latent_pool_create(ctypes.byref(cfg), None if own_memory and storage is None
+                                              else ctypes.c_void_p(self.storage.data_ptr()), total, ctypes.byref(handle)),
+              "vk_latent_pool_create")
+        self.handle = handle
+
+    def latent_view(self) -> torch.Tensor:
+        """View [L, num_pages, page_tokens, latent_dim + rope_dim] of the pool."""
+        if self.storage is None:
+            raise RuntimeError("latent_view needs a torch-backed pool")
+        return self.storage.view(torch.uint8).view(self.dtype).view(self.num_layers, self.num_pages, self.page_tokens, self.width)
+
+    def append(self, layer: int, latent: torch.Tensor, k_rope: torch.Tensor, block_tables: torch.Tensor,
+               positions: torch.Tensor, offsets: Optional[torch.Tensor] = None, norm_weight: Optional[torch.Tensor] = None,
+               eps: float = 1e-6, rope: Optional[RotaryEmbedding] = None, stream=None) -> None:
+        """latent [tokens, latent_dim], k_rope [tokens, rope_dim] (row-strided views); sequence b takes the rows
+        offsets[b]..offsets[b+1]-1 (None: the same number each) from position positions[b] on.  ``norm_weight``: root
+        mean square norm of the latent first; ``rope``: k_rope rotated at its position."""
+        dev = self.device
+        batch = _tables(block_tables, dev)
+        for t, name, d in ((latent, "latent", self.latent_dim), (k_rope, "k_rope", self.rope_dim)):
+            _on(t, self.dtype, name, dev)
+            if t.dim() != 2 or t.shape[1] != d or t.stride(1) != 1:
+                raise ValueError("%s must be [tokens, %d] with unit stride along its rows" % (name, d))
+        tokens = latent.shape[0]
+        if k_rope.shape[0] != tokens:
+            raise ValueError("latent and k_rope must have the same tokens")
+        if norm_weight is not None:
+            _on(norm_weight, self.dtype, "norm_weight", dev)
+            if norm_weight.numel() != self.latent_dim or not norm_weight.is_contiguous():
+                raise ValueError("norm_weight must be contiguous with %d elements" % self.latent_dim)
+        check(self._lib.vk_latent_append(
+            self.handle, layer, latent.data_ptr(), latent.stride(0), k_rope.data_ptr(), k_rope.stride(0),
+            None if norm_weight is None else norm_weight.data_ptr(), eps, None if rope is None else rope.handle,
+            block_tables.data_ptr(), block_tables.shape[1], _i32(positions, "positions", dev, batch),
+            None if offsets is None else _i32(offsets, "offsets", dev, batch + 1), batch, tokens, _stream_of(stream, dev)),
+            "vk_latent_append")
+
+    def decode_workspace_size(self, batch: int, tokens_per_seq: int, num_heads: int) -> int:
+        return self._lib.vk_latent_decode_workspace_size(self.handle, batch, tokens_per_seq, num_heads)
+
+    def decode(self, layer: int, q_latent: torch.Tensor, q_rope: torch.Tensor, block_tables: torch.Tensor,
+               seq_lens: torch.Tensor, scale: float, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+               return_lse: bool = False, workspace: Optional[torch.Tensor] = None, stream=None):
+        """Absorbed form.  q_latent [B, H, latent_dim] or [B, T, H, latent_dim], q_rope likewise with rope_dim
+        (rotated; strided views allowed); seq_lens [B] int32: rows to attend, the T new ones included (query token t
+        sees seq_lens[b] - (T-1-t)).  Returns out like q_latent, or (out, lse)."""
+        dev = self.device
+        batch = _tables(block_tables, dev)
+        _on(q_latent, self.dtype, "q_latent", dev)
+        _on(q_rope, self.dtype, "q_rope", dev)
+        if q_latent.dim() not in (3, 4) or q_latent.shape[:-1] != q_rope.shape[:-1] or q_latent.shape[0] != batch or \
+                q_latent.shape[-1] != self.latent_dim or q_rope.shape[-1] != self.rope_dim:
+            raise ValueError("q_latent must be [B, (T,) H, %d] and q_rope [B, (T,) H, %d]" % (self.latent_dim, self.rope_dim))
+        tokens, heads = (q_latent.shape[1] if q_latent.dim() == 4 else 1), q_latent.shape[-2]
+        lt, lh = _token_head(q_latent, "q_latent")
+        rt, rh = _token_head(q_rope, "q_rope")
+        if out is None:
+            out = _empty(q_latent.shape, self.dtype, dev, stream)
+        else:
+            _on(out, self.dtype, "out", dev)
+            if out.shape != q_latent.shape or not out.is_contiguous():
+                raise ValueError("out must be contiguous with the shape of q_latent")
+        if lse is not None:
+            _on(lse, torch.float32, "lse", dev)
+            if lse.shape != q_latent.shape[:-1] or not lse.is_contiguous():
+                raise ValueError("lse must be contiguous [B, (T,) H]")
+        elif return_lse:
+            lse = _empty(q_latent.shape[:-1], torch.float32, dev, stream)
+        ws = workspace if workspace is not None else _empty((self.decode_workspace_size(batch, tokens, heads),), torch.uint8,
+                                                            dev, stream)
+        check(self._lib.vk_latent_decode(
+            self.handle, layer, q_latent.data_ptr(), lt, lh, q_rope.data_ptr(), rt, rh, out.data_ptr(),
+            None if lse is None else lse.data_ptr(), block_tables.data_ptr(), block_tables.shape[1],
+            _i32(seq_lens, "seq_lens", dev, batch), batch, tokens, heads, scale, ws.data_ptr(),
+            ws.numel() * ws.element_size(), _stream_of(stream, dev)), "vk_latent_decode")
+        return (out, lse) if return_lse else out
+
+    def plan(self, *args, **kwargs):
+        raise TypeError("a latent pool has no planned decode: use decode")
+
+    workspace = workspace_size = pages_per_split = set_split = set_rope = set_plan_workers = set_prefill_path = plan
