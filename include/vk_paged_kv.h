@@ -490,6 +490,33 @@ vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* q_latent, i
                            int32_t bt_stride, const int32_t* seq_lens, int32_t batch, int32_t tokens_per_seq,
                            int32_t num_heads, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention in the expanded form, for chunks of new tokens (append them first):
+ * keys [W_k,h c | r] and values W_v,h c of 128 (+ rope_dim) elements a head are
+ * made from the cached rows in the workspace, then attended causally: chunk
+ * token i of sequence b sits at positions[b]+i and sees rows 0..positions[b]+i.
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,   scale 0: 1/sqrt(128 + rope_dim)
+ * Token rows come concatenated, with offsets as in vk_latent_append; rows
+ * behind offsets[batch] are left as they were.  q: [tokens, num_heads, 128 +
+ * rope_dim] by strides in elements, its last rope_dim elements rotated already;
+ * w_kv: [num_heads * 256, latent_dim], row stride w_stride, per head the 128
+ * rows of W_k,h, then the 128 of W_v,h (an [out, in] projection weight as it
+ * is); out: [tokens, num_heads, 128].  All of the pool's type, 16-byte aligned,
+ * strides multiples of 8.
+ * max_tokens and max_seq_len bound the longest chunk and the longest sequence
+ * after it, on the host (they size the launches and the workspace); a sequence
+ * beyond them, or beyond its table, records VK_ERR_SEQ_LEN and is left out.
+ * workspace: vk_latent_prefill_workspace_size() bytes (512 a token and head, in
+ * groups of heads of up to 1 GiB), 128-byte aligned; calls that may overlap on
+ * the GPU need one each.  From ~170 new tokens a sequence on this does less work
+ * than vk_latent_decode at latent_dim 512. */
+size_t    vk_latent_prefill_workspace_size(const vk_pool* pool, int32_t batch, int32_t max_seq_len, int32_t num_heads);
+vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void* q, int64_t q_token_stride,
+                            int64_t q_head_stride, const void* w_kv, int64_t w_stride, void* out,
+                            const int32_t* block_tables, int32_t bt_stride, const int32_t* positions,
+                            const int32_t* offsets, int32_t batch, int32_t tokens, int32_t max_tokens,
+                            int32_t max_seq_len, int32_t num_heads, float scale, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* ---- K3: chunked prefill -------------------------------------------------
  * The prefill use of launch_attention (src/transformer.cpp:136-189 with
  * num_tokens = chunk, src/engine.cpp:70-101): query token t of sequence b sits

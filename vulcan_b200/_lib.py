@@ -124,6 +124,9 @@ SIGNATURES = {
     "vk_latent_decode_workspace_size": (c_sz, [vp, c_i32, c_i32, c_i32]),
     "vk_latent_decode": (c_i32, [vp, c_i32, vp, c_i64, c_i64, vp, c_i64, c_i64, vp, vp, vp, c_i32, vp, c_i32, c_i32,
                                  c_i32, c_f32, vp, c_sz, vp]),
+    "vk_latent_prefill_workspace_size": (c_sz, [vp, c_i32, c_i32, c_i32]),
+    "vk_latent_prefill": (c_i32, [vp, c_i32, vp, c_i64, c_i64, vp, c_i64, vp, vp, c_i32, vp, vp, c_i32, c_i32, c_i32,
+                                  c_i32, c_i32, c_f32, vp, c_sz, vp]),
     "vk_last_error_string": (ctypes.c_char_p, []),
     "vk_status_string": (ctypes.c_char_p, [c_i32]),
     "vk_version": (c_i32, []),

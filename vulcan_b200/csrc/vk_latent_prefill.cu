@@ -1,0 +1,659 @@
+// Latent attention, expanded form (vk_latent_prefill): a chunk of new tokens
+// over the latent cache, with keys and values per head
+//
+//   k_h,j = [W_k,h c_j | r_j]  (128 + rope elements),  v_h,j = W_v,h c_j  (128)
+//   out_t = sum_{j <= pos_t} softmax_j(scale * q_t . k_j) v_j
+//
+// A (query, key, head) triple costs 2 * (256 + rope) flop here against
+// 2 * (2 latent + rope) absorbed (640 and 2,176 at 512 + 64), and a cached token
+// and head 2 * 256 * latent once for the expansion: from ~170 new tokens on the
+// expanded form does less.  Two kernels per group of heads:
+//
+//  * latent_expand_kernel: [128 cached tokens] x [one head's 256 rows of W] as a
+//    tcgen05 GEMM.  The 128 gathered latent rows stay in shared memory (128 KiB
+//    at 512) for all heads of the CTA; W streams through a ring of 32 KiB
+//    stages; two TMEM accumulators of 256 columns, so a head is stored while the
+//    next one multiplies.  Output rows [token][head][128 K | 128 V] in the
+//    workspace, rounded to the cache's 16-bit type (relative 2^-9 or 2^-12 of
+//    each element, as a cache of keys and values holds them); rows behind the
+//    sequence are stored as zeros, so the attention reads no stale bytes.
+//  * latent_prefill_kernel: causal attention, one CTA per (256 query rows, head,
+//    sequence): the rows are two 128-row tiles whose softmax steps alternate on
+//    one tensor core (S_A, S_B, then P V of one tile while the other's softmax
+//    runs), P in TMEM as the A operand.  K and V move through one ring of eight
+//    16 KiB units (128 keys x 64 elements): a key tile takes three for K (two of
+//    W_k c from the workspace, one of r from the pages) and two for V.  K and V
+//    of whole 32 + 16 KiB tiles would not fit twice beside 96 KiB of queries;
+//    units let the next K load while the last V is read.
+#include "vk_internal.h"
+#include "vk_latent.cuh"
+#include "vk_ptx.cuh"
+#include "vk_rotary.cuh"
+#include "vk_tc.cuh"
+
+namespace vk {
+
+constexpr int kLpKeys = 128;
+constexpr int kLpRows = 128;           // rows of a tile; a CTA has two
+constexpr int kLpHead = 128;           // elements of W_k,h c and of v
+constexpr int kLpUnit = kLpKeys * 128;  // 16 KiB
+constexpr int kLpSmemMax = 232448;
+
+struct LpParams {
+    const int32_t* bt;
+    const int32_t* pos;
+    const int32_t* offsets;  // NULL: tokens / B each
+    uint32_t* err;
+    char* ws;     // [B * lpad][heads][256]
+    char* out;    // [tokens][H][128]
+    int bt_stride, B, tokens, H, heads, h0, layer, num_pages, P, latent, rope, lpad, max_tokens, max_len, stages, per_cta;
+    float scale_log2;
+};
+
+struct LpSeq {
+    int row0, n, pos;  // first row of the chunk, its tokens, position of its first token
+};
+
+// The chunk of sequence b; n = 0 when there is nothing to do or the arguments
+// are out of range (recorded by the caller's `record` thread).
+__device__ __forceinline__ LpSeq lp_seq(const LpParams& p, int b, bool record) {
+    LpSeq s;
+    int64_t end;
+    if (p.offsets) {
+        s.row0 = __ldg(p.offsets + b);
+        end = __ldg(p.offsets + b + 1);
+    } else {
+        const int per = p.tokens / p.B;
+        s.row0 = b * per;
+        end = s.row0 + per;
+    }
+    s.pos = __ldg(p.pos + b);
+    const int64_t n = end - s.row0;
+    s.n = static_cast<int>(n);
+    if (n <= 0 || s.row0 < 0 || end > p.tokens || n > p.max_tokens || s.pos < 0 || s.pos + n > p.max_len ||
+        s.pos + n > static_cast<int64_t>(p.bt_stride) * p.P) {
+        if (n != 0 && record) atomicOr(p.err, VK_ERR_SEQ_LEN);
+        s.n = 0;
+    }
+    return s;
+}
+
+// ------------------------------------------------------------------ expansion
+
+constexpr int kLeThreads = 192;   // 4 epilogue warps, TMA warp, MMA warp
+constexpr int kLeStage = 32768;   // 256 rows of W x 64
+constexpr int kLeMaxStages = 6;
+
+template <typename T>
+__global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __grid_constant__ CUtensorMap tmap,
+                                                                      const __grid_constant__ CUtensorMap tmapw,
+                                                                      const __grid_constant__ LpParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_u32(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.z, kt = blockIdx.y;
+    const LpSeq sq = lp_seq(p, b, threadIdx.x == 0 && blockIdx.x == 0 && kt == 0 && p.h0 == 0);
+    const int len = sq.pos + sq.n;
+    if (sq.n == 0 || kt * kLpKeys >= len) return;
+    const int hfirst = blockIdx.x * p.per_cta, nh = min(p.per_cta, p.heads - hfirst);
+    const int lch = p.latent >> 6;
+    const uint32_t s_b = sbase + lch * kLpUnit;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + lch * kLpUnit + p.stages * kLeStage);
+    uint64_t* a_full = bars;             // [8]
+    uint64_t* b_full = bars + 8;         // [stages]
+    uint64_t* b_empty = b_full + kLeMaxStages;
+    uint64_t* acc_full = b_empty + kLeMaxStages;  // [2]
+    uint64_t* acc_empty = acc_full + 2;           // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&a_full[i]), 1);
+        for (int i = 0; i < p.stages; ++i) {
+            mbar_init(smem_u32(&b_full[i]), 1);
+            mbar_init(smem_u32(&b_empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&acc_full[i]), 1);
+            mbar_init(smem_u32(&acc_empty[i]), 4);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 5) {
+        tmem_alloc(smem_u32(tmem_slot), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 4) {
+        const uint64_t pol = l2_evict_last_policy();
+        const int cnt = min(kLpKeys / p.P, (len + p.P - 1) / p.P - kt * (kLpKeys / p.P));
+        int page = 0;
+        if (lane < cnt) {
+            page = __ldg(p.bt + static_cast<int64_t>(b) * p.bt_stride + kt * (kLpKeys / p.P) + lane);
+            if (page < 0 || page >= p.num_pages) {
+                atomicOr(p.err, VK_ERR_PAGE_ID);
+                page = 0;
+            }
+        }
+        bool ok = true;
+        auto load_b = [&](int it) {
+            const int st = it % p.stages;
+            if (it >= p.stages) ok = mbar_wait(smem_u32(&b_empty[st]), (it / p.stages - 1) & 1, p.err);
+            if (!ok) return;
+            const uint32_t bar = smem_u32(&b_full[st]);
+            mbar_expect_tx(bar, kLeStage);
+            tma_load_2d(s_b + st * kLeStage, &tmapw, (it % lch) * 64, (p.h0 + hfirst + it / lch) * 256, bar, pol);
+        };
+        const int total = nh * lch, lead = min(p.stages, total);
+        if (lane == 0) {
+            prefetch_tmap(&tmapw);
+            for (int it = 0; it < lead; ++it) load_b(it);
+            for (int c = 0; c < lch; ++c) mbar_expect_tx(smem_u32(&a_full[c]), cnt * p.P * 128);
+        }
+        __syncwarp();
+        for (int c = 0; c < lch; ++c)
+            if (lane < cnt)
+                tma_load_2d(sbase + c * kLpUnit + lane * p.P * 128, &tmap, c * 64, (p.layer * p.num_pages + page) * p.P,
+                            smem_u32(&a_full[c]), pol);
+        if (lane == 0)
+            for (int it = lead; it < total && ok; ++it) load_b(it);
+    } else if (warp == 5) {
+        if (lane == 0) {
+            constexpr uint32_t id = idesc_16(Elem<T>::kBf16, 128, 256, 0, 0);
+            bool ok = true;
+            int it = 0;
+            for (int h = 0; h < nh && ok; ++h) {
+                const int buf = h & 1;
+                if (h >= 2) ok = mbar_wait(smem_u32(&acc_empty[buf]), ((h >> 1) - 1) & 1, p.err);
+                for (int c = 0; c < lch && ok; ++c, ++it) {
+                    const int st = it % p.stages;
+                    if (h == 0) ok = mbar_wait(smem_u32(&a_full[c]), 0, p.err);
+                    ok = ok && mbar_wait(smem_u32(&b_full[st]), (it / p.stages) & 1, p.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t da = umma_desc_sw128(sbase + c * kLpUnit, 16, 1024);
+                    const uint64_t db = umma_desc_sw128(s_b + st * kLeStage, 16, 1024);
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        umma_ss(tmem + buf * 256, da + ((ks * 32) >> 4), db + ((ks * 32) >> 4), id, (c | ks) != 0);
+                    umma_commit(smem_u32(&b_empty[st]));
+                }
+                if (ok) umma_commit(smem_u32(&acc_full[buf]));
+            }
+        }
+    } else {
+        const int r = warp * 32 + lane;
+        const bool inside = kt * kLpKeys + r < len;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+        const int64_t row = static_cast<int64_t>(b) * p.lpad + kt * kLpKeys + r;
+        for (int h = 0; h < nh; ++h) {
+            const int buf = h & 1;
+            if (!wait_all(smem_u32(&acc_full[buf]), (h >> 1) & 1, p.err)) break;
+            tc_fence_after();
+            char* dst = p.ws + 2 * ((row * p.heads + hfirst + h) * 256);
+            // a key whose every element is NaN or infinite comes from such a latent;
+            // rows that may not see it multiply its value by a weight of zero, so
+            // its value is stored as zeros (rows that see it get their NaN through S)
+            bool bad = true;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                float v[32];
+                tmem_ld32(lane_base + buf * 256 + c * 32, v);
+                tmem_wait_ld();
+                if (c < 4) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) bad = bad && !(fabsf(v[i]) <= 3.4028234e38f);
+                } else if (bad) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = fabsf(v[i]) <= 3.4028234e38f ? v[i] : 0.f;
+                }
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = inside ? Elem<T>::pack(v[2 * i], v[2 * i + 1]) : 0u;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c * 64 + i * 32),
+                                 "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]), "r"(w[8 * i + 3]), "r"(w[8 * i + 4]),
+                                 "r"(w[8 * i + 5]), "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
+                                 : "memory");
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&acc_empty[buf]));
+        }
+    }
+    __syncthreads();
+    if (warp == 5) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ------------------------------------------------------------------ attention
+
+constexpr int kLaThreads = 320;
+constexpr int kLaQ = 0;                              // [2 tiles][3 chunks][128 rows][128 B]
+constexpr int kLaRing = 2 * 3 * kLpUnit;             // 96 KiB
+constexpr int kLaUnits = 8;
+constexpr int kLaBar = kLaRing + kLaUnits * kLpUnit;  // 224 KiB
+constexpr int kLaSmem = kLaBar + 256 + 1024;
+static_assert(kLaSmem <= kLpSmemMax, "latent prefill shared memory");
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __grid_constant__ CUtensorMap tmap,
+                                                                       const __grid_constant__ CUtensorMap tmapq,
+                                                                       const __grid_constant__ CUtensorMap tmapkv,
+                                                                       const __grid_constant__ LpParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_u32(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.z, hl = blockIdx.y, h = p.h0 + hl;
+    const LpSeq sq = lp_seq(p, b, false);
+    const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * kLpRows;  // most keys first
+    if (q0 >= sq.n) return;
+    const int pos0 = sq.pos;
+    const int rowsA = min(kLpRows, sq.n - q0), rowsB = max(0, min(kLpRows, sq.n - q0 - kLpRows));
+    const int lenA = pos0 + q0 + rowsA, lenB = rowsB > 0 ? pos0 + q0 + kLpRows + rowsB : 0;
+    const int ntA = (lenA + kLpKeys - 1) / kLpKeys, ntB = (lenB + kLpKeys - 1) / kLpKeys;
+    const int kv_len = max(lenA, lenB), ntiles = max(ntA, ntB);
+
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kLaBar);
+    uint64_t* k_full = bars;       // [2] the three K units of a tile landed
+    uint64_t* v_full = bars + 2;   // [2]
+    // even and odd key tiles have barriers of their own: the tile after the one the
+    // producer waits for may complete first, and one barrier would then be a phase ahead
+    uint64_t* k_empty = bars + 4;  // [2] both row tiles' S of a key tile done
+    uint64_t* v_empty = bars + 6;  // [2]
+    uint64_t* s_full = bars + 8;   // [row tile]
+    uint64_t* p_full = bars + 10;  // [row tile]
+    uint64_t* o_full = bars + 12;  // [row tile]
+    uint64_t* q_full = bars + 14;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 10; ++i) mbar_init(smem_u32(&bars[i]), 1);
+        mbar_init(smem_u32(&p_full[0]), 4);
+        mbar_init(smem_u32(&p_full[1]), 4);
+        mbar_init(smem_u32(&o_full[0]), 1);
+        mbar_init(smem_u32(&o_full[1]), 1);
+        mbar_init(smem_u32(q_full), 1);
+        mbar_fence_init();
+        // rows past the chunk read the next rows of q or zeros and are not stored
+        prefetch_tmap(&tmapq);
+        mbar_expect_tx(smem_u32(q_full), 2 * 3 * kLpUnit);
+        const uint64_t pol = l2_evict_first_policy();
+        for (int t = 0; t < 2; ++t)
+            for (int c = 0; c < 3; ++c)
+                tma_load_3d(sbase + kLaQ + (t * 3 + c) * kLpUnit, &tmapq, c * 64, h, sq.row0 + q0 + t * kLpRows,
+                            smem_u32(q_full), pol);
+    }
+    if (warp == 9) {
+        tmem_alloc(smem_u32(tmem_slot), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 8) {
+        // ------------------------------------------------------------ TMA producer
+        const uint64_t pol = l2_evict_last_policy();  // other row tiles read the same K and V
+        const int32_t* btrow = p.bt + static_cast<int64_t>(b) * p.bt_stride;
+        const int npages = (kv_len + p.P - 1) / p.P, ppt = kLpKeys / p.P;
+        const int wrow = b * p.lpad;
+        bool ok = true;
+        for (int j = 0; j < ntiles && ok; ++j) {
+            int page = 0;  // a page of the tile's rotary parts per lane
+            const int cnt = min(ppt, npages - j * ppt);
+            if (lane < cnt) {
+                page = __ldg(btrow + j * ppt + lane);
+                if (page < 0 || page >= p.num_pages) {
+                    atomicOr(p.err, VK_ERR_PAGE_ID);
+                    page = 0;
+                }
+            }
+            // units 5j .. 5j+2 take the ring slots of tile j-2's last K unit and its V,
+            // units 5j+3, 5j+4 those of tile j-1's first two K units
+            if (j >= 2) ok = wait_all(smem_u32(&v_empty[j & 1]), ((j >> 1) - 1) & 1, p.err);
+            if (!ok) break;
+            const uint32_t kbar = smem_u32(&k_full[j & 1]);
+            if (lane == 0) {
+                mbar_expect_tx(kbar, 2 * kLpUnit + cnt * p.P * 128);
+                for (int u = 0; u < 2; ++u)
+                    tma_load_2d(sbase + kLaRing + ((5 * j + u) & 7) * kLpUnit, &tmapkv, hl * 256 + u * 64, wrow + j * kLpKeys,
+                                kbar, pol);
+            }
+            __syncwarp();
+            if (lane < cnt)
+                tma_load_2d(sbase + kLaRing + ((5 * j + 2) & 7) * kLpUnit + lane * p.P * 128, &tmap, p.latent,
+                            (p.layer * p.num_pages + page) * p.P, kbar, pol);
+            if (j >= 1) ok = wait_all(smem_u32(&k_empty[(j - 1) & 1]), ((j - 1) >> 1) & 1, p.err);
+            if (ok && lane == 0) {
+                const uint32_t vbar = smem_u32(&v_full[j & 1]);
+                mbar_expect_tx(vbar, 2 * kLpUnit);
+                for (int u = 0; u < 2; ++u)
+                    tma_load_2d(sbase + kLaRing + ((5 * j + 3 + u) & 7) * kLpUnit, &tmapkv, hl * 256 + kLpHead + u * 64,
+                                wrow + j * kLpKeys, vbar, pol);
+            }
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc_16(Elem<T>::kBf16, 128, 128, 0, 0);
+            constexpr uint32_t id_pv = idesc_16(Elem<T>::kBf16, 128, 64, 0, 1);
+            bool ok = mbar_wait(smem_u32(q_full), 0, p.err);
+            tc_fence_after();
+            const int nt[2] = {ntA, ntB};
+            int k_waited = -1, v_waited = -1;
+            const int rsteps = p.rope >> 4;
+            const uint64_t dq0 = umma_desc_sw128(sbase + kLaQ, 16, 1024);
+            const uint64_t dr0 = umma_desc_sw128(sbase + kLaRing, 16, 1024);
+            auto issue_s = [&](int t, int j) {
+                if (j > k_waited) {
+                    ok = ok && mbar_wait(smem_u32(&k_full[j & 1]), (j >> 1) & 1, p.err);
+                    k_waited = j;
+                }
+                if (!ok) return;
+                tc_fence_after();
+                const uint64_t dq = dq0 + static_cast<uint64_t>(t * 3 * (kLpUnit >> 4));
+                const uint32_t d = tmem + t * 128;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint64_t dk = dr0 + static_cast<uint64_t>(((5 * j + u) & 7) * (kLpUnit >> 4));
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        umma_ss(d, dq + u * (kLpUnit >> 4) + ((ks * 32) >> 4), dk + ((ks * 32) >> 4), id_s, (u | ks) != 0);
+                }
+                const uint64_t dk = dr0 + static_cast<uint64_t>(((5 * j + 2) & 7) * (kLpUnit >> 4));
+                for (int ks = 0; ks < rsteps; ++ks)
+                    umma_ss(d, dq + 2 * (kLpUnit >> 4) + ((ks * 32) >> 4), dk + ((ks * 32) >> 4), id_s, 1);
+                umma_commit(smem_u32(&s_full[t]));
+                if (t == 1 || j >= ntB) umma_commit(smem_u32(&k_empty[j & 1]));
+            };
+            auto issue_pv = [&](int t, int j) {
+                ok = ok && mbar_wait(smem_u32(&p_full[t]), j & 1, p.err);
+                if (j > v_waited) {
+                    ok = ok && mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, p.err);
+                    v_waited = j;
+                }
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t d = tmem + 256 + t * 128, a = tmem + t * 128;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint64_t dv = dr0 + static_cast<uint64_t>(((5 * j + 3 + u) & 7) * (kLpUnit >> 4));
+#pragma unroll
+                    for (int ks = 0; ks < kLpKeys / 16; ++ks)
+                        umma_ts(d + u * 64, a + ks * 8, dv + ((ks * 2048) >> 4), id_pv, (j > 0 || ks > 0) ? 1u : 0u);
+                }
+                umma_commit(smem_u32(&o_full[t]));
+                if (t == 1 || j >= ntB) umma_commit(smem_u32(&v_empty[j & 1]));
+            };
+            issue_s(0, 0);
+            if (ntB > 0) issue_s(1, 0);
+            for (int j = 0; j < ntiles && ok; ++j) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (j < nt[t]) {
+                        issue_pv(t, j);
+                        if (j + 1 < nt[t]) issue_s(t, j + 1);
+                    }
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ softmax, one query row per thread
+        const int t = warp >> 2, r = threadIdx.x & 127, qrow = q0 + t * kLpRows + r;
+        const bool valid_row = qrow < sq.n;
+        const int qpos = pos0 + qrow, ntt = t ? ntB : ntA;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const uint32_t s_col = t * 128, o_col = 256 + t * 128;
+        const float sc = p.scale_log2;
+        float m_ref = -INFINITY, l = 0.f;
+        bool alive = true;
+        for (int j = 0; j < ntt; ++j) {
+            if (!wait_all(smem_u32(&s_full[t]), j & 1, p.err)) { alive = false; break; }
+            tc_fence_after();
+            const int key0 = j * kLpKeys;
+            float v[kLpKeys / 32][32];
+#pragma unroll
+            for (int c = 0; c < kLpKeys / 32; ++c) tmem_ld32(lane_base + s_col + c * 32, v[c]);
+            tmem_wait_ld();
+            if (key0 + kLpKeys - 1 > pos0 + q0 + t * kLpRows) {
+                const int lim = qpos - key0;
+#pragma unroll
+                for (int c = 0; c < kLpKeys / 32; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c * 32 + i > lim) v[c][i] = -INFINITY;
+            }
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < kLpKeys / 32; ++c)
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    mx4[0] = max3(mx4[0], v[c][i], v[c][i + 1]);
+                    mx4[1] = max3(mx4[1], v[c][i + 2], v[c][i + 3]);
+                    mx4[2] = max3(mx4[2], v[c][i + 4], v[c][i + 5]);
+                    mx4[3] = max3(mx4[3], v[c][i + 6], v[c][i + 7]);
+                }
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+            float alpha = 1.f;
+            if (mx > m_ref + 8.f || m_ref == -INFINITY) {
+                const float m_new = fmaxf(m_ref, mx);
+                alpha = ex2(m_ref - m_new);
+                m_ref = m_new;
+            }
+            const float mneg = m_ref == -INFINITY ? 0.f : -m_ref;
+            float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < kLpKeys / 32; ++c) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float a0 = ex2(fmaf(v[c][i], sc, mneg));
+                    const float a1 = ex2(fmaf(v[c][i + 1], sc, mneg));
+                    sum4[(i >> 1) & 3] += a0 + a1;
+                    pk[i >> 1] = Elem<T>::pack(a0, a1);
+                }
+                tmem_st16(lane_base + s_col + c * 16, pk);
+            }
+            l = l * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+            // after P is stored, when the S row's registers are dead
+            if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+                for (int c = 0; c < kLpHead / 32; ++c) {
+                    float o[32];
+                    tmem_ld32(lane_base + o_col + c * 32, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] *= alpha;
+                    tmem_st32(lane_base + o_col + c * 32, o);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&p_full[t]));
+        }
+        if (alive && ntt > 0 && wait_all(smem_u32(&o_full[t]), (ntt - 1) & 1, p.err)) {
+            tc_fence_after();
+            const float inv = 1.f / l;
+            char* dst = p.out + 2 * ((static_cast<int64_t>(sq.row0) + (valid_row ? qrow : 0)) * p.H + h) * kLpHead;
+#pragma unroll
+            for (int c = 0; c < kLpHead / 32; ++c) {
+                float o[32];
+                tmem_ld32(lane_base + o_col + c * 32, o);
+                tmem_wait_ld();
+                if (valid_row) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        *reinterpret_cast<uint4*>(dst + 2 * (c * 32 + i)) =
+                            make_uint4(Elem<T>::pack(o[i] * inv, o[i + 1] * inv), Elem<T>::pack(o[i + 2] * inv, o[i + 3] * inv),
+                                       Elem<T>::pack(o[i + 4] * inv, o[i + 5] * inv), Elem<T>::pack(o[i + 6] * inv, o[i + 7] * inv));
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Heads whose keys and values the workspace holds at once: all, up to 1 GiB.
+constexpr uint64_t kLpWorkspace = 1ull << 30;
+static int lp_heads(int64_t rows, int H) {
+    const uint64_t per_head = static_cast<uint64_t>(rows) * 512;
+    const int64_t fit = static_cast<int64_t>(kLpWorkspace / per_head);
+    const int most = static_cast<int>(fit < 1 ? 1 : fit > H ? H : fit);
+    const int groups = (H + most - 1) / most;
+    return (H + groups - 1) / groups;  // even groups
+}
+
+template <typename T>
+static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensorMap& tq, const CUtensorMap& tw, const CUtensorMap& tkv,
+                                       cudaStream_t st) {
+    static uint64_t attr_set = 0;
+    const uint64_t bit = 1ull << (pool->device & 63);
+    if (!(attr_set & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(latent_expand_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLpSmemMax);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(latent_prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLaSmem);
+        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(latent prefill)");
+        attr_set |= bit;
+    }
+    const int tiles = p.lpad / kLpKeys;
+    const int lch = p.latent / 64;
+    p.stages = min(kLeMaxStages, (kLpSmemMax - 2048 - lch * kLpUnit) / kLeStage);
+    const size_t smem = static_cast<size_t>(lch) * kLpUnit + static_cast<size_t>(p.stages) * kLeStage + 2048;
+    // heads per CTA: at most 8 (the 128 gathered rows are then read once per 2 MiB of
+    // W at 512), fewer when that would leave SMs idle
+    const int64_t items = static_cast<int64_t>(p.B) * tiles * p.heads;
+    p.per_cta = static_cast<int>(min(static_cast<int64_t>(8), max(static_cast<int64_t>(1), items / (2 * pool->num_sms))));
+    latent_expand_kernel<T><<<dim3((p.heads + p.per_cta - 1) / p.per_cta, tiles, p.B), kLeThreads, smem, st>>>(pool->tmap16, tw, p);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "latent_expand_kernel launch");
+    const dim3 grid((p.max_tokens + 2 * kLpRows - 1) / (2 * kLpRows), p.heads, p.B);
+    latent_prefill_kernel<T><<<grid, kLaThreads, kLaSmem, st>>>(pool->tmap16, tq, tkv, p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "latent_prefill_kernel launch");
+    return VK_OK;
+}
+
+}  // namespace vk
+
+using namespace vk;
+
+extern "C" size_t vk_latent_prefill_workspace_size(const vk_pool* pool, int32_t batch, int32_t max_seq_len, int32_t num_heads) {
+    if (!pool || !is_latent(pool) || batch <= 0 || max_seq_len <= 0 || num_heads <= 0) return 0;
+    const int64_t rows = static_cast<int64_t>(batch) * ((static_cast<int64_t>(max_seq_len) + kLpKeys - 1) / kLpKeys * kLpKeys);
+    if (rows >= (1ll << 31)) return 0;
+    return static_cast<size_t>(rows) * 512 * lp_heads(rows, num_heads);
+}
+
+extern "C" vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                       const void* w_kv, int64_t w_stride, void* out, const int32_t* block_tables,
+                                       int32_t bt_stride, const int32_t* positions, const int32_t* offsets, int32_t batch,
+                                       int32_t tokens, int32_t max_tokens, int32_t max_seq_len, int32_t num_heads, float scale,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+    if (!pool) return fail(VK_INVALID_ARG, "pool is NULL");
+    if (!is_latent(pool)) return fail(VK_UNSUPPORTED, "latent prefill needs a latent pool");
+    if (layer < 0 || layer >= pool->cfg.num_layers) return fail(VK_INVALID_ARG, "layer out of range");
+    if (batch < 0 || tokens < 0 || num_heads <= 0 || bt_stride <= 0) return fail(VK_INVALID_ARG, "bad batch/tokens/heads/bt_stride");
+    if (!(scale >= 0.f) || scale > 3.0e38f) return fail(VK_INVALID_ARG, "scale must be finite, > 0 or 0 for 1/sqrt(128 + rope_dim)");
+    if (batch == 0 || tokens == 0) return VK_OK;
+    if (!q || !w_kv || !out || !block_tables || !positions) return fail(VK_INVALID_ARG, "NULL array");
+    if (!offsets && tokens % batch) return fail(VK_INVALID_ARG, "without offsets, tokens must be a multiple of batch");
+    if (max_tokens <= 0 || max_seq_len < max_tokens) return fail(VK_INVALID_ARG, "max_tokens must be > 0 and max_seq_len >= max_tokens");
+    if (!offsets && max_tokens < tokens / batch) return fail(VK_INVALID_ARG, "max_tokens is smaller than the chunk");
+    if (max_seq_len > static_cast<int64_t>(bt_stride) * pool->cfg.page_tokens)
+        return fail(VK_INVALID_ARG, "max_seq_len exceeds the block table capacity");
+    if (batch > 65535 || num_heads > 65535) return fail(VK_INVALID_ARG, "batch and num_heads must be <= 65535");
+    if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(w_kv) | reinterpret_cast<uintptr_t>(out)) & 15) ||
+        q_token_stride % 8 || q_head_stride % 8 || w_stride % 8)
+        return fail(VK_INVALID_ARG, "q, w_kv and out must be 16-byte aligned, strides multiples of 8");
+    if (q_token_stride < 0 || q_head_stride < 0 || w_stride < pool->latent_dim)
+        return fail(VK_INVALID_ARG, "q strides must be >= 0, w_stride >= latent_dim");
+    const size_t need = vk_latent_prefill_workspace_size(pool, batch, max_seq_len, num_heads);
+    if (need == 0 || max_seq_len > 65535 * kLpKeys) return fail(VK_INVALID_ARG, "batch * max_seq_len too large");
+    if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 127))
+        return fail(VK_INVALID_ARG, "workspace missing, too small or not 128-byte aligned");
+    LpParams p{};
+    p.bt = block_tables;
+    p.pos = positions;
+    p.offsets = offsets;
+    p.err = pool->d_err;
+    p.ws = static_cast<char*>(workspace);
+    p.out = static_cast<char*>(out);
+    p.bt_stride = bt_stride;
+    p.B = batch;
+    p.tokens = tokens;
+    p.H = num_heads;
+    p.layer = layer;
+    p.num_pages = pool->num_pages;
+    p.P = pool->cfg.page_tokens;
+    p.latent = pool->latent_dim;
+    p.rope = pool->rope_dim;
+    p.lpad = (max_seq_len + kLpKeys - 1) / kLpKeys * kLpKeys;
+    p.max_tokens = max_tokens;
+    p.max_len = max_seq_len;
+    const int width = kLpHead + p.rope;
+    p.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(width))) * 1.4426950408889634f;
+    const int64_t rows = static_cast<int64_t>(batch) * p.lpad;
+    const int group = lp_heads(rows, num_heads);
+
+    const CUtensorMapDataType type = pool->kv_format == VK_KV_LATENT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    alignas(64) CUtensorMap tq, tw, tkv;
+    auto encode = tmap_encode_fn();
+    if (!encode) return fail(VK_CUDA_ERROR, "cuTensorMapEncodeTiled unavailable");
+    const cuuint32_t estr[3] = {1, 1, 1};
+    {
+        // a stride of a dimension of one element is never used: any valid one will do
+        const cuuint64_t hs = static_cast<cuuint64_t>(num_heads > 1 ? q_head_stride : width + 8) * 2 & ~cuuint64_t(15);
+        const cuuint64_t ts = static_cast<cuuint64_t>(tokens > 1 ? q_token_stride : width + 8) * 2 & ~cuuint64_t(15);
+        const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(num_heads), static_cast<cuuint64_t>(tokens)};
+        const cuuint64_t strides[2] = {hs, ts};
+        const cuuint32_t box[3] = {64, 1, kLpRows};
+        if (encode(&tq, type, 3, const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return fail(VK_INVALID_ARG, "q's shape or strides cannot be addressed by TMA");
+    }
+    {
+        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.latent), static_cast<cuuint64_t>(num_heads) * 256};
+        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(w_stride) * 2};
+        const cuuint32_t box[2] = {64, 256};
+        if (encode(&tw, type, 2, const_cast<void*>(w_kv), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return fail(VK_INVALID_ARG, "w_kv's shape or stride cannot be addressed by TMA");
+    }
+    DeviceGuard g(pool->device);
+    // the last group may have fewer heads; its rows keep its own pitch, so it has its own map
+    for (int h0 = 0; h0 < num_heads; h0 += group) {
+        p.h0 = h0;
+        p.heads = min(group, num_heads - h0);
+        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.heads) * 256, static_cast<cuuint64_t>(rows)};
+        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.heads) * 512};
+        const cuuint32_t box[2] = {64, kLpKeys};
+        if (encode(&tkv, type, 2, workspace, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return fail(VK_CUDA_ERROR, "cuTensorMapEncodeTiled failed for the workspace");
+        const vk_status s = pool->kv_format == VK_KV_LATENT_BF16
+                                ? launch_latent_prefill<__nv_bfloat16>(pool, p, tq, tw, tkv, as_stream(stream))
+                                : launch_latent_prefill<__half>(pool, p, tq, tw, tkv, as_stream(stream));
+        if (s != VK_OK) return s;
+    }
+    return VK_OK;
+}

@@ -4,8 +4,8 @@
   half layout, the leading part of a head, frequencies scaled for long contexts.
 * ``LatentKVPool`` — vk_latent: a paged cache of one latent vector and one shared
   rotary key part a token, its append (norm and rotation fused) and its
-  attention in the absorbed form (decode).  The page operations
-  of ``PagedKVPool`` (alloc, free, copy, compaction, swap) work on it unchanged.
+  attention in the absorbed form (decode) and the expanded form (prefill).  The
+  page operations of ``PagedKVPool`` (alloc, free, copy, compaction, swap) work on it unchanged.
 
 No reference counterpart: the reference has neither.
 """
@@ -266,6 +266,50 @@ class LatentKVPool(PagedKVPool):
             _i32(seq_lens, "seq_lens", dev, batch), batch, tokens, heads, scale, ws.data_ptr(),
             ws.numel() * ws.element_size(), _stream_of(stream, dev)), "vk_latent_decode")
         return (out, lse) if return_lse else out
+
+    def prefill_workspace_size(self, batch: int, max_seq_len: int, num_heads: int) -> int:
+        return self._lib.vk_latent_prefill_workspace_size(self.handle, batch, max_seq_len, num_heads)
+
+    def prefill(self, layer: int, q: torch.Tensor, w_kv: torch.Tensor, block_tables: torch.Tensor, positions: torch.Tensor,
+                offsets: Optional[torch.Tensor] = None, max_tokens: Optional[int] = None, max_seq_len: Optional[int] = None,
+                scale: float = 0.0, out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                stream=None) -> torch.Tensor:
+        """Expanded form.  q [tokens, H, 128 + rope_dim] or [B, T, H, 128 + rope_dim] (rotary part rotated; strided
+        views allowed), w_kv [H*256, latent_dim]: per head 128 rows of the key and 128 of the value up-projection.
+        Sequence b's rows are offsets[b]..offsets[b+1]-1 (None: the same number each), from position positions[b] on.
+        ``max_tokens`` bounds the longest chunk (default: without offsets the chunk, with them all tokens),
+        ``max_seq_len`` the longest sequence after the chunk (default: what the tables hold).  Returns
+        [..., H, 128]."""
+        dev = self.device
+        batch = _tables(block_tables, dev)
+        _on(q, self.dtype, "q", dev)
+        _on(w_kv, self.dtype, "w_kv", dev)
+        qt, qh = _token_head(q, "q")
+        heads = q.shape[-2]
+        if q.shape[-1] != 128 + self.rope_dim:
+            raise ValueError("q must have %d elements a head" % (128 + self.rope_dim))
+        if w_kv.dim() != 2 or w_kv.shape[0] != heads * 256 or w_kv.shape[1] != self.latent_dim or w_kv.stride(1) != 1:
+            raise ValueError("w_kv must be [%d, %d] with unit stride along its rows" % (heads * 256, self.latent_dim))
+        tokens = q.shape[0] if q.dim() == 3 else q.shape[0] * q.shape[1]
+        if max_tokens is None:
+            max_tokens = tokens if offsets is not None else tokens // max(1, batch)
+        if max_seq_len is None:
+            max_seq_len = block_tables.shape[1] * self.page_tokens
+        shape = q.shape[:-1] + (128,)
+        if out is None:
+            out = _empty(shape, self.dtype, dev, stream)
+        else:
+            _on(out, self.dtype, "out", dev)
+            if out.shape != shape or not out.is_contiguous():
+                raise ValueError("out must be contiguous with shape %s" % (tuple(shape),))
+        ws = workspace if workspace is not None else _empty((self.prefill_workspace_size(batch, max_seq_len, heads),),
+                                                            torch.uint8, dev, stream)
+        check(self._lib.vk_latent_prefill(
+            self.handle, layer, q.data_ptr(), qt, qh, w_kv.data_ptr(), w_kv.stride(0), out.data_ptr(),
+            block_tables.data_ptr(), block_tables.shape[1], _i32(positions, "positions", dev, batch),
+            None if offsets is None else _i32(offsets, "offsets", dev, batch + 1), batch, tokens, max_tokens, max_seq_len,
+            heads, scale, ws.data_ptr(), ws.numel() * ws.element_size(), _stream_of(stream, dev)), "vk_latent_prefill")
+        return out
 
     def plan(self, *args, **kwargs):
         raise TypeError("a latent pool has no planned decode: use decode")
