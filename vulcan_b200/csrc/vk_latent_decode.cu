@@ -54,6 +54,9 @@ constexpr int kLdUnitCost = 2;
 // Least cost of a CTA's range: fewer, longer pieces when there is little work
 constexpr int kLdMinRange = 4;
 
+// Non-blocking polls (~50 cycles each) before the MMA warp gives up: over a second
+constexpr uint32_t kLdPolls = 1u << 26;
+
 struct LdParams {
     const char* ql;
     const char* qr;
@@ -145,7 +148,7 @@ __device__ __forceinline__ uint32_t finite_word(uint32_t w) {
     return w;
 }
 
-template <typename T>
+template <typename T, int LCH>  // LCH: latent_dim / 64
 __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __grid_constant__ CUtensorMap tmap,
                                                                       const __grid_constant__ LdParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -278,55 +281,64 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         }
     } else if (warp == 5) {
         // ------------------------------------------------------------ MMA issuer
+        // S of tile si and the output product of tile pi are issued as they become
+        // possible (pi <= si <= pi + 2, S has two buffers), products first: they
+        // free a stage of the ring, whose refill is what the kernel waits for.
         if (lane == 0) {
             LdWalk w = walk0;
             LdPiece c;
-            int it = 0, piece = 0;
+            int si = 0, pi = 0, piece = 0;
             bool ok = true;
             constexpr uint32_t id_s = idesc_16(Elem<T>::kBf16, 64, 64, 0, 0);
             constexpr uint32_t id_pv = idesc_16(Elem<T>::kBf16, 128, 64, 1, 0);
-            const uint64_t dq = umma_desc_sw128(s_q, 16, 1024);
-            const uint64_t dp = umma_desc_sw128(s_p, 16, 1024);
-            const int lch = p.latent >> 6, rsteps = p.rope >> 4;
-            auto issue_s = [&](int i) {
-                const int st = i % p.stages;
-                ok = ok && mbar_wait(smem_u32(&k_full[st]), (i / p.stages) & 1, p.err);
-                if (!ok) return;
-                tc_fence_after();
-                const uint64_t dk = umma_desc_sw128(sbase + st * stage_bytes, 16, 1024);
-                const uint32_t d = tmem + 256 + (i & 1) * 64;
-                for (int ch = 0; ch < lch; ++ch)
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        const uint64_t off = static_cast<uint64_t>((ch * kLdChunk + ks * 32) >> 4);
-                        umma_ss(d, dq + off, dk + off, id_s, (ch | ks) != 0);
-                    }
-                for (int ks = 0; ks < rsteps; ++ks) {
-                    const uint64_t off = static_cast<uint64_t>((lch * kLdChunk + ks * 32) >> 4);
-                    umma_ss(d, dq + off, dk + off, id_s, 1);
-                }
-                umma_commit(smem_u32(&s_full[i & 1]));
-            };
+            const uint64_t dk0 = umma_desc_sw128(sbase, 16, 1024), dv0 = umma_desc_sw128(sbase, kLdChunk, 1024);
+            const uint32_t k_hi = static_cast<uint32_t>(dk0 >> 32), v_hi = static_cast<uint32_t>(dv0 >> 32);
+            const uint32_t k_lo = static_cast<uint32_t>(dk0), v_lo = static_cast<uint32_t>(dv0);
+            const uint32_t q_lo = k_lo + ((s_q - sbase) >> 4), p_lo = k_lo + ((s_p - sbase) >> 4);
+            const int rsteps = p.rope >> 4;
             while (ok && w.next_real(p, c)) {
-                const int nt = c.t1 - c.t0;
+                const int first = si, end = si + c.t1 - c.t0;
                 ok = mbar_wait(smem_u32(q_full), piece & 1, p.err);
                 ++piece;
-                if (!ok) break;
-                issue_s(it);
-                for (int j = 0; j < nt && ok; ++j, ++it) {
-                    if (j + 1 < nt) issue_s(it + 1);
-                    ok = ok && mbar_wait(smem_u32(p_full), it & 1, p.err);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const int st = it % p.stages;
-                    const uint64_t dv = umma_desc_sw128(sbase + st * stage_bytes, kLdChunk, 1024);
-                    for (int mb = 0; mb < (p.latent >> 7); ++mb)
+                uint32_t polls = 0;
+                while (ok && pi < end) {
+                    if (pi < si && mbar_test(smem_u32(p_full), pi & 1)) {
+                        tc_fence_after();
+                        const int st = pi % p.stages;
+                        const uint32_t vl = v_lo + st * (stage_bytes >> 4);
+                        const uint32_t acc = pi != first;
 #pragma unroll
-                        for (int ks = 0; ks < kLdKeys / 16; ++ks)
-                            umma_ss(tmem + mb * 64, dv + static_cast<uint64_t>((mb * 2 * kLdChunk + ks * 2048) >> 4),
-                                    dp + static_cast<uint64_t>((ks * 32) >> 4), id_pv, (j | ks) != 0);
-                    umma_commit(smem_u32(pv_done));
-                    umma_commit(smem_u32(&k_empty[st]));
+                        for (int mb = 0; mb < LCH / 2; ++mb)
+#pragma unroll
+                            for (int ks = 0; ks < kLdKeys / 16; ++ks)
+                                umma_ss_lo(tmem + mb * 64, vl + ((mb * 2 * kLdChunk + ks * 2048) >> 4), v_hi, p_lo + ks * 2, k_hi, id_pv,
+                                           ks ? 1 : acc);
+                        umma_commit(smem_u32(&k_empty[st]));
+                        umma_commit(smem_u32(pv_done));
+                        ++pi;
+                        polls = 0;
+                    } else if (si < end && si < pi + 2 && mbar_test(smem_u32(&k_full[si % p.stages]), (si / p.stages) & 1)) {
+                        tc_fence_after();
+                        const uint32_t kl = k_lo + (si % p.stages) * (stage_bytes >> 4);
+                        const uint32_t d = tmem + 256 + (si & 1) * 64;
+#pragma unroll
+                        for (int ch = 0; ch < LCH; ++ch)
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks)
+                                umma_ss_lo(d, q_lo + ((ch * kLdChunk + ks * 32) >> 4), k_hi, kl + ((ch * kLdChunk + ks * 32) >> 4), k_hi, id_s,
+                                           (ch | ks) != 0);
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            if (ks < rsteps)
+                                umma_ss_lo(d, q_lo + ((LCH * kLdChunk + ks * 32) >> 4), k_hi, kl + ((LCH * kLdChunk + ks * 32) >> 4), k_hi,
+                                           id_s, 1);
+                        umma_commit(smem_u32(&s_full[si & 1]));
+                        ++si;
+                        polls = 0;
+                    } else if (++polls >= kLdPolls) {
+                        atomicOr(p.err, VK_ERR_TIMEOUT);
+                        ok = false;
+                    }
                 }
             }
         }
@@ -336,7 +348,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         LdPiece c, nx;
         const int r = warp * 16 + (lane & 15), hi = lane >> 4;  // row of the group; which half of a tile's keys
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-        const int width8 = (p.latent + p.rope) >> 3, lat8 = p.latent >> 3;
+        const int rope8 = p.rope >> 3, lat8 = LCH * 8;
 
         // next piece with tiles; rows of empty units are written on the way
         auto advance = [&](LdPiece& o) -> bool {
@@ -351,16 +363,30 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
             }
             return false;
         };
+        // 16 rows a warp, a row's 16-byte vectors across the lanes; one division per
+        // piece, then (token, head) step along
         auto load_q = [&](const LdPiece& o) {
-            for (int k = warp; k < 64; k += 4) {
-                const int rr = o.g * 64 + k;
-                const bool live = rr < rows;
-                const int t = live ? rr / p.H : 0, h = live ? rr % p.H : 0;
-                const int64_t tok = static_cast<int64_t>(o.b) * p.T + t;
-                const char* ql = p.ql + 2 * (tok * p.ql_token + h * p.ql_head);
-                const char* qr = p.qr + 2 * (tok * p.qr_token + h * p.qr_head);
-                for (int v = lane; v < width8; v += 32)
-                    cp_async16(s_q + (v >> 3) * kLdChunk + swz128(k, v & 7), v < lat8 ? ql + v * 16 : qr + (v - lat8) * 16, live);
+            int t = (o.g * 64 + warp * 16) / p.H, h = (o.g * 64 + warp * 16) % p.H;
+            const char* ql = p.ql + 2 * ((static_cast<int64_t>(o.b) * p.T + t) * p.ql_token + h * p.ql_head) + lane * 16;
+            const char* qr = p.qr + 2 * ((static_cast<int64_t>(o.b) * p.T + t) * p.qr_token + h * p.qr_head) + lane * 16;
+            const int live = rows - o.g * 64 - warp * 16;  // rows of this warp that exist
+#pragma unroll 4
+            for (int k = 0; k < 16; ++k) {
+                const bool on = k < live;
+                const uint32_t dst = s_q + swz128(warp * 16 + k, lane & 7) + (lane >> 3) * kLdChunk;
+#pragma unroll
+                for (int i = 0; i < (LCH + 3) / 4; ++i)
+                    if (lane + 32 * i < LCH * 8) cp_async16(dst + i * 4 * kLdChunk, on ? ql + i * 512 : p.ql, on);
+                if (lane < rope8)
+                    cp_async16(s_q + LCH * kLdChunk + swz128(warp * 16 + k, lane), on ? qr : p.qr, on);
+                ql += 2 * p.ql_head;
+                qr += 2 * p.qr_head;
+                if (++h == p.H) {
+                    h = 0;
+                    ++t;
+                    ql += 2 * (p.ql_token - p.H * p.ql_head);
+                    qr += 2 * (p.qr_token - p.H * p.qr_head);
+                }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             fence_async_smem();
@@ -451,7 +477,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                     tc_fence_after();
                     if (!hi) alpha[r] = resc ? al : 1.f;
                     bar_softmax();
-                    for (int col = 0; col < (p.latent >> 1); col += 32) {
+                    for (int col = 0; col < (LCH * 32); col += 32) {
                         float o[32];
                         tmem_ld32(lane_base + col, o);
                         tmem_wait_ld();
@@ -496,7 +522,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
             if (bar_softmax_or(fail)) goto done;
             tc_fence_after();
             const int live = min(64, rows - c.g * 64);
-            for (int mb = 0; mb < (p.latent >> 7); ++mb)
+            for (int mb = 0; mb < LCH / 2; ++mb)
 #pragma unroll
                 for (int hc = 0; hc < 2; ++hc) {
                     if (hc * 32 >= live) break;
@@ -606,18 +632,26 @@ __global__ void latent_merge_kernel(const LdParams p) {
 
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-template <typename T>
-static vk_status launch_latent_decode(vk_pool* pool, const LdParams& p, cudaStream_t st) {
+template <typename T, int LCH>
+static cudaError_t launch_latent_split(vk_pool* pool, const LdParams& p, cudaStream_t st) {
     static uint64_t attr_set = 0;
     const uint64_t bit = 1ull << (pool->device & 63);
     const size_t smem = static_cast<size_t>(p.stages + 1) * p.nch * kLdChunk + kLdChunk + kLdAux + 1024;
     if (!(attr_set & bit)) {
-        cudaError_t e = cudaFuncSetAttribute(latent_decode_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLdSmemMax);
-        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(latent_decode)");
+        cudaError_t e = cudaFuncSetAttribute(latent_decode_kernel<T, LCH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLdSmemMax);
+        if (e != cudaSuccess) return e;
         attr_set |= bit;
     }
-    latent_decode_kernel<T><<<pool->num_sms, kLdThreads, smem, st>>>(pool->tmap16, p);
-    cudaError_t e = cudaGetLastError();
+    latent_decode_kernel<T, LCH><<<pool->num_sms, kLdThreads, smem, st>>>(pool->tmap16, p);
+    return cudaGetLastError();
+}
+
+template <typename T>
+static vk_status launch_latent_decode(vk_pool* pool, const LdParams& p, cudaStream_t st) {
+    cudaError_t e = p.latent == 512   ? launch_latent_split<T, 8>(pool, p, st)
+                    : p.latent == 384 ? launch_latent_split<T, 6>(pool, p, st)
+                    : p.latent == 256 ? launch_latent_split<T, 4>(pool, p, st)
+                                      : launch_latent_split<T, 2>(pool, p, st);
     if (e != cudaSuccess) return cuda_fail(e, "latent_decode_kernel launch");
     // few rows: many pieces each, so more warps share a row's pieces
     const int64_t units = static_cast<int64_t>(p.B) * p.groups;
