@@ -10,4 +10,11 @@ __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, uint32_t
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
 }
 
+// 3-input max (one instruction on sm_100)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 }  // namespace vk

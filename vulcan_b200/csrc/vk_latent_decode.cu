@@ -15,17 +15,19 @@
 //
 //  * warp 4 streams tiles with 2-D TMA boxes (64 elements x one page's rows,
 //    128-byte swizzle) into a ring of as many stages as fit (2 at 512 + 64);
-//  * warp 5, one thread, issues tcgen05.mma:  S[64 rows x 64 keys] = Q K^T (M 64,
-//    K-major both), then  O^T[latent x 64 rows] += V^T P^T  as M = 128 blocks of
-//    latent elements.  The transposed output keeps all 128 lanes at work with 64
+//  * warp 5 issues  S[64 rows x 64 keys] = Q K^T  (tcgen05.mma, M 64, K-major
+//    both) and warp 6  O^T[latent x 64 rows] += V^T P^T  as M = 128 blocks of
+//    latent elements: an MMA costs its thread 40-60 cycles to issue, more than the
+//    tensor core takes, so two threads issue.  The transposed output keeps all 128 lanes at work with 64
 //    rows (O itself would be M = 64 at half the rate) and needs 256 TMEM columns
 //    instead of 512, so S has two buffers beside it: S of tile i+1 is issued
 //    before O of tile i and the tensor core works through the softmax.  V^T is
 //    the K tile itself read MN-major, P^T is P read K-major: nothing is copied;
 //  * warps 0-3: softmax with running maximum and sum.  Row r of S lies in lane
-//    (r/16)*32 + r%16 of TMEM (M = 64 fills 16 lanes of each warp), so the upper
-//    16 lanes take the second half of each row's keys by shuffle.  O is rescaled
-//    only when a row's maximum grows by more than 2^8 (all warps vote).
+//    (r/16)*32 + r%16 of TMEM (M = 64 fills 16 lanes of each warp's quarter); the
+//    matrix-fragment load spreads them over all 32 threads (2 rows x 16 keys
+//    each), and P goes to shared memory by stmatrix.  O is rescaled only when a
+//    row's maximum grows by more than 2^8 (all warps vote).
 //
 // P is rounded to the cache's 16-bit type for the second product: relative
 // error 2^-9 (bf16) or 2^-12 (fp16) a weight, below the output's own rounding;
@@ -44,18 +46,19 @@
 namespace vk {
 
 constexpr int kLdKeys = 64;       // keys of a tile
-constexpr int kLdThreads = 192;   // 4 softmax warps, TMA warp, MMA warp
+constexpr int kLdThreads = 224;   // 4 softmax warps, TMA warp, two MMA warps
 constexpr int kLdMaxStages = 8;
+constexpr int kLdParts = 5;       // barriers of a stage: pairs of chunks of the latent, the rotary chunk
 constexpr int kLdChunk = kLdKeys * 128;  // 64 keys x 64 elements, 128-byte rows
-constexpr int kLdAux = 1024;             // barriers, alpha, 1/l, schedule
+constexpr int kLdAux = 1536;             // barriers, alpha, 1/l, schedule
 constexpr int kLdSmemMax = 232448;
 // A unit's prologue and epilogue (q load, output) in tiles, for the deal.
 constexpr int kLdUnitCost = 2;
 // Least cost of a CTA's range: fewer, longer pieces when there is little work
 constexpr int kLdMinRange = 4;
 
-// Non-blocking polls (~50 cycles each) before the MMA warp gives up: over a second
-constexpr uint32_t kLdPolls = 1u << 26;
+// Tiles of L2 prefetch ahead of the ring.
+constexpr int kLdAhead = 3;
 
 struct LdParams {
     const char* ql;
@@ -65,6 +68,7 @@ struct LdParams {
     float* lse;
     const int32_t* bt;
     const int32_t* lens;
+    const char* layer_base;  // the pool's rows of this layer
     uint32_t* err;
     float* ws_o;     // [2 * CTAs][64][latent]
     float2* ws_ml;   // [2 * CTAs][64]: maximum (log2 domain), sum
@@ -159,16 +163,16 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
     const uint32_t s_q = sbase + p.stages * stage_bytes, s_p = s_q + stage_bytes;
     uint8_t* aux = smem + (p.stages + 1) * stage_bytes + kLdChunk;
     uint64_t* bars = reinterpret_cast<uint64_t*>(aux);
-    uint64_t* k_full = bars;                    // [stages] tile landed
-    uint64_t* k_empty = bars + kLdMaxStages;    // [stages] both products have read it
-    uint64_t* s_full = bars + 2 * kLdMaxStages;  // [2]
-    uint64_t* p_full = s_full + 2;              // P written, O rescaled, last piece's O read
-    uint64_t* pv_done = s_full + 3;
-    uint64_t* q_full = s_full + 4;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 5);
-    float* alpha = reinterpret_cast<float*>(aux + 256);   // [64] rescale factors
-    float* inv_l = reinterpret_cast<float*>(aux + 512);   // [64]
-    int64_t* sched = reinterpret_cast<int64_t*>(aux + 768);  // total, first b, its start; then warp sums
+    uint64_t* k_full = bars;                                // [stages][parts] a part of the tile landed
+    uint64_t* k_empty = bars + kLdMaxStages * kLdParts;     // [stages][parts] its last product is done
+    uint64_t* s_full = bars + 2 * kLdMaxStages * kLdParts;  // [2]
+    uint64_t* p_full = s_full + 2;  // [2] S read, P written, O rescaled, last piece's O read
+    uint64_t* pv_done = s_full + 4;
+    uint64_t* q_full = s_full + 5;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 6);
+    float* alpha = reinterpret_cast<float*>(aux + 768);   // [64] rescale factors
+    float* inv_l = reinterpret_cast<float*>(aux + 1024);  // [64]
+    int64_t* sched = reinterpret_cast<int64_t*>(aux + 1280);  // first b, its start; then warp sums
     int64_t* wsum = sched + 4;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -189,13 +193,14 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
     }
     if (lane == 31) wsum[warp] = incl;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < p.stages; ++i) {
+        for (int i = 0; i < p.stages * kLdParts; ++i) {
             mbar_init(smem_u32(&k_full[i]), 1);
             mbar_init(smem_u32(&k_empty[i]), 1);
         }
-        mbar_init(smem_u32(&s_full[0]), 1);
-        mbar_init(smem_u32(&s_full[1]), 1);
-        mbar_init(smem_u32(p_full), 4);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&p_full[i]), 4);
+        }
         mbar_init(smem_u32(pv_done), 1);
         mbar_init(smem_u32(q_full), 4);
         mbar_fence_init();
@@ -244,101 +249,146 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         // ------------------------------------------------------------ TMA producer
         LdWalk w = walk0;
         LdPiece c;
-        int it = 0;
+        int st = 0;
+        uint32_t ph = 1;  // parity of the stage's release before this fill (first round: none)
         bool ok = true;
         if (lane == 0) prefetch_tmap(&tmap);
         const uint64_t pol = p.groups > 1 ? l2_evict_last_policy() : l2_evict_first_policy();
         const int ppt = kLdKeys / p.P;  // pages of a full tile
+        const uint32_t page_bytes = p.P * 2 * (LCH * 64 + p.rope);
+        bool filled = false;  // every stage has been filled once
         while (ok && w.next_real(p, c)) {
             const int32_t* row = p.bt + static_cast<int64_t>(c.b) * p.bt_stride;
-            const int npages = (c.len + p.P - 1) / p.P;
-            int win = -32, entry = 0;  // block-table entries win..win+31, one a lane
-            for (int t = c.t0; t < c.t1 && ok; ++t, ++it) {
+            const int npages = (c.len + p.P - 1) / p.P, pend = min(npages, c.t1 * ppt);  // this piece's pages end
+            int win = c.t0 * ppt, entry = 0;  // block-table entries win..win+31, one a lane
+            int fetched = win;                // pages before this one are on their way to L2
+            auto load_window = [&]() {
+                entry = win + lane < npages ? __ldg(row + win + lane) : 0;
+                if (entry < 0 || entry >= p.num_pages) {
+                    atomicOr(p.err, VK_ERR_PAGE_ID);
+                    entry = 0;
+                }
+            };
+            load_window();
+            for (int t = c.t0; t < c.t1 && ok; ++t) {
                 const int first = t * ppt, cnt = min(ppt, npages - first);
                 if (first + cnt > win + 32) {
                     win = first;
-                    entry = win + lane < npages ? __ldg(row + win + lane) : 0;
-                    if (entry < 0 || entry >= p.num_pages) {
-                        atomicOr(p.err, VK_ERR_PAGE_ID);
-                        entry = 0;
-                    }
+                    load_window();
                 }
-                const int st = it % p.stages;
-                if (it >= p.stages) ok = wait_all(smem_u32(&k_empty[st]), (it / p.stages - 1) & 1, p.err);
-                if (!ok) break;
-                const uint32_t bar = smem_u32(&k_full[st]);
-                if (lane == 0) mbar_expect_tx(bar, cnt * p.nch * p.P * 128);
-                __syncwarp();
+                // L2 prefetch up to kLdAhead tiles ahead (within the window): the ring holds
+                // two tiles, too few bytes in flight to cover HBM's latency
+                const int to = min(min(pend, (t + 1 + kLdAhead) * ppt), win + 32);
+                if (win + lane >= fetched && win + lane < to)
+                    l2_prefetch(p.layer_base + static_cast<uint64_t>(entry) * page_bytes, page_bytes);
+                fetched = max(fetched, to);
                 const uint32_t dst = sbase + st * stage_bytes;
-                for (int k0 = 0; k0 < cnt * p.nch; k0 += 32) {
-                    const int k = k0 + lane, i = min(k / p.nch, cnt - 1), ch = k % p.nch;
-                    const int page = __shfl_sync(0xffffffffu, entry, first - win + i);
-                    if (k < cnt * p.nch)
-                        tma_load_2d(dst + ch * kLdChunk + i * p.P * 128, &tmap, ch * 64, (p.layer * p.num_pages + page) * p.P,
-                                    bar, pol);
+                const int i = lane >> 1, page = __shfl_sync(0xffffffffu, entry, first - win + min(i, cnt - 1));
+                const int y = (p.layer * p.num_pages + page) * p.P;
+                const uint32_t dst_i = dst + (lane & 1) * kLdChunk + i * p.P * 128;
+                const uint32_t part_bytes = cnt * p.P * 128;
+#pragma unroll
+                for (int g = 0; g <= LCH / 2; ++g) {  // two chunks of 64 elements a part, the rotary chunk last
+                    if (filled) ok = ok && wait_all(smem_u32(&k_empty[st * kLdParts + g]), ph, p.err);
+                    if (!ok) break;
+                    const uint32_t bar = smem_u32(&k_full[st * kLdParts + g]);
+                    const int chunks = g < LCH / 2 ? 2 : 1;
+                    if (lane == 0) mbar_expect_tx(bar, chunks * part_bytes);
+                    if (i < cnt && (lane & 1) < chunks)
+                        tma_load_2d(dst_i + 2 * g * kLdChunk, &tmap, (2 * g + (lane & 1)) * 64, y, bar, pol);
+                }
+                if (++st == p.stages) {
+                    st = 0;
+                    ph ^= 1;
+                    filled = true;
                 }
             }
         }
     } else if (warp == 5) {
-        // ------------------------------------------------------------ MMA issuer
-        // S of tile si and the output product of tile pi are issued as they become
-        // possible (pi <= si <= pi + 2, S has two buffers), products first: they
-        // free a stage of the ring, whose refill is what the kernel waits for.
-        if (lane == 0) {
-            LdWalk w = walk0;
-            LdPiece c;
-            int si = 0, pi = 0, piece = 0;
-            bool ok = true;
-            constexpr uint32_t id_s = idesc_16(Elem<T>::kBf16, 64, 64, 0, 0);
-            constexpr uint32_t id_pv = idesc_16(Elem<T>::kBf16, 128, 64, 1, 0);
-            const uint64_t dk0 = umma_desc_sw128(sbase, 16, 1024), dv0 = umma_desc_sw128(sbase, kLdChunk, 1024);
-            const uint32_t k_hi = static_cast<uint32_t>(dk0 >> 32), v_hi = static_cast<uint32_t>(dv0 >> 32);
-            const uint32_t k_lo = static_cast<uint32_t>(dk0), v_lo = static_cast<uint32_t>(dv0);
-            const uint32_t q_lo = k_lo + ((s_q - sbase) >> 4), p_lo = k_lo + ((s_p - sbase) >> 4);
-            const int rsteps = p.rope >> 4;
-            while (ok && w.next_real(p, c)) {
-                const int first = si, end = si + c.t1 - c.t0;
-                ok = mbar_wait(smem_u32(q_full), piece & 1, p.err);
-                ++piece;
-                uint32_t polls = 0;
-                while (ok && pi < end) {
-                    if (pi < si && mbar_test(smem_u32(p_full), pi & 1)) {
+        // ------------------------------------------------------------ S = Q K^T
+        LdWalk w = walk0;
+        LdPiece c;
+        int si = 0, piece = 0, st = 0, ph = 0;
+        bool ok = true;
+        constexpr uint32_t id_s = idesc_16(Elem<T>::kBf16, 64, 64, 0, 0);
+        const uint64_t dk0 = umma_desc_sw128(sbase, 16, 1024);
+        const uint32_t k_hi = static_cast<uint32_t>(dk0 >> 32), k_lo = static_cast<uint32_t>(dk0);
+        const uint32_t q_lo = k_lo + ((s_q - sbase) >> 4);
+        const int rsteps = p.rope >> 4;
+        const bool lead = elect_lane();
+        while (ok && w.next_real(p, c)) {
+            ok = wait_all(smem_u32(q_full), piece & 1, p.err);
+            ++piece;
+            for (int t = c.t0; t < c.t1 && ok; ++t, ++si) {
+                if (si >= 2) ok = wait_all(smem_u32(&p_full[si & 1]), ((si >> 1) - 1) & 1, p.err);  // S's buffer has been read
+                const uint32_t kl = k_lo + st * (stage_bytes >> 4);
+                const uint32_t d = tmem + 256 + (si & 1) * 64;
+#pragma unroll
+                for (int g = 0; g < LCH / 2; ++g) {
+                    ok = ok && wait_all(smem_u32(&k_full[st * kLdParts + g]), ph, p.err);
+                    if (ok && lead) {
                         tc_fence_after();
-                        const int st = pi % p.stages;
-                        const uint32_t vl = v_lo + st * (stage_bytes >> 4);
-                        const uint32_t acc = pi != first;
 #pragma unroll
-                        for (int mb = 0; mb < LCH / 2; ++mb)
-#pragma unroll
-                            for (int ks = 0; ks < kLdKeys / 16; ++ks)
-                                umma_ss_lo(tmem + mb * 64, vl + ((mb * 2 * kLdChunk + ks * 2048) >> 4), v_hi, p_lo + ks * 2, k_hi, id_pv,
-                                           ks ? 1 : acc);
-                        umma_commit(smem_u32(&k_empty[st]));
-                        umma_commit(smem_u32(pv_done));
-                        ++pi;
-                        polls = 0;
-                    } else if (si < end && si < pi + 2 && mbar_test(smem_u32(&k_full[si % p.stages]), (si / p.stages) & 1)) {
-                        tc_fence_after();
-                        const uint32_t kl = k_lo + (si % p.stages) * (stage_bytes >> 4);
-                        const uint32_t d = tmem + 256 + (si & 1) * 64;
-#pragma unroll
-                        for (int ch = 0; ch < LCH; ++ch)
-#pragma unroll
-                            for (int ks = 0; ks < 4; ++ks)
-                                umma_ss_lo(d, q_lo + ((ch * kLdChunk + ks * 32) >> 4), k_hi, kl + ((ch * kLdChunk + ks * 32) >> 4), k_hi, id_s,
-                                           (ch | ks) != 0);
-#pragma unroll
-                        for (int ks = 0; ks < 4; ++ks)
-                            if (ks < rsteps)
-                                umma_ss_lo(d, q_lo + ((LCH * kLdChunk + ks * 32) >> 4), k_hi, kl + ((LCH * kLdChunk + ks * 32) >> 4), k_hi,
-                                           id_s, 1);
-                        umma_commit(smem_u32(&s_full[si & 1]));
-                        ++si;
-                        polls = 0;
-                    } else if (++polls >= kLdPolls) {
-                        atomicOr(p.err, VK_ERR_TIMEOUT);
-                        ok = false;
+                        for (int k = 0; k < 8; ++k) {
+                            const uint32_t off = ((2 * g + (k >> 2)) * kLdChunk + (k & 3) * 32) >> 4;
+                            umma_ss_lo(d, q_lo + off, k_hi, kl + off, k_hi, id_s, (g | k) != 0);
+                        }
                     }
+                    __syncwarp();
+                }
+                ok = ok && wait_all(smem_u32(&k_full[st * kLdParts + LCH / 2]), ph, p.err);
+                if (ok && lead) {
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        const uint32_t off = (LCH * kLdChunk + ks * 32) >> 4;
+                        if (ks < rsteps) umma_ss_lo(d, q_lo + off, k_hi, kl + off, k_hi, id_s, 1);
+                    }
+                    umma_commit(smem_u32(&s_full[si & 1]));
+                    umma_commit(smem_u32(&k_empty[st * kLdParts + LCH / 2]));
+                }
+                __syncwarp();
+                if (++st == p.stages) {
+                    st = 0;
+                    ph ^= 1;
+                }
+            }
+        }
+    } else if (warp == 6) {
+        // ------------------------------------------------------------ O^T += V^T P^T
+        LdWalk w = walk0;
+        LdPiece c;
+        int pi = 0, st = 0, ph = 0;
+        bool ok = true;
+        constexpr uint32_t id_pv = idesc_16(Elem<T>::kBf16, 128, 64, 1, 0);
+        const uint64_t dv0 = umma_desc_sw128(sbase, kLdChunk, 1024), dp0 = umma_desc_sw128(s_p, 16, 1024);
+        const uint32_t v_hi = static_cast<uint32_t>(dv0 >> 32), v_lo = static_cast<uint32_t>(dv0);
+        const uint32_t p_hi = static_cast<uint32_t>(dp0 >> 32), p_lo = static_cast<uint32_t>(dp0);
+        const bool lead = elect_lane();
+        while (ok && w.next_real(p, c)) {
+            for (int t = c.t0; t < c.t1 && ok; ++t, ++pi) {
+#pragma unroll
+                for (int g = 0; g < LCH / 2; ++g)  // long complete: S has read them
+                    ok = ok && wait_all(smem_u32(&k_full[st * kLdParts + g]), ph, p.err);
+                ok = ok && wait_all(smem_u32(&p_full[pi & 1]), (pi >> 1) & 1, p.err);
+                if (ok && lead) {
+                    tc_fence_after();
+                    const uint32_t vl = v_lo + st * (stage_bytes >> 4);
+                    const uint32_t acc = t != c.t0;
+#pragma unroll
+                    for (int mb = 0; mb < LCH / 2; ++mb) {
+#pragma unroll
+                        for (int ks = 0; ks < kLdKeys / 16; ++ks)
+                            umma_ss_lo(tmem + mb * 64, vl + ((mb * 2 * kLdChunk + ks * 2048) >> 4), v_hi, p_lo + ks * 2, p_hi, id_pv,
+                                       ks ? 1 : acc);
+                        umma_commit(smem_u32(&k_empty[st * kLdParts + mb]));
+                    }
+                    umma_commit(smem_u32(pv_done));
+                }
+                __syncwarp();
+                if (++st == p.stages) {
+                    st = 0;
+                    ph ^= 1;
                 }
             }
         }
@@ -346,7 +396,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         // ------------------------------------------------------------ softmax and output
         LdWalk w = walk0;
         LdPiece c, nx;
-        const int r = warp * 16 + (lane & 15), hi = lane >> 4;  // row of the group; which half of a tile's keys
+        // this thread's rows of the group: r and r + 8; its keys of a tile: 8j + kq and the next
+        const int r = warp * 16 + (lane >> 2), kq = 2 * (lane & 3);
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
         const int rope8 = p.rope >> 3, lat8 = LCH * 8;
 
@@ -394,68 +445,74 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
             if (lane == 0) mbar_arrive(smem_u32(q_full));
         };
 
-        int it = 0;
+        int it = 0, st = 0;
         bool fail = false;
         bool have = advance(c);
         if (have) load_q(c);
         while (have) {
-            float m = -INFINITY, l = 0.f;  // log2 domain; l: this lane's half of the keys
-            const int row = c.g * 64 + r;
-            const int tq = row < rows ? row / p.H : p.T - 1;
-            const int lim = c.len - (p.T - 1 - tq);   // this row's keys
-            const int lim0 = c.len - (p.T - 1);       // keys that every token sees
+            float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // log2 domain; l: this thread's keys
+            int lim[2];  // keys that the row sees
+            bool live_row[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int row = c.g * 64 + r + 8 * u;
+                live_row[u] = row < rows;
+                lim[u] = c.len - (p.T - 1 - (live_row[u] ? row / p.H : p.T - 1));
+            }
+            const int lim0 = c.len - (p.T - 1);  // keys that every token sees
             for (int t = c.t0; t < c.t1; ++t, ++it) {
                 const int key0 = t * kLdKeys;
                 fail = !wait_all(smem_u32(&s_full[it & 1]), (it >> 1) & 1, p.err) || fail;
                 tc_fence_after();
-                float a[32], bq[32];
-                tmem_ld32(lane_base + 256 + (it & 1) * 64, a);
-                tmem_ld32(lane_base + 256 + (it & 1) * 64 + 32, bq);
+                float a[32];
+                tmem_ld_16x64(lane_base + 256 + (it & 1) * 64, a);
                 tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float x = __shfl_sync(0xffffffffu, bq[i], lane & 15);
-                    if (hi) a[i] = x;
-                }
                 const bool tail = key0 + kLdKeys > lim0;
                 if (tail) {
-                    const int left = lim - key0 - 32 * hi;
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
-                        if (i >= left) a[i] = -INFINITY;
+                        if (key0 + (i >> 2) * 8 + kq + (i & 1) >= lim[(i >> 1) & 1]) a[i] = -INFINITY;
                 }
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float al[2];
+                bool resc = false;
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    mx[0] = fmaxf(mx[0], a[i]);
-                    mx[1] = fmaxf(mx[1], a[i + 1]);
-                    mx[2] = fmaxf(mx[2], a[i + 2]);
-                    mx[3] = fmaxf(mx[3], a[i + 3]);
-                }
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                float al = 1.f;
-                if (top > m + 8.f || m == -INFINITY) {
-                    const float mn = fmaxf(m, top);
-                    al = m == -INFINITY ? 0.f : ex2(m - mn);
-                    m = mn;
+                for (int u = 0; u < 2; ++u) {
+                    float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        x0 = max3(x0, a[4 * j + 2 * u], a[4 * j + 2 * u + 1]);
+                        x1 = max3(x1, a[4 * j + 4 + 2 * u], a[4 * j + 4 + 2 * u + 1]);
+                    }
+                    float top = fmaxf(x0, x1) * p.scale_log2;
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    al[u] = 1.f;
+                    if (top > m[u] + 8.f || m[u] == -INFINITY) {
+                        const float mn = fmaxf(m[u], top);
+                        al[u] = m[u] == -INFINITY ? 0.f : ex2(m[u] - mn);
+                        m[u] = mn;
+                        resc = resc || live_row[u];
+                    }
                 }
                 // before the unit's first product O holds nothing to rescale
-                const bool resc = t > c.t0 && al != 1.f && row < rows;
+                resc = resc && t > c.t0;
                 const bool any = bar_softmax_or(resc || fail);
                 if (any && bar_softmax_or(fail)) goto done;
-                const float mneg = m == -INFINITY ? 0.f : -m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
                 uint32_t pk[16];
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float e0 = ex2(fmaf(a[i], p.scale_log2, mneg)), e1 = ex2(fmaf(a[i + 1], p.scale_log2, mneg));
-                    sum[(i >> 1) & 3] += e0 + e1;
-                    pk[i >> 1] = Elem<T>::pack(e0, e1);
+                for (int u = 0; u < 2; ++u) {
+                    const float mneg = m[u] == -INFINITY ? 0.f : -m[u];
+                    float sum[2] = {0.f, 0.f};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float e0 = ex2(fmaf(a[4 * j + 2 * u], p.scale_log2, mneg));
+                        const float e1 = ex2(fmaf(a[4 * j + 2 * u + 1], p.scale_log2, mneg));
+                        sum[j & 1] += e0 + e1;
+                        pk[2 * j + u] = Elem<T>::pack(e0, e1);
+                    }
+                    l[u] = l[u] * al[u] + (sum[0] + sum[1]);
                 }
-                l = l * al + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
                 if (tail) {  // V rows: zeros behind the sequence, finite where some token may not look
-                    const int st = it % p.stages;
                     const int lo = max(0, lim0 - key0), nrow = kLdKeys - lo;
                     for (int i = threadIdx.x; i < nrow * lat8; i += 128) {
                         const int kr = lo + i / lat8, v = i % lat8;
@@ -475,7 +532,10 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                 if (it > 0) fail = !wait_all(smem_u32(pv_done), (it - 1) & 1, p.err) || fail;
                 if (any) {
                     tc_fence_after();
-                    if (!hi) alpha[r] = resc ? al : 1.f;
+                    if ((lane & 3) == 0) {
+                        alpha[r] = al[0];
+                        alpha[r + 8] = al[1];
+                    }
                     bar_softmax();
                     for (int col = 0; col < (LCH * 32); col += 32) {
                         float o[32];
@@ -487,29 +547,34 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                     }
                     tmem_wait_st();
                 }
+                // P: 8x8 blocks (rows +0 / +8, key blocks j and j + 1); lane i gives the address
+                // of row i % 8 of block i / 8
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(s_p + swz128(r, hi * 4 + k)), "r"(pk[4 * k]),
-                                 "r"(pk[4 * k + 1]), "r"(pk[4 * k + 2]), "r"(pk[4 * k + 3])
-                                 : "memory");
+                for (int j = 0; j < 8; j += 2)
+                    stsm_x4(s_p + swz128(warp * 16 + (lane & 15), j + (lane >> 4)), pk[2 * j], pk[2 * j + 1], pk[2 * j + 2],
+                            pk[2 * j + 3]);
                 fence_async_smem();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(p_full));
+                if (lane == 0) mbar_arrive(smem_u32(&p_full[it & 1]));
+                if (++st == p.stages) st = 0;
             }
             // the last S of this piece has been read: the next piece's queries may land
             have = advance(nx);
             if (have) load_q(nx);
-            l += __shfl_xor_sync(0xffffffffu, l, 16);
             const bool whole = c.whole();
             const int64_t row0 = static_cast<int64_t>(c.b) * rows + c.g * 64;
             const int slot = 2 * blockIdx.x + (c.t0 == 0 ? 1 : 0);
-            if (!hi) {
-                inv_l[r] = l > 0.f || l != l ? 1.f / l : 0.f;
-                if (whole) {
-                    if (p.lse && row < rows) p.lse[row0 + r] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
-                } else {
-                    p.ws_ml[slot * 64 + r] = make_float2(m, l);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+                l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+                if ((lane & 3) == 0) {
+                    const int rr = r + 8 * u;
+                    inv_l[rr] = l[u] > 0.f || l[u] != l[u] ? 1.f / l[u] : 0.f;
+                    if (!whole) p.ws_ml[slot * 64 + rr] = make_float2(m[u], l[u]);
+                    else if (p.lse && live_row[u])
+                        p.lse[row0 + rr] = l[u] == 0.f ? -INFINITY : (m[u] + log2f(l[u])) * 0.69314718055994531f;
                 }
             }
             if (threadIdx.x == 0 && c.t0 == 0) {
@@ -714,6 +779,7 @@ extern "C" vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* 
     p.lse = lse;
     p.bt = block_tables;
     p.lens = seq_lens;
+    p.layer_base = pool->base + static_cast<uint64_t>(layer) * pool->seg_stride;
     p.err = pool->d_err;
     p.bt_stride = bt_stride;
     p.B = batch;
@@ -727,7 +793,7 @@ extern "C" vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* 
     p.rope = pool->rope_dim;
     p.nch = p.latent / 64 + 1;
     const int stage = p.nch * kLdChunk;
-    p.stages = (kLdSmemMax - 1024 - kLdAux - kLdChunk - stage) / stage;
+    p.stages = (kLdSmemMax - 1024 - kLdAux - kLdChunk - stage) / stage;  // 2, 2, 4, 7 at 512, 384, 256, 128
     if (p.stages > kLdMaxStages) p.stages = kLdMaxStages;
     p.scale_log2 = scale * 1.4426950408889634f;
     const size_t slots = 2 * static_cast<size_t>(pool->num_sms);

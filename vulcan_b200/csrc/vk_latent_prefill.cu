@@ -242,12 +242,6 @@ constexpr int kLaBar = kLaRing + kLaUnits * kLpUnit;  // 224 KiB
 constexpr int kLaSmem = kLaBar + 256 + 1024;
 static_assert(kLaSmem <= kLpSmemMax, "latent prefill shared memory");
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __grid_constant__ CUtensorMap tmap,
                                                                        const __grid_constant__ CUtensorMap tmapq,
