@@ -13,8 +13,8 @@
 // graph replays with other lengths).  A unit that several CTAs share leaves
 // fp32 partials (O, m, l) that latent_merge_kernel joins.
 //
-//  * warp 4 streams tiles with 2-D TMA boxes (64 elements x one page's rows,
-//    128-byte swizzle) into a ring of as many stages as fit (2 at 512 + 64);
+//  * warps 4 and 7-10 stream tiles with 2-D TMA boxes (64 elements x one page's
+//    rows, 128-byte swizzle) into a ring of as many stages as fit (2 at 512 + 64);
 //  * warp 5 issues  S[64 rows x 64 keys] = Q K^T  (tcgen05.mma, M 64, K-major
 //    both) and warp 6  O^T[latent x 64 rows] += V^T P^T  as M = 128 blocks of
 //    latent elements: an MMA costs its thread 40-60 cycles to issue, more than the
@@ -46,7 +46,7 @@
 namespace vk {
 
 constexpr int kLdKeys = 64;       // keys of a tile
-constexpr int kLdThreads = 224;   // 4 softmax warps, TMA warp, two MMA warps
+constexpr int kLdThreads = 352;   // 4 softmax warps, five TMA warps, two MMA warps
 constexpr int kLdMaxStages = 8;
 constexpr int kLdParts = 5;       // barriers of a stage: pairs of chunks of the latent, the rotary chunk
 constexpr int kLdChunk = kLdKeys * 128;  // 64 keys x 64 elements, 128-byte rows
@@ -57,9 +57,6 @@ constexpr int kLdUnitCost = 2;
 // Least cost of a CTA's range: fewer, longer pieces when there is little work
 constexpr int kLdMinRange = 4;
 
-// Tiles of L2 prefetch ahead of the ring.
-constexpr int kLdAhead = 3;
-
 struct LdParams {
     const char* ql;
     const char* qr;
@@ -68,9 +65,8 @@ struct LdParams {
     float* lse;
     const int32_t* bt;
     const int32_t* lens;
-    const char* layer_base;  // the pool's rows of this layer
     uint32_t* err;
-    float* ws_o;     // [2 * CTAs][64][latent]
+    float4* ws_o;    // partial O: ld_part()
     float2* ws_ml;   // [2 * CTAs][64]: maximum (log2 domain), sum
     int2* ws_unit;   // [units]: first and last CTA of a split unit, or (-1, -1)
     int bt_stride, B, T, H, groups, layer, num_pages, P, latent, rope, nch, stages;
@@ -126,6 +122,13 @@ struct LdWalk {
     }
 };
 
+// Partial O of a slot as [16 row quads][latent / 128][128 elements] of four rows
+// each: what a thread reads from TMEM, stored and loaded 16 bytes at a time.
+template <int LCH>
+__device__ __forceinline__ int64_t ld_part(int slot, int quad, int mb, int d) {
+    return ((static_cast<int64_t>(slot) * 16 + quad) * (LCH / 2) + mb) * 128 + d;
+}
+
 __device__ __forceinline__ void bar_softmax() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ bool bar_softmax_or(bool x) {
     uint32_t r;
@@ -172,26 +175,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 6);
     float* alpha = reinterpret_cast<float*>(aux + 768);   // [64] rescale factors
     float* inv_l = reinterpret_cast<float*>(aux + 1024);  // [64]
-    int64_t* sched = reinterpret_cast<int64_t*>(aux + 1280);  // first b, its start; then warp sums
-    int64_t* wsum = sched + 4;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    // ---- the deal: cost of every sequence from the device's lengths, a block scan, this CTA's start
-    const int per = (p.B + kLdThreads - 1) / kLdThreads;
-    const int b_lo = threadIdx.x * per, b_hi = min(p.B, b_lo + per);
-    int64_t mine = 0;
-    for (int b = b_lo; b < b_hi; ++b) {
-        const int len = ld_len(p, b);
-        mine += static_cast<int64_t>(p.groups) * ((len + kLdKeys - 1) / kLdKeys + kLdUnitCost);
-        if (blockIdx.x == 0 && len != __ldg(p.lens + b)) atomicOr(p.err, VK_ERR_SEQ_LEN);
-    }
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-    }
-    if (lane == 31) wsum[warp] = incl;
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages * kLdParts; ++i) {
             mbar_init(smem_u32(&k_full[i]), 1);
@@ -205,28 +190,42 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         mbar_init(smem_u32(q_full), 4);
         mbar_fence_init();
     }
-    __syncthreads();
-    int64_t total = 0, before = incl - mine;
-    for (int w = 0; w < kLdThreads / 32; ++w) {
-        total += wsum[w];
-        if (w < warp) before += wsum[w];
+    // ---- the deal, by every warp for itself: the sequences' costs from the device's
+    // lengths, their prefix sums, this CTA's range and the unit it starts in
+    const int per = (p.B + 31) >> 5, b_lo = min(p.B, lane * per), b_hi = min(p.B, b_lo + per);
+    int64_t mine = 0;
+#pragma unroll 4
+    for (int b = b_lo; b < b_hi; ++b)
+        mine += static_cast<int64_t>(p.groups) * ((ld_len(p, b) + kLdKeys - 1) / kLdKeys + kLdUnitCost);
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
     }
+    const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
     const int64_t n = min(static_cast<int64_t>(gridDim.x), (total + kLdMinRange - 1) / kLdMinRange);
     if (blockIdx.x >= n) return;  // the whole CTA: nothing allocated yet
     LdWalk walk0;
     walk0.v = blockIdx.x * total / n;
     walk0.v1 = (blockIdx.x + 1) * total / n;
-    if (walk0.v >= before && walk0.v < before + mine) {  // one thread: it finds the first unit
-        int64_t at = before;
-        int b = b_lo;
+    {
+        const int src = __ffs(__ballot_sync(0xffffffffu, walk0.v < upto)) - 1;
+        int64_t at = __shfl_sync(0xffffffffu, upto - mine, src);
+        int b = src * per;
         for (;; ++b) {
-            const int64_t c = static_cast<int64_t>(p.groups) * ((ld_len(p, b) + kLdKeys - 1) / kLdKeys + kLdUnitCost);
+            walk0.len = ld_len(p, b);
+            walk0.tiles = (walk0.len + kLdKeys - 1) / kLdKeys;
+            const int64_t c = static_cast<int64_t>(p.groups) * (walk0.tiles + kLdUnitCost);
             if (walk0.v < at + c) break;
             at += c;
         }
-        sched[0] = b;
-        sched[1] = at;
+        const int span = walk0.tiles + kLdUnitCost;
+        walk0.b = b;
+        walk0.g = p.groups > 1 ? static_cast<int>((walk0.v - at) / span) : 0;
+        walk0.unit_start = at + static_cast<int64_t>(walk0.g) * span;
     }
+    const int rows = p.T * p.H;
     if (warp == 5) {
         tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
@@ -235,68 +234,52 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    walk0.b = static_cast<int>(sched[0]);
-    walk0.len = ld_len(p, walk0.b);
-    walk0.tiles = (walk0.len + kLdKeys - 1) / kLdKeys;
-    {
-        const int64_t span = walk0.tiles + kLdUnitCost;
-        walk0.g = static_cast<int>((walk0.v - sched[1]) / span);
-        walk0.unit_start = sched[1] + walk0.g * span;
-    }
-    const int rows = p.T * p.H;
 
-    if (warp == 4) {
-        // ------------------------------------------------------------ TMA producer
+    if (warp == 4 || (warp >= 7 && warp <= 6 + LCH / 2)) {
+        const int g = warp == 4 ? 0 : warp - 6;
+        // ------------------------------------------------------------ TMA producers
+        // Warp g of five brings part g of every tile (two chunks of 64 elements, the
+        // rotary chunk last): a part of 16-token pages takes eight copies, ~70 cycles
+        // each to issue, and all 36 of a tile from one warp took longer than the tile
+        // (24 x 16k tokens: 116 us with one issuing warp, 96 with five).
         LdWalk w = walk0;
         LdPiece c;
         int st = 0;
-        uint32_t ph = 1;  // parity of the stage's release before this fill (first round: none)
-        bool ok = true;
+        uint32_t ph = 1;      // parity of the stage's release before this fill
+        bool ok = true, filled = false;  // filled: every stage has been, releases to wait for
         if (lane == 0) prefetch_tmap(&tmap);
         const uint64_t pol = p.groups > 1 ? l2_evict_last_policy() : l2_evict_first_policy();
         const int ppt = kLdKeys / p.P;  // pages of a full tile
-        const uint32_t page_bytes = p.P * 2 * (LCH * 64 + p.rope);
-        bool filled = false;  // every stage has been filled once
+        const int chunks = g < LCH / 2 ? 2 : 1, i = lane >> 1;  // lane: page i of the tile, chunk lane % 2 of the part
         while (ok && w.next_real(p, c)) {
             const int32_t* row = p.bt + static_cast<int64_t>(c.b) * p.bt_stride;
-            const int npages = (c.len + p.P - 1) / p.P, pend = min(npages, c.t1 * ppt);  // this piece's pages end
-            int win = c.t0 * ppt, entry = 0;  // block-table entries win..win+31, one a lane
-            int fetched = win;                // pages before this one are on their way to L2
-            auto load_window = [&]() {
-                entry = win + lane < npages ? __ldg(row + win + lane) : 0;
-                if (entry < 0 || entry >= p.num_pages) {
+            const int npages = (c.len + p.P - 1) / p.P;
+            // block-table entries win .. win+63, two a lane
+            int win = c.t0 * ppt;
+            auto entry = [&](int k) {
+                int e = k < npages ? __ldg(row + k) : 0;
+                if (e < 0 || e >= p.num_pages) {
                     atomicOr(p.err, VK_ERR_PAGE_ID);
-                    entry = 0;
+                    e = 0;
                 }
+                return e;
             };
-            load_window();
+            int e0 = entry(win + lane), e1 = entry(win + 32 + lane);
             for (int t = c.t0; t < c.t1 && ok; ++t) {
                 const int first = t * ppt, cnt = min(ppt, npages - first);
-                if (first + cnt > win + 32) {
-                    win = first;
-                    load_window();
+                if (first + cnt > win + 32) {  // tiles do not straddle windows: 32 is a multiple of ppt
+                    win += 32;
+                    e0 = e1;
+                    e1 = entry(win + 32 + lane);
                 }
-                // L2 prefetch up to kLdAhead tiles ahead (within the window): the ring holds
-                // two tiles, too few bytes in flight to cover HBM's latency
-                const int to = min(min(pend, (t + 1 + kLdAhead) * ppt), win + 32);
-                if (win + lane >= fetched && win + lane < to)
-                    l2_prefetch(p.layer_base + static_cast<uint64_t>(entry) * page_bytes, page_bytes);
-                fetched = max(fetched, to);
-                const uint32_t dst = sbase + st * stage_bytes;
-                const int i = lane >> 1, page = __shfl_sync(0xffffffffu, entry, first - win + min(i, cnt - 1));
-                const int y = (p.layer * p.num_pages + page) * p.P;
-                const uint32_t dst_i = dst + (lane & 1) * kLdChunk + i * p.P * 128;
-                const uint32_t part_bytes = cnt * p.P * 128;
-#pragma unroll
-                for (int g = 0; g <= LCH / 2; ++g) {  // two chunks of 64 elements a part, the rotary chunk last
-                    if (filled) ok = ok && wait_all(smem_u32(&k_empty[st * kLdParts + g]), ph, p.err);
-                    if (!ok) break;
-                    const uint32_t bar = smem_u32(&k_full[st * kLdParts + g]);
-                    const int chunks = g < LCH / 2 ? 2 : 1;
-                    if (lane == 0) mbar_expect_tx(bar, chunks * part_bytes);
-                    if (i < cnt && (lane & 1) < chunks)
-                        tma_load_2d(dst_i + 2 * g * kLdChunk, &tmap, (2 * g + (lane & 1)) * 64, y, bar, pol);
-                }
+                const int page = __shfl_sync(0xffffffffu, e0, (first - win + min(i, cnt - 1)) & 31);
+                if (filled) ok = wait_all(smem_u32(&k_empty[st * kLdParts + g]), ph, p.err);
+                if (!ok) break;
+                const uint32_t bar = smem_u32(&k_full[st * kLdParts + g]);
+                if (lane == 0) mbar_expect_tx(bar, chunks * cnt * p.P * 128);
+                if (i < cnt && (lane & 1) < chunks)
+                    tma_load_2d(sbase + st * stage_bytes + (2 * g + (lane & 1)) * kLdChunk + i * p.P * 128, &tmap,
+                                (2 * g + (lane & 1)) * 64, (p.layer * p.num_pages + page) * p.P, bar, pol);
                 if (++st == p.stages) {
                     st = 0;
                     ph ^= 1;
@@ -392,7 +375,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                 }
             }
         }
-    } else {
+    } else if (warp < 4) {
         // ------------------------------------------------------------ softmax and output
         LdWalk w = walk0;
         LdPiece c, nx;
@@ -401,6 +384,9 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
         const int rope8 = p.rope >> 3, lat8 = LCH * 8;
 
+        if (blockIdx.x == 0)
+            for (int b = threadIdx.x; b < p.B; b += 128)
+                if (__ldg(p.lens + b) != ld_len(p, b)) atomicOr(p.err, VK_ERR_SEQ_LEN);
         // next piece with tiles; rows of empty units are written on the way
         auto advance = [&](LdPiece& o) -> bool {
             while (w.next(p, o)) {
@@ -587,34 +573,59 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
             if (bar_softmax_or(fail)) goto done;
             tc_fence_after();
             const int live = min(64, rows - c.g * 64);
-            for (int mb = 0; mb < LCH / 2; ++mb)
+            // rolled loops: a CTA runs this once or twice, and unrolled code would arrive
+            // through cold instruction fetches
+#pragma unroll 1
+            for (int k = 0; k < LCH; ++k) {
+                const int mb = k >> 1, hc = k & 1;  // 128 latent elements, 32 rows
+                if (hc * 32 >= live) continue;
+                if (whole) {
+                    // O^T fragments, scaled, transposed on the way to shared memory (P's
+                    // buffer: [32 rows][128 elements], 16-byte chunks XOR row % 8)
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        float o[16];
+                        tmem_ld_16x32(lane_base + (static_cast<uint32_t>(half * 16) << 16) + mb * 64 + hc * 32, o);
+                        tmem_wait_ld();
+                        uint32_t w2[8];
 #pragma unroll
-                for (int hc = 0; hc < 2; ++hc) {
-                    if (hc * 32 >= live) break;
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 i2 = *reinterpret_cast<const float2*>(inv_l + hc * 32 + 8 * j + kq);
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+                                w2[2 * j + u] = Elem<T>::pack(i2.x == 0.f ? 0.f : o[4 * j + 2 * u] * i2.x,
+                                                              i2.y == 0.f ? 0.f : o[4 * j + 2 * u + 1] * i2.y);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; j += 2) {
+                            const int rr = 8 * (j + (lane >> 4)) + (lane & 7), ch = warp * 4 + half * 2 + ((lane >> 3) & 1);
+                            stsm_x4_t(s_p + rr * 256 + ((ch ^ (rr & 7)) << 4), w2[2 * j], w2[2 * j + 1], w2[2 * j + 2], w2[2 * j + 3]);
+                        }
+                    }
+                    bar_softmax();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int rr = (threadIdx.x >> 4) + 8 * i, ch = threadIdx.x & 15;
+                        uint4 x;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                                     : "r"(s_p + rr * 256 + ((ch ^ (rr & 7)) << 4)));
+                        if (hc * 32 + rr < live)
+                            *reinterpret_cast<uint4*>(p.out + 2 * ((row0 + hc * 32 + rr) * (LCH * 64) + mb * 128) + ch * 16) = x;
+                    }
+                    bar_softmax();
+                } else {
+                    // four rows of one latent element a 16-byte store (ld_part)
                     float o[32];
                     tmem_ld32(lane_base + mb * 64 + hc * 32, o);
                     tmem_wait_ld();
-                    const int d = mb * 128 + warp * 32 + lane;
-                    if (whole) {
-                        // neighbouring lanes hold neighbouring elements: they trade so that each
-                        // stores two elements of one row
+                    float4* dst = p.ws_o + ld_part<LCH>(slot, hc * 8, mb, warp * 32 + lane);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float i0 = inv_l[hc * 32 + i], i1 = inv_l[hc * 32 + i + 1];
-                            const float x0 = i0 == 0.f ? 0.f : o[i] * i0, x1 = i1 == 0.f ? 0.f : o[i + 1] * i1;
-                            const float got = __shfl_xor_sync(0xffffffffu, lane & 1 ? x0 : x1, 1);
-                            const int rr = hc * 32 + i + (lane & 1);
-                            const uint32_t wv = lane & 1 ? Elem<T>::pack(got, x1) : Elem<T>::pack(x0, got);
-                            if (rr < live)
-                                *reinterpret_cast<uint32_t*>(p.out + 2 * ((row0 + rr) * p.latent + (d & ~1))) = wv;
-                        }
-                    } else {
-                        float* dst = p.ws_o + (static_cast<int64_t>(slot) * 64 + hc * 32) * p.latent + d;
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (hc * 32 + i < live) dst[static_cast<int64_t>(i) * p.latent] = o[i];
-                    }
+                    for (int i = 0; i < 8; ++i)
+                        if (hc * 32 + 4 * i < live)
+                            dst[i * (LCH / 2) * 128] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 }
+            }
             tc_fence_before();
             c = nx;
         }
@@ -627,113 +638,118 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
     }
 }
 
-// Joins the partials of units that several CTAs share.  Block (row, unit):
-// its warps take the unit's pieces in turn, then meet in shared memory; the
-// order of the sums is fixed by the pieces, so results repeat bit for bit.
-template <typename T>
-__global__ void latent_merge_kernel(const LdParams p) {
-    extern __shared__ float part[];  // [warps][latent]
-    __shared__ float lsum[32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+// Joins the partials of units that several CTAs share.  Block (unit, row quad x
+// 128 latent elements): a thread has one element of four rows; `groups` groups
+// of 128 threads take the pieces in turn and meet in shared memory.  The order of
+// the sums is fixed by the pieces, so results repeat bit for bit.
+constexpr int kLdMergeGroups = 8;
+template <typename T, int LCH>
+__global__ void __launch_bounds__(128 * kLdMergeGroups) latent_merge_kernel(const __grid_constant__ LdParams p) {
+    __shared__ float4 part[kLdMergeGroups][128];
+    __shared__ float4 part_l[kLdMergeGroups];
+    const int lane = threadIdx.x & 31, d = threadIdx.x & 127, kg = threadIdx.x >> 7, kgs = blockDim.x >> 7;
     const int64_t unit = blockIdx.x;
+    const int quad = blockIdx.y / (LCH / 2), mb = blockIdx.y % (LCH / 2);
     const int b = static_cast<int>(unit / p.groups), g = static_cast<int>(unit % p.groups);
-    const int r = blockIdx.y, rows = p.T * p.H;
-    if (g * 64 + r >= rows) return;
+    const int rows = p.T * p.H, row_in = g * 64 + quad * 4;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int2 u = p.ws_unit[unit];
-    if (u.x < 0) return;
+    if (u.x < 0 || row_in >= rows) return;
     // piece i of CTA u.x + i: the first tile's piece in the odd slot, the others in even ones
     auto slot_of = [&](int i) { return 2 * (u.x + i) + (i == 0 ? 1 : 0); };
     const int pieces = u.y - u.x + 1;
-    float m = -INFINITY;
-    for (int i = lane; i < pieces; i += 32) m = fmaxf(m, p.ws_ml[slot_of(i) * 64 + r].x);
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    for (int i = lane; i < pieces; i += 32) {
+        const float4* ml = reinterpret_cast<const float4*>(p.ws_ml + slot_of(i) * 64 + quad * 4);
+        const float4 x = ml[0], y = ml[1];
+        m[0] = fmaxf(m[0], x.x);
+        m[1] = fmaxf(m[1], x.z);
+        m[2] = fmaxf(m[2], y.x);
+        m[3] = fmaxf(m[3], y.z);
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float mref = m == -INFINITY ? 0.f : m;
-    const int nv = p.latent >> 7;  // float4 a lane
-    float4 acc[4];
+    for (int k = 0; k < 4; ++k) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
+        for (int o = 16; o > 0; o >>= 1) m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
+    }
+    auto weight = [&](float mi, int k) { return ex2(mi - (m[k] == -INFINITY ? 0.f : m[k])); };
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f), l = acc;
 #pragma unroll 4
-    for (int i = warp; i < pieces; i += warps) {
+    for (int i = kg; i < pieces; i += kgs) {
         const int slot = slot_of(i);
-        const float2 ml = p.ws_ml[slot * 64 + r];
-        const float f = ex2(ml.x - mref);
-        const float4* src = reinterpret_cast<const float4*>(p.ws_o + (static_cast<int64_t>(slot) * 64 + r) * p.latent);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < nv) {
-                const float4 x = src[k * 32 + lane];
-                // a piece whose keys this row may not see has f = l = 0
-                acc[k].x = fmaf(f, x.x, acc[k].x);
-                acc[k].y = fmaf(f, x.y, acc[k].y);
-                acc[k].z = fmaf(f, x.z, acc[k].z);
-                acc[k].w = fmaf(f, x.w, acc[k].w);
-            }
-        l = fmaf(f, ml.y, l);
+        const float4 o = p.ws_o[ld_part<LCH>(slot, quad, mb, d)];
+        const float4* ml = reinterpret_cast<const float4*>(p.ws_ml + slot * 64 + quad * 4);
+        const float4 x = ml[0], y = ml[1];
+        // a piece whose keys a row may not see has weight, O and l of zero
+        const float f0 = weight(x.x, 0), f1 = weight(x.z, 1), f2 = weight(y.x, 2), f3 = weight(y.z, 3);
+        acc = make_float4(fmaf(f0, o.x, acc.x), fmaf(f1, o.y, acc.y), fmaf(f2, o.z, acc.z), fmaf(f3, o.w, acc.w));
+        l = make_float4(fmaf(f0, x.y, l.x), fmaf(f1, x.w, l.y), fmaf(f2, y.y, l.z), fmaf(f3, y.w, l.w));
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (k < nv) *reinterpret_cast<float4*>(part + warp * p.latent + (k * 32 + lane) * 4) = acc[k];
-    if (lane == 0) lsum[warp] = l;
-    __syncthreads();
-    float lt = 0.f;
-    for (int w = 0; w < warps; ++w) lt += lsum[w];
-    const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
-    const int64_t row = static_cast<int64_t>(b) * rows + g * 64 + r;
-    for (int d = threadIdx.x * 2; d < p.latent; d += blockDim.x * 2) {
-        float2 x = make_float2(0.f, 0.f);
-        for (int w = 0; w < warps; ++w) {
-            const float2 y = *reinterpret_cast<const float2*>(part + w * p.latent + d);
-            x.x += y.x;
-            x.y += y.y;
+    if (kgs > 1) {
+        part[kg][d] = acc;
+        if (d == 0) part_l[kg] = l;
+        __syncthreads();
+        if (kg) return;
+        acc = part[0][d];
+        l = part_l[0];
+        for (int k = 1; k < kgs; ++k) {
+            const float4 a = part[k][d], c = part_l[k];
+            acc = make_float4(acc.x + a.x, acc.y + a.y, acc.z + a.z, acc.w + a.w);
+            l = make_float4(l.x + c.x, l.y + c.y, l.z + c.z, l.w + c.w);
         }
-        *reinterpret_cast<uint32_t*>(p.out + 2 * (row * p.latent + d)) =
-            Elem<T>::pack(inv == 0.f ? 0.f : x.x * inv, inv == 0.f ? 0.f : x.y * inv);
     }
-    if (p.lse && threadIdx.x == 0) p.lse[row] = lt == 0.f ? -INFINITY : (m + log2f(lt)) * 0.69314718055994531f;
+    const int64_t row = static_cast<int64_t>(b) * rows + row_in;
+    const float av[4] = {acc.x, acc.y, acc.z, acc.w}, lv[4] = {l.x, l.y, l.z, l.w};
+    T* out = reinterpret_cast<T*>(p.out) + row * (LCH * 64) + mb * 128 + d;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (row_in + k >= rows) break;
+        out[k * LCH * 64] = Elem<T>::down(lv[k] > 0.f || lv[k] != lv[k] ? av[k] / lv[k] : 0.f);
+        if (p.lse && mb == 0 && d == 0) p.lse[row + k] = lv[k] == 0.f ? -INFINITY : (m[k] + log2f(lv[k])) * 0.69314718055994531f;
+    }
 }
 
 static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 template <typename T, int LCH>
-static cudaError_t launch_latent_split(vk_pool* pool, const LdParams& p, cudaStream_t st) {
+static vk_status launch_latent_decode(vk_pool* pool, const LdParams& p, cudaStream_t st) {
     static uint64_t attr_set = 0;
     const uint64_t bit = 1ull << (pool->device & 63);
     const size_t smem = static_cast<size_t>(p.stages + 1) * p.nch * kLdChunk + kLdChunk + kLdAux + 1024;
+    cudaError_t e = cudaSuccess;
     if (!(attr_set & bit)) {
-        cudaError_t e = cudaFuncSetAttribute(latent_decode_kernel<T, LCH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLdSmemMax);
-        if (e != cudaSuccess) return e;
+        e = cudaFuncSetAttribute(latent_decode_kernel<T, LCH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLdSmemMax);
+        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(latent_decode)");
         attr_set |= bit;
     }
     latent_decode_kernel<T, LCH><<<pool->num_sms, kLdThreads, smem, st>>>(pool->tmap16, p);
-    return cudaGetLastError();
-}
-
-template <typename T>
-static vk_status launch_latent_decode(vk_pool* pool, const LdParams& p, cudaStream_t st) {
-    cudaError_t e = p.latent == 512   ? launch_latent_split<T, 8>(pool, p, st)
-                    : p.latent == 384 ? launch_latent_split<T, 6>(pool, p, st)
-                    : p.latent == 256 ? launch_latent_split<T, 4>(pool, p, st)
-                                      : launch_latent_split<T, 2>(pool, p, st);
+    e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "latent_decode_kernel launch");
-    // few rows: many pieces each, so more warps share a row's pieces
     const int64_t units = static_cast<int64_t>(p.B) * p.groups;
-    const int rows = min(64, p.T * p.H);
-    const int warps = units * rows <= 4 * pool->num_sms ? 16 : 4;
+    const int quads = (min(64, p.T * p.H) + 3) / 4;
+    // few blocks: few units, so many pieces each, which more groups share
+    const int groups = units * quads * (LCH / 2) <= 4 * pool->num_sms ? kLdMergeGroups : 1;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(rows));
-    cfg.blockDim = dim3(warps * 32);
-    cfg.dynamicSmemBytes = static_cast<size_t>(warps) * p.latent * 4;
+    cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(quads * (LCH / 2)));
+    cfg.blockDim = dim3(groups * 128);
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, latent_merge_kernel<T>, p);
+    e = cudaLaunchKernelEx(&cfg, latent_merge_kernel<T, LCH>, p);
     return e == cudaSuccess ? VK_OK : cuda_fail(e, "latent_merge_kernel launch");
+}
+
+template <typename T>
+static vk_status launch_latent_decode(vk_pool* pool, const LdParams& p, cudaStream_t st) {
+    switch (pool->latent_dim) {
+        case 512: return launch_latent_decode<T, 8>(pool, p, st);
+        case 384: return launch_latent_decode<T, 6>(pool, p, st);
+        case 256: return launch_latent_decode<T, 4>(pool, p, st);
+        default: return launch_latent_decode<T, 2>(pool, p, st);
+    }
 }
 
 }  // namespace vk
@@ -779,7 +795,6 @@ extern "C" vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* 
     p.lse = lse;
     p.bt = block_tables;
     p.lens = seq_lens;
-    p.layer_base = pool->base + static_cast<uint64_t>(layer) * pool->seg_stride;
     p.err = pool->d_err;
     p.bt_stride = bt_stride;
     p.B = batch;
@@ -798,7 +813,7 @@ extern "C" vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* 
     p.scale_log2 = scale * 1.4426950408889634f;
     const size_t slots = 2 * static_cast<size_t>(pool->num_sms);
     char* ws = static_cast<char*>(workspace);
-    p.ws_o = reinterpret_cast<float*>(ws);
+    p.ws_o = reinterpret_cast<float4*>(ws);
     ws += align256(slots * 64 * p.latent * 4);
     p.ws_ml = reinterpret_cast<float2*>(ws);
     ws += align256(slots * 64 * 8);
