@@ -13,7 +13,7 @@
 // graph replays with other lengths).  A unit that several CTAs share leaves
 // fp32 partials (O, m, l) that latent_merge_kernel joins.
 //
-//  * warps 4 and 7-10 stream tiles with 2-D TMA boxes (64 elements x one page's
+//  * warps 4 and 7-9 stream tiles with 2-D TMA boxes (64 elements x one page's
 //    rows, 128-byte swizzle) into a ring of as many stages as fit (2 at 512 + 64);
 //  * warp 5 issues  S[64 rows x 64 keys] = Q K^T  (tcgen05.mma, M 64, K-major
 //    both) and warp 6  O^T[latent x 64 rows] += V^T P^T  as M = 128 blocks of
@@ -46,7 +46,7 @@
 namespace vk {
 
 constexpr int kLdKeys = 64;       // keys of a tile
-constexpr int kLdThreads = 352;   // 4 softmax warps, five TMA warps, two MMA warps
+constexpr int kLdThreads = 320;   // 4 softmax warps, four TMA warps, two MMA warps
 constexpr int kLdMaxStages = 8;
 constexpr int kLdParts = 5;       // barriers of a stage: pairs of chunks of the latent, the rotary chunk
 constexpr int kLdChunk = kLdKeys * 128;  // 64 keys x 64 elements, 128-byte rows
@@ -77,6 +77,26 @@ __device__ __forceinline__ int ld_len(const LdParams& p, int b) {
     const int len = __ldg(p.lens + b);
     return len < 0 || len > static_cast<int64_t>(p.bt_stride) * p.P ? 0 : len;
 }
+
+// n CTAs share `total`: the first `rem` take q + 1, the others q.  (64-bit
+// divisions cost hundreds of cycles of every launch; totals below 2^32 need none.)
+struct LdDeal {
+    int64_t q, rem;
+    int n;
+    __device__ __forceinline__ LdDeal(int64_t total, int ctas) {
+        n = static_cast<int>(min(static_cast<int64_t>(ctas), (total + kLdMinRange - 1) / kLdMinRange));
+        q = div(total, n);
+        rem = total - q * n;
+    }
+    static __device__ __forceinline__ int64_t div(int64_t a, int64_t b) {
+        return (a | b) >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+    }
+    __device__ __forceinline__ int64_t start(int c) const { return c * q + min(static_cast<int64_t>(c), rem); }
+    __device__ __forceinline__ int owner(int64_t v) const {  // the CTA whose range holds v
+        const int64_t head = rem * (q + 1);
+        return static_cast<int>(v < head ? div(v, q + 1) : rem + div(v - head, q));
+    }
+};
 
 struct LdPiece {
     int b, g, t0, t1, tiles, len;
@@ -204,11 +224,11 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         if (lane >= o) upto += up;
     }
     const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
-    const int64_t n = min(static_cast<int64_t>(gridDim.x), (total + kLdMinRange - 1) / kLdMinRange);
-    if (blockIdx.x >= n) return;  // the whole CTA: nothing allocated yet
+    const LdDeal deal(total, gridDim.x);
+    if (static_cast<int>(blockIdx.x) >= deal.n) return;  // the whole CTA: nothing allocated yet
     LdWalk walk0;
-    walk0.v = blockIdx.x * total / n;
-    walk0.v1 = (blockIdx.x + 1) * total / n;
+    walk0.v = deal.start(blockIdx.x);
+    walk0.v1 = deal.start(blockIdx.x + 1);
     {
         const int src = __ffs(__ballot_sync(0xffffffffu, walk0.v < upto)) - 1;
         int64_t at = __shfl_sync(0xffffffffu, upto - mine, src);
@@ -225,8 +245,62 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         walk0.g = p.groups > 1 ? static_cast<int>((walk0.v - at) / span) : 0;
         walk0.unit_start = at + static_cast<int64_t>(walk0.g) * span;
     }
-    const int rows = p.T * p.H;
-    if (warp == 5) {
+    const int rows = p.T * p.H, rope8 = p.rope >> 3, lat8 = LCH * 8;
+    LdWalk w = walk0;  // every role walks the CTA's pieces for itself
+    LdPiece c;
+            // next piece with tiles; rows of empty units are written on the way
+            auto advance = [&](LdPiece& o) -> bool {
+                while (w.next(p, o)) {
+                    if (o.t0 < o.t1) return true;
+                    const int live = min(64, rows - o.g * 64);
+                    const int64_t row0 = static_cast<int64_t>(o.b) * rows + o.g * 64;
+                    uint4* dst = reinterpret_cast<uint4*>(p.out + 2 * row0 * p.latent);
+                    for (int i = threadIdx.x; i < live * lat8; i += 128) dst[i] = make_uint4(0, 0, 0, 0);
+                    if (p.lse && threadIdx.x < live) p.lse[row0 + threadIdx.x] = -INFINITY;
+                    if (threadIdx.x == 0) p.ws_unit[static_cast<int64_t>(o.b) * p.groups + o.g] = make_int2(-1, -1);
+                }
+                return false;
+            };
+            // 16 rows a warp, a row's 16-byte vectors across the lanes; one division per
+            // piece, then (token, head) step along
+            auto load_q = [&](const LdPiece& o) {
+                int t = (o.g * 64 + warp * 16) / p.H, h = (o.g * 64 + warp * 16) % p.H;
+                const char* ql = p.ql + 2 * ((static_cast<int64_t>(o.b) * p.T + t) * p.ql_token + h * p.ql_head) + lane * 16;
+                const char* qr = p.qr + 2 * ((static_cast<int64_t>(o.b) * p.T + t) * p.qr_token + h * p.qr_head) + lane * 16;
+                const int live = rows - o.g * 64 - warp * 16;  // rows of this warp that exist
+    #pragma unroll 4
+                for (int k = 0; k < 16; ++k) {
+                    const bool on = k < live;
+                    const uint32_t dst = s_q + swz128(warp * 16 + k, lane & 7) + (lane >> 3) * kLdChunk;
+    #pragma unroll
+                    for (int i = 0; i < (LCH + 3) / 4; ++i)
+                        if (lane + 32 * i < LCH * 8) cp_async16(dst + i * 4 * kLdChunk, on ? ql + i * 512 : p.ql, on);
+                    if (lane < rope8)
+                        cp_async16(s_q + LCH * kLdChunk + swz128(warp * 16 + k, lane), on ? qr : p.qr, on);
+                    ql += 2 * p.ql_head;
+                    qr += 2 * p.qr_head;
+                    if (++h == p.H) {
+                        h = 0;
+                        ++t;
+                        ql += 2 * (p.ql_token - p.H * p.ql_head);
+                        qr += 2 * (p.qr_token - p.H * p.qr_head);
+                    }
+                }
+            };
+            auto q_landed = [&]() {
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(q_full));
+            };
+
+    // The first queries are on their way before any tile is: behind the tiles of all
+    // SMs they took 2 us longer to arrive.
+    bool have = false;
+    if (warp < 4) {
+        have = advance(c);
+        if (have) load_q(c);
+    } else if (warp == 5) {
         tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
     }
@@ -235,22 +309,20 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 4 || (warp >= 7 && warp <= 6 + LCH / 2)) {
+    if (warp == 4 || (warp >= 7 && warp <= 5 + LCH / 2)) {
         const int g = warp == 4 ? 0 : warp - 6;
         // ------------------------------------------------------------ TMA producers
-        // Warp g of five brings part g of every tile (two chunks of 64 elements, the
-        // rotary chunk last): a part of 16-token pages takes eight copies, ~70 cycles
-        // each to issue, and all 36 of a tile from one warp took longer than the tile
-        // (24 x 16k tokens: 116 us with one issuing warp, 96 with five).
-        LdWalk w = walk0;
-        LdPiece c;
+        // Warp g of latent / 128 brings part g of every tile (two chunks of 64 elements;
+        // the first warp the rotary chunk too): a part of 16-token pages takes eight
+        // copies, ~70 cycles each to issue, and all 36 of a tile from one warp took
+        // longer than the tile (24 x 16k tokens: 116 us with one warp, 96 with several).
         int st = 0;
         uint32_t ph = 1;      // parity of the stage's release before this fill
         bool ok = true, filled = false;  // filled: every stage has been, releases to wait for
         if (lane == 0) prefetch_tmap(&tmap);
         const uint64_t pol = p.groups > 1 ? l2_evict_last_policy() : l2_evict_first_policy();
         const int ppt = kLdKeys / p.P;  // pages of a full tile
-        const int chunks = g < LCH / 2 ? 2 : 1, i = lane >> 1;  // lane: page i of the tile, chunk lane % 2 of the part
+        const int i = lane >> 1;  // lane: page i of the tile, chunk lane % 2 of the part
         while (ok && w.next_real(p, c)) {
             const int32_t* row = p.bt + static_cast<int64_t>(c.b) * p.bt_stride;
             const int npages = (c.len + p.P - 1) / p.P;
@@ -273,13 +345,18 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                     e1 = entry(win + 32 + lane);
                 }
                 const int page = __shfl_sync(0xffffffffu, e0, (first - win + min(i, cnt - 1)) & 31);
-                if (filled) ok = wait_all(smem_u32(&k_empty[st * kLdParts + g]), ph, p.err);
-                if (!ok) break;
-                const uint32_t bar = smem_u32(&k_full[st * kLdParts + g]);
-                if (lane == 0) mbar_expect_tx(bar, chunks * cnt * p.P * 128);
-                if (i < cnt && (lane & 1) < chunks)
-                    tma_load_2d(sbase + st * stage_bytes + (2 * g + (lane & 1)) * kLdChunk + i * p.P * 128, &tmap,
-                                (2 * g + (lane & 1)) * 64, (p.layer * p.num_pages + page) * p.P, bar, pol);
+                const int y = (p.layer * p.num_pages + page) * p.P;
+                auto bring = [&](int part, int chunks) {
+                    if (filled) ok = ok && wait_all(smem_u32(&k_empty[st * kLdParts + part]), ph, p.err);
+                    if (!ok) return;
+                    const uint32_t bar = smem_u32(&k_full[st * kLdParts + part]);
+                    if (lane == 0) mbar_expect_tx(bar, chunks * cnt * p.P * 128);
+                    const int ch = 2 * part + (lane & 1);
+                    if (i < cnt && (lane & 1) < chunks)
+                        tma_load_2d(sbase + st * stage_bytes + ch * kLdChunk + i * p.P * 128, &tmap, ch * 64, y, bar, pol);
+                };
+                bring(g, 2);
+                if (g == 0) bring(LCH / 2, 1);
                 if (++st == p.stages) {
                     st = 0;
                     ph ^= 1;
@@ -289,8 +366,6 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         }
     } else if (warp == 5) {
         // ------------------------------------------------------------ S = Q K^T
-        LdWalk w = walk0;
-        LdPiece c;
         int si = 0, piece = 0, st = 0, ph = 0;
         bool ok = true;
         constexpr uint32_t id_s = idesc_16(Elem<T>::kBf16, 64, 64, 0, 0);
@@ -339,8 +414,6 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         }
     } else if (warp == 6) {
         // ------------------------------------------------------------ O^T += V^T P^T
-        LdWalk w = walk0;
-        LdPiece c;
         int pi = 0, st = 0, ph = 0;
         bool ok = true;
         constexpr uint32_t id_pv = idesc_16(Elem<T>::kBf16, 128, 64, 1, 0);
@@ -377,64 +450,16 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         }
     } else if (warp < 4) {
         // ------------------------------------------------------------ softmax and output
-        LdWalk w = walk0;
-        LdPiece c, nx;
+        LdPiece nx;
         // this thread's rows of the group: r and r + 8; its keys of a tile: 8j + kq and the next
         const int r = warp * 16 + (lane >> 2), kq = 2 * (lane & 3);
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-        const int rope8 = p.rope >> 3, lat8 = LCH * 8;
-
         if (blockIdx.x == 0)
             for (int b = threadIdx.x; b < p.B; b += 128)
                 if (__ldg(p.lens + b) != ld_len(p, b)) atomicOr(p.err, VK_ERR_SEQ_LEN);
-        // next piece with tiles; rows of empty units are written on the way
-        auto advance = [&](LdPiece& o) -> bool {
-            while (w.next(p, o)) {
-                if (o.t0 < o.t1) return true;
-                const int live = min(64, rows - o.g * 64);
-                const int64_t row0 = static_cast<int64_t>(o.b) * rows + o.g * 64;
-                uint4* dst = reinterpret_cast<uint4*>(p.out + 2 * row0 * p.latent);
-                for (int i = threadIdx.x; i < live * lat8; i += 128) dst[i] = make_uint4(0, 0, 0, 0);
-                if (p.lse && threadIdx.x < live) p.lse[row0 + threadIdx.x] = -INFINITY;
-                if (threadIdx.x == 0) p.ws_unit[static_cast<int64_t>(o.b) * p.groups + o.g] = make_int2(-1, -1);
-            }
-            return false;
-        };
-        // 16 rows a warp, a row's 16-byte vectors across the lanes; one division per
-        // piece, then (token, head) step along
-        auto load_q = [&](const LdPiece& o) {
-            int t = (o.g * 64 + warp * 16) / p.H, h = (o.g * 64 + warp * 16) % p.H;
-            const char* ql = p.ql + 2 * ((static_cast<int64_t>(o.b) * p.T + t) * p.ql_token + h * p.ql_head) + lane * 16;
-            const char* qr = p.qr + 2 * ((static_cast<int64_t>(o.b) * p.T + t) * p.qr_token + h * p.qr_head) + lane * 16;
-            const int live = rows - o.g * 64 - warp * 16;  // rows of this warp that exist
-#pragma unroll 4
-            for (int k = 0; k < 16; ++k) {
-                const bool on = k < live;
-                const uint32_t dst = s_q + swz128(warp * 16 + k, lane & 7) + (lane >> 3) * kLdChunk;
-#pragma unroll
-                for (int i = 0; i < (LCH + 3) / 4; ++i)
-                    if (lane + 32 * i < LCH * 8) cp_async16(dst + i * 4 * kLdChunk, on ? ql + i * 512 : p.ql, on);
-                if (lane < rope8)
-                    cp_async16(s_q + LCH * kLdChunk + swz128(warp * 16 + k, lane), on ? qr : p.qr, on);
-                ql += 2 * p.ql_head;
-                qr += 2 * p.qr_head;
-                if (++h == p.H) {
-                    h = 0;
-                    ++t;
-                    ql += 2 * (p.ql_token - p.H * p.ql_head);
-                    qr += 2 * (p.qr_token - p.H * p.qr_head);
-                }
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(q_full));
-        };
-
         int it = 0, st = 0;
         bool fail = false;
-        bool have = advance(c);
-        if (have) load_q(c);
+        if (have) q_landed();
         while (have) {
             float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // log2 domain; l: this thread's keys
             int lim[2];  // keys that the row sees
@@ -547,7 +572,10 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
             }
             // the last S of this piece has been read: the next piece's queries may land
             have = advance(nx);
-            if (have) load_q(nx);
+            if (have) {
+                load_q(nx);
+                q_landed();
+            }
             const bool whole = c.whole();
             const int64_t row0 = static_cast<int64_t>(c.b) * rows + c.g * 64;
             const int slot = 2 * blockIdx.x + (c.t0 == 0 ? 1 : 0);
@@ -565,8 +593,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
             }
             if (threadIdx.x == 0 && c.t0 == 0) {
                 int2 u = make_int2(-1, -1);
-                if (!whole)  // CTA of the unit's last tile: the largest i with i * total / n <= its position
-                    u = make_int2(blockIdx.x, static_cast<int>(((c.unit_start + c.tiles) * n - 1) / total));
+                if (!whole)
+                    u = make_int2(blockIdx.x, deal.owner(c.unit_start + c.tiles - 1));
                 p.ws_unit[static_cast<int64_t>(c.b) * p.groups + c.g] = u;
             }
             fail = !wait_all(smem_u32(pv_done), (it - 1) & 1, p.err) || fail;
@@ -638,74 +666,130 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
     }
 }
 
-// Joins the partials of units that several CTAs share.  Block (unit, row quad x
-// 128 latent elements): a thread has one element of four rows; `groups` groups
-// of 128 threads take the pieces in turn and meet in shared memory.  The order of
-// the sums is fixed by the pieces, so results repeat bit for bit.
-constexpr int kLdMergeGroups = 8;
-template <typename T, int LCH>
-__global__ void __launch_bounds__(128 * kLdMergeGroups) latent_merge_kernel(const __grid_constant__ LdParams p) {
-    __shared__ float4 part[kLdMergeGroups][128];
-    __shared__ float4 part_l[kLdMergeGroups];
-    const int lane = threadIdx.x & 31, d = threadIdx.x & 127, kg = threadIdx.x >> 7, kgs = blockDim.x >> 7;
+// Joins the partials of units that several CTAs share.  A thread has one latent
+// element (of each of MBS blocks of 128) of four rows; KG groups of D threads take
+// the pieces in turn and meet in shared memory.  Bound by latency: the pieces'
+// weights come from one round of loads, a piece per thread, while the first
+// partials are already on their way.  The order of the sums is fixed by the
+// pieces, so results repeat bit for bit.
+//   many units, few pieces each: MBS = latent / 128, D 128, KG 1 (one wave)
+//   few units, up to a piece per SM: MBS 1, D 64, KG 16 (more SMs, short loops)
+constexpr int kLdMaxPieces = 256;  // CTAs of a launch
+template <typename T, int LCH, int MBS, int D, int KG>
+__global__ void __launch_bounds__(D * KG) latent_merge_kernel(const __grid_constant__ LdParams p) {
+    __shared__ float4 part[KG > 1 ? KG : 1][KG > 1 ? D : 1];
+    __shared__ float4 wts[kLdMaxPieces];
+    __shared__ float4 m_warp[kLdMaxPieces / 32], l_warp[kLdMaxPieces / 32];
+    constexpr int kSplit = LCH * 64 / (MBS * 128) * (128 / D);  // blocks per row quad
+    const int lane = threadIdx.x & 31, kg = threadIdx.x / D;
     const int64_t unit = blockIdx.x;
-    const int quad = blockIdx.y / (LCH / 2), mb = blockIdx.y % (LCH / 2);
+    const int quad = blockIdx.y / kSplit, e0 = blockIdx.y % kSplit * D + threadIdx.x % D;  // element in its blocks
     const int b = static_cast<int>(unit / p.groups), g = static_cast<int>(unit % p.groups);
     const int rows = p.T * p.H, row_in = g * 64 + quad * 4;
+    if (row_in >= rows) return;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int2 u = p.ws_unit[unit];
-    if (u.x < 0 || row_in >= rows) return;
+    if (u.x < 0) return;
     // piece i of CTA u.x + i: the first tile's piece in the odd slot, the others in even ones
     auto slot_of = [&](int i) { return 2 * (u.x + i) + (i == 0 ? 1 : 0); };
     const int pieces = u.y - u.x + 1;
-    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    for (int i = lane; i < pieces; i += 32) {
-        const float4* ml = reinterpret_cast<const float4*>(p.ws_ml + slot_of(i) * 64 + quad * 4);
-        const float4 x = ml[0], y = ml[1];
-        m[0] = fmaxf(m[0], x.x);
-        m[1] = fmaxf(m[1], x.z);
-        m[2] = fmaxf(m[2], y.x);
-        m[3] = fmaxf(m[3], y.z);
-    }
+    constexpr int kAhead = KG > 1 ? 5 : 16 / MBS;  // pieces in flight
+    float4 o[kAhead][MBS];
+    auto fetch = [&](int i0) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+        for (int j = 0; j < kAhead; ++j)
+            if (i0 + j * KG < pieces) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m[k] = fmaxf(m[k], __shfl_xor_sync(0xffffffffu, m[k], o));
+                for (int k = 0; k < MBS; ++k)
+                    o[j][k] = __ldcs(p.ws_o + ld_part<LCH>(slot_of(i0 + j * KG), quad, k + (MBS == 1 ? e0 >> 7 : 0), e0 & 127));
+            }
+    };
+    fetch(kg);
+    // Weights: a thread per piece, the block's maxima and sums through the warps.
+    constexpr int kThreads = D * KG, kPer = kLdMaxPieces > kThreads ? kLdMaxPieces / kThreads : 1;
+    const int warp = threadIdx.x >> 5, used = min(kThreads / 32, (pieces + 31) >> 5);  // warps that hold pieces
+    float4 x[kPer], y[kPer], m = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), l = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int i = threadIdx.x + j * kThreads;
+        x[j] = y[j] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);  // (m, l) of rows 0, 1 and 2, 3
+        if (i < pieces) {
+            const float4* ml = reinterpret_cast<const float4*>(p.ws_ml + slot_of(i) * 64 + quad * 4);
+            x[j] = ml[0];
+            y[j] = ml[1];
+        }
+        m = make_float4(fmaxf(m.x, x[j].x), fmaxf(m.y, x[j].z), fmaxf(m.z, y[j].x), fmaxf(m.w, y[j].z));
     }
-    auto weight = [&](float mi, int k) { return ex2(mi - (m[k] == -INFINITY ? 0.f : m[k])); };
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f), l = acc;
-#pragma unroll 4
-    for (int i = kg; i < pieces; i += kgs) {
-        const int slot = slot_of(i);
-        const float4 o = p.ws_o[ld_part<LCH>(slot, quad, mb, d)];
-        const float4* ml = reinterpret_cast<const float4*>(p.ws_ml + slot * 64 + quad * 4);
-        const float4 x = ml[0], y = ml[1];
-        // a piece whose keys a row may not see has weight, O and l of zero
-        const float f0 = weight(x.x, 0), f1 = weight(x.z, 1), f2 = weight(y.x, 2), f3 = weight(y.z, 3);
-        acc = make_float4(fmaf(f0, o.x, acc.x), fmaf(f1, o.y, acc.y), fmaf(f2, o.z, acc.z), fmaf(f3, o.w, acc.w));
-        l = make_float4(fmaf(f0, x.y, l.x), fmaf(f1, x.w, l.y), fmaf(f2, y.y, l.z), fmaf(f3, y.w, l.w));
+    if (warp < used) {
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1)
+            m = make_float4(fmaxf(m.x, __shfl_xor_sync(0xffffffffu, m.x, s)), fmaxf(m.y, __shfl_xor_sync(0xffffffffu, m.y, s)),
+                            fmaxf(m.z, __shfl_xor_sync(0xffffffffu, m.z, s)), fmaxf(m.w, __shfl_xor_sync(0xffffffffu, m.w, s)));
+        if (lane == 0) m_warp[warp] = m;
     }
-    if (kgs > 1) {
-        part[kg][d] = acc;
-        if (d == 0) part_l[kg] = l;
+    __syncthreads();
+    m = m_warp[0];
+    for (int k = 1; k < used; ++k)
+        m = make_float4(fmaxf(m.x, m_warp[k].x), fmaxf(m.y, m_warp[k].y), fmaxf(m.z, m_warp[k].z), fmaxf(m.w, m_warp[k].w));
+    if (warp < used) {
+        auto weight = [](float mi, float mm) { return ex2(mi - (mm == -INFINITY ? 0.f : mm)); };
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int i = threadIdx.x + j * kThreads;
+            // a piece whose keys a row may not see has weight, O and l of zero
+            const float4 f = make_float4(weight(x[j].x, m.x), weight(x[j].z, m.y), weight(y[j].x, m.z), weight(y[j].z, m.w));
+            if (i < pieces) {
+                wts[i] = f;
+                l = make_float4(fmaf(f.x, x[j].y, l.x), fmaf(f.y, x[j].w, l.y), fmaf(f.z, y[j].y, l.z), fmaf(f.w, y[j].w, l.w));
+            }
+        }
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1)
+            l = make_float4(l.x + __shfl_xor_sync(0xffffffffu, l.x, s), l.y + __shfl_xor_sync(0xffffffffu, l.y, s),
+                            l.z + __shfl_xor_sync(0xffffffffu, l.z, s), l.w + __shfl_xor_sync(0xffffffffu, l.w, s));
+        if (lane == 0) l_warp[warp] = l;
+    }
+    __syncthreads();
+    l = l_warp[0];
+    for (int k = 1; k < used; ++k) l = make_float4(l.x + l_warp[k].x, l.y + l_warp[k].y, l.z + l_warp[k].z, l.w + l_warp[k].w);
+    float4 acc[MBS];
+#pragma unroll
+    for (int k = 0; k < MBS; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = kg; i0 < pieces; i0 += kAhead * KG) {
+        if (i0 != kg) fetch(i0);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (i0 + j * KG < pieces) {
+                const float4 f = wts[i0 + j * KG];
+#pragma unroll
+                for (int k = 0; k < MBS; ++k)
+                    acc[k] = make_float4(fmaf(f.x, o[j][k].x, acc[k].x), fmaf(f.y, o[j][k].y, acc[k].y),
+                                         fmaf(f.z, o[j][k].z, acc[k].z), fmaf(f.w, o[j][k].w, acc[k].w));
+            }
+    }
+    if constexpr (KG > 1) {
+        part[kg][threadIdx.x % D] = acc[0];
         __syncthreads();
         if (kg) return;
-        acc = part[0][d];
-        l = part_l[0];
-        for (int k = 1; k < kgs; ++k) {
-            const float4 a = part[k][d], c = part_l[k];
-            acc = make_float4(acc.x + a.x, acc.y + a.y, acc.z + a.z, acc.w + a.w);
-            l = make_float4(l.x + c.x, l.y + c.y, l.z + c.z, l.w + c.w);
+#pragma unroll
+        for (int k = 1; k < KG; ++k) {
+            const float4 a = part[k][threadIdx.x];
+            acc[0] = make_float4(acc[0].x + a.x, acc[0].y + a.y, acc[0].z + a.z, acc[0].w + a.w);
         }
     }
     const int64_t row = static_cast<int64_t>(b) * rows + row_in;
-    const float av[4] = {acc.x, acc.y, acc.z, acc.w}, lv[4] = {l.x, l.y, l.z, l.w};
-    T* out = reinterpret_cast<T*>(p.out) + row * (LCH * 64) + mb * 128 + d;
+    const float lv[4] = {l.x, l.y, l.z, l.w}, mv[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        if (row_in + k >= rows) break;
-        out[k * LCH * 64] = Elem<T>::down(lv[k] > 0.f || lv[k] != lv[k] ? av[k] / lv[k] : 0.f);
-        if (p.lse && mb == 0 && d == 0) p.lse[row + k] = lv[k] == 0.f ? -INFINITY : (m[k] + log2f(lv[k])) * 0.69314718055994531f;
+    for (int r = 0; r < 4; ++r) {
+        if (row_in + r >= rows) break;
+        const float inv = lv[r] > 0.f || lv[r] != lv[r] ? 1.f / lv[r] : 0.f;
+#pragma unroll
+        for (int k = 0; k < MBS; ++k) {
+            const float a = r == 0 ? acc[k].x : r == 1 ? acc[k].y : r == 2 ? acc[k].z : acc[k].w;
+            reinterpret_cast<T*>(p.out)[(row + r) * (LCH * 64) + k * 128 + e0] = Elem<T>::down(inv == 0.f ? 0.f : a * inv);
+        }
+        if (p.lse && blockIdx.y % kSplit == 0 && threadIdx.x == 0)
+            p.lse[row + r] = lv[r] == 0.f ? -INFINITY : (mv[r] + log2f(lv[r])) * 0.69314718055994531f;
     }
 }
 
@@ -722,23 +806,27 @@ static vk_status launch_latent_decode(vk_pool* pool, const LdParams& p, cudaStre
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(latent_decode)");
         attr_set |= bit;
     }
-    latent_decode_kernel<T, LCH><<<pool->num_sms, kLdThreads, smem, st>>>(pool->tmap16, p);
+    latent_decode_kernel<T, LCH><<<min(pool->num_sms, kLdMaxPieces), kLdThreads, smem, st>>>(pool->tmap16, p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "latent_decode_kernel launch");
     const int64_t units = static_cast<int64_t>(p.B) * p.groups;
     const int quads = (min(64, p.T * p.H) + 3) / 4;
-    // few blocks: few units, so many pieces each, which more groups share
-    const int groups = units * quads * (LCH / 2) <= 4 * pool->num_sms ? kLdMergeGroups : 1;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(quads * (LCH / 2)));
-    cfg.blockDim = dim3(groups * 128);
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, latent_merge_kernel<T, LCH>, p);
+    if (units * quads <= pool->num_sms / 2) {
+        cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(quads * LCH));
+        cfg.blockDim = dim3(1024);
+        e = cudaLaunchKernelEx(&cfg, latent_merge_kernel<T, LCH, 1, 64, 16>, p);
+    } else {
+        cfg.gridDim = dim3(static_cast<unsigned>(units), static_cast<unsigned>(quads));
+        cfg.blockDim = dim3(128);
+        e = cudaLaunchKernelEx(&cfg, latent_merge_kernel<T, LCH, LCH / 2, 128, 1>, p);
+    }
     return e == cudaSuccess ? VK_OK : cuda_fail(e, "latent_merge_kernel launch");
 }
 
