@@ -52,10 +52,12 @@ constexpr int kLdParts = 5;       // barriers of a stage: pairs of chunks of the
 constexpr int kLdChunk = kLdKeys * 128;  // 64 keys x 64 elements, 128-byte rows
 constexpr int kLdAux = 1536;             // barriers, alpha, 1/l, schedule
 constexpr int kLdSmemMax = 232448;
-// A unit's prologue and epilogue (q load, output) in tiles, for the deal.
-constexpr int kLdUnitCost = 2;
-// Least cost of a CTA's range: fewer, longer pieces when there is little work
-constexpr int kLdMinRange = 4;
+// A unit's prologue and epilogue (q load, output) in tiles, for the deal (2 to 4 are
+// within 2% of one another, 1 and 6 slower).
+constexpr int kLdUnitCost = 3;
+// Least cost of a CTA's range (1 x 200 tokens: 12.5 us with 1, 14.7 with 4: tiles in
+// parallel and a merge beat tiles in turn)
+constexpr int kLdMinRange = 1;
 
 struct LdParams {
     const char* ql;
@@ -248,51 +250,51 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
     const int rows = p.T * p.H, rope8 = p.rope >> 3, lat8 = LCH * 8;
     LdWalk w = walk0;  // every role walks the CTA's pieces for itself
     LdPiece c;
-            // next piece with tiles; rows of empty units are written on the way
-            auto advance = [&](LdPiece& o) -> bool {
-                while (w.next(p, o)) {
-                    if (o.t0 < o.t1) return true;
-                    const int live = min(64, rows - o.g * 64);
-                    const int64_t row0 = static_cast<int64_t>(o.b) * rows + o.g * 64;
-                    uint4* dst = reinterpret_cast<uint4*>(p.out + 2 * row0 * p.latent);
-                    for (int i = threadIdx.x; i < live * lat8; i += 128) dst[i] = make_uint4(0, 0, 0, 0);
-                    if (p.lse && threadIdx.x < live) p.lse[row0 + threadIdx.x] = -INFINITY;
-                    if (threadIdx.x == 0) p.ws_unit[static_cast<int64_t>(o.b) * p.groups + o.g] = make_int2(-1, -1);
-                }
-                return false;
-            };
-            // 16 rows a warp, a row's 16-byte vectors across the lanes; one division per
-            // piece, then (token, head) step along
-            auto load_q = [&](const LdPiece& o) {
-                int t = (o.g * 64 + warp * 16) / p.H, h = (o.g * 64 + warp * 16) % p.H;
-                const char* ql = p.ql + 2 * ((static_cast<int64_t>(o.b) * p.T + t) * p.ql_token + h * p.ql_head) + lane * 16;
-                const char* qr = p.qr + 2 * ((static_cast<int64_t>(o.b) * p.T + t) * p.qr_token + h * p.qr_head) + lane * 16;
-                const int live = rows - o.g * 64 - warp * 16;  // rows of this warp that exist
-    #pragma unroll 4
-                for (int k = 0; k < 16; ++k) {
-                    const bool on = k < live;
-                    const uint32_t dst = s_q + swz128(warp * 16 + k, lane & 7) + (lane >> 3) * kLdChunk;
-    #pragma unroll
-                    for (int i = 0; i < (LCH + 3) / 4; ++i)
-                        if (lane + 32 * i < LCH * 8) cp_async16(dst + i * 4 * kLdChunk, on ? ql + i * 512 : p.ql, on);
-                    if (lane < rope8)
-                        cp_async16(s_q + LCH * kLdChunk + swz128(warp * 16 + k, lane), on ? qr : p.qr, on);
-                    ql += 2 * p.ql_head;
-                    qr += 2 * p.qr_head;
-                    if (++h == p.H) {
-                        h = 0;
-                        ++t;
-                        ql += 2 * (p.ql_token - p.H * p.ql_head);
-                        qr += 2 * (p.qr_token - p.H * p.qr_head);
-                    }
-                }
-            };
-            auto q_landed = [&]() {
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(q_full));
-            };
+    // next piece with tiles; rows of empty units are written on the way
+    auto advance = [&](LdPiece& o) -> bool {
+        while (w.next(p, o)) {
+            if (o.t0 < o.t1) return true;
+            const int live = min(64, rows - o.g * 64);
+            const int64_t row0 = static_cast<int64_t>(o.b) * rows + o.g * 64;
+            uint4* dst = reinterpret_cast<uint4*>(p.out + 2 * row0 * p.latent);
+            for (int i = threadIdx.x; i < live * lat8; i += 128) dst[i] = make_uint4(0, 0, 0, 0);
+            if (p.lse && threadIdx.x < live) p.lse[row0 + threadIdx.x] = -INFINITY;
+            if (threadIdx.x == 0) p.ws_unit[static_cast<int64_t>(o.b) * p.groups + o.g] = make_int2(-1, -1);
+        }
+        return false;
+    };
+    // 16 rows a warp, a row's 16-byte vectors across the lanes; one division per
+    // piece, then (token, head) step along
+    auto load_q = [&](const LdPiece& o) {
+        int t = (o.g * 64 + warp * 16) / p.H, h = (o.g * 64 + warp * 16) % p.H;
+        const char* ql = p.ql + 2 * ((static_cast<int64_t>(o.b) * p.T + t) * p.ql_token + h * p.ql_head) + lane * 16;
+        const char* qr = p.qr + 2 * ((static_cast<int64_t>(o.b) * p.T + t) * p.qr_token + h * p.qr_head) + lane * 16;
+        const int live = rows - o.g * 64 - warp * 16;  // rows of this warp that exist
+#pragma unroll 4
+        for (int k = 0; k < 16; ++k) {
+            const bool on = k < live;
+            const uint32_t dst = s_q + swz128(warp * 16 + k, lane & 7) + (lane >> 3) * kLdChunk;
+#pragma unroll
+            for (int i = 0; i < (LCH + 3) / 4; ++i)
+                if (lane + 32 * i < LCH * 8) cp_async16(dst + i * 4 * kLdChunk, on ? ql + i * 512 : p.ql, on);
+            if (lane < rope8)
+                cp_async16(s_q + LCH * kLdChunk + swz128(warp * 16 + k, lane), on ? qr : p.qr, on);
+            ql += 2 * p.ql_head;
+            qr += 2 * p.qr_head;
+            if (++h == p.H) {
+                h = 0;
+                ++t;
+                ql += 2 * (p.ql_token - p.H * p.ql_head);
+                qr += 2 * (p.qr_token - p.H * p.qr_head);
+            }
+        }
+    };
+    auto q_landed = [&]() {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(q_full));
+    };
 
     // The first queries are on their way before any tile is: behind the tiles of all
     // SMs they took 2 us longer to arrive.
