@@ -342,66 +342,77 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
         }
     } else if (warp == 9) {
         // ------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            constexpr uint32_t id_s = idesc_16(Elem<T>::kBf16, 128, 128, 0, 0);
-            constexpr uint32_t id_pv = idesc_16(Elem<T>::kBf16, 128, 64, 0, 1);
-            bool ok = mbar_wait(smem_u32(q_full), 0, p.err);
-            tc_fence_after();
-            const int nt[2] = {ntA, ntB};
-            int k_waited = -1, v_waited = -1;
-            const int rsteps = p.rope >> 4;
-            const uint64_t dq0 = umma_desc_sw128(sbase + kLaQ, 16, 1024);
-            const uint64_t dr0 = umma_desc_sw128(sbase + kLaRing, 16, 1024);
-            auto issue_s = [&](int t, int j) {
-                if (j > k_waited) {
-                    ok = ok && mbar_wait(smem_u32(&k_full[j & 1]), (j >> 1) & 1, p.err);
-                    k_waited = j;
-                }
-                if (!ok) return;
+        // The whole warp waits and one lane issues: unrolled runs on 32-bit descriptor
+        // words, ~40 cycles an MMA (a lane alone on 64-bit descriptors took ~60, with
+        // the two 64-column halves of P V apart 28 MMAs a step: 35% tensor activity).
+        constexpr uint32_t id_s = idesc_16(Elem<T>::kBf16, 128, 128, 0, 0);
+        constexpr uint32_t id_pv = idesc_16(Elem<T>::kBf16, 128, 128, 0, 1), id_half = idesc_16(Elem<T>::kBf16, 128, 64, 0, 1);
+        const bool lead = elect_lane();
+        bool ok = wait_all(smem_u32(q_full), 0, p.err);
+        const int nt[2] = {ntA, ntB};
+        int k_waited = -1, v_waited = -1;
+        const int rsteps = p.rope >> 4;
+        const uint64_t dk0 = umma_desc_sw128(sbase + kLaRing, 16, 1024), dv0 = umma_desc_sw128(sbase + kLaRing, kLpUnit, 1024);
+        const uint32_t k_hi = static_cast<uint32_t>(dk0 >> 32), k_lo = static_cast<uint32_t>(dk0);
+        const uint32_t v_hi = static_cast<uint32_t>(dv0 >> 32), v_lo = static_cast<uint32_t>(dv0);
+        const uint32_t q_lo = k_lo - (kLaRing >> 4);
+        constexpr uint32_t kUnit16 = kLpUnit >> 4;
+        auto issue_s = [&](int t, int j) {
+            if (j > k_waited) {
+                ok = ok && wait_all(smem_u32(&k_full[j & 1]), (j >> 1) & 1, p.err);
+                k_waited = j;
+            }
+            if (ok && lead) {
                 tc_fence_after();
-                const uint64_t dq = dq0 + static_cast<uint64_t>(t * 3 * (kLpUnit >> 4));
-                const uint32_t d = tmem + t * 128;
+                const uint32_t ql = q_lo + t * 3 * kUnit16, d = tmem + t * 128;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint64_t dk = dr0 + static_cast<uint64_t>(((5 * j + u) & 7) * (kLpUnit >> 4));
+                for (int u = 0; u < 3; ++u) {
+                    const uint32_t kl = k_lo + ((5 * j + u) & 7) * kUnit16;
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks)
-                        umma_ss(d, dq + u * (kLpUnit >> 4) + ((ks * 32) >> 4), dk + ((ks * 32) >> 4), id_s, (u | ks) != 0);
+                        if (u < 2 || ks < rsteps) umma_ss_lo(d, ql + u * kUnit16 + ks * 2, k_hi, kl + ks * 2, k_hi, id_s, (u | ks) != 0);
                 }
-                const uint64_t dk = dr0 + static_cast<uint64_t>(((5 * j + 2) & 7) * (kLpUnit >> 4));
-                for (int ks = 0; ks < rsteps; ++ks)
-                    umma_ss(d, dq + 2 * (kLpUnit >> 4) + ((ks * 32) >> 4), dk + ((ks * 32) >> 4), id_s, 1);
                 umma_commit(smem_u32(&s_full[t]));
                 if (t == 1 || j >= ntB) umma_commit(smem_u32(&k_empty[j & 1]));
-            };
-            auto issue_pv = [&](int t, int j) {
-                ok = ok && mbar_wait(smem_u32(&p_full[t]), j & 1, p.err);
-                if (j > v_waited) {
-                    ok = ok && mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, p.err);
-                    v_waited = j;
-                }
-                if (!ok) return;
+            }
+            __syncwarp();
+        };
+        auto issue_pv = [&](int t, int j) {
+            ok = ok && wait_all(smem_u32(&p_full[t]), j & 1, p.err);
+            if (j > v_waited) {
+                ok = ok && wait_all(smem_u32(&v_full[j & 1]), (j >> 1) & 1, p.err);
+                v_waited = j;
+            }
+            if (ok && lead) {
                 tc_fence_after();
-                const uint32_t d = tmem + 256 + t * 128, a = tmem + t * 128;
+                const uint32_t d = tmem + 256 + t * 128, a = tmem + t * 128, acc = j > 0;
+                const int slot = (5 * j + 3) & 7;
+                if (slot < 7) {  // both 64-column units side by side: one MMA spans them
+                    const uint32_t vl = v_lo + slot * kUnit16;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint64_t dv = dr0 + static_cast<uint64_t>(((5 * j + 3 + u) & 7) * (kLpUnit >> 4));
+                    for (int ks = 0; ks < kLpKeys / 16; ++ks) umma_ts_lo(d, a + ks * 8, vl + ks * 128, v_hi, id_pv, ks ? 1 : acc);
+                } else {
+#pragma unroll 1
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t vl = v_lo + ((slot + u) & 7) * kUnit16;
 #pragma unroll
-                    for (int ks = 0; ks < kLpKeys / 16; ++ks)
-                        umma_ts(d + u * 64, a + ks * 8, dv + ((ks * 2048) >> 4), id_pv, (j > 0 || ks > 0) ? 1u : 0u);
+                        for (int ks = 0; ks < kLpKeys / 16; ++ks)
+                            umma_ts_lo(d + u * 64, a + ks * 8, vl + ks * 128, v_hi, id_half, ks ? 1 : acc);
+                    }
                 }
                 umma_commit(smem_u32(&o_full[t]));
                 if (t == 1 || j >= ntB) umma_commit(smem_u32(&v_empty[j & 1]));
-            };
-            issue_s(0, 0);
-            if (ntB > 0) issue_s(1, 0);
-            for (int j = 0; j < ntiles && ok; ++j) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (j < nt[t]) {
-                        issue_pv(t, j);
-                        if (j + 1 < nt[t]) issue_s(t, j + 1);
-                    }
+            }
+            __syncwarp();
+        };
+        issue_s(0, 0);
+        if (ntB > 0) issue_s(1, 0);
+        for (int j = 0; j < ntiles && ok; ++j) {
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+                if (j < nt[t]) {
+                    issue_pv(t, j);
+                    if (j + 1 < nt[t]) issue_s(t, j + 1);
                 }
             }
         }
@@ -533,10 +544,18 @@ static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensor
     const int lch = p.latent / 64;
     p.stages = min(kLeMaxStages, (kLpSmemMax - 2048 - lch * kLpUnit) / kLeStage);
     const size_t smem = static_cast<size_t>(lch) * kLpUnit + static_cast<size_t>(p.stages) * kLeStage + 2048;
-    // heads per CTA: at most 8 (the 128 gathered rows are then read once per 2 MiB of
-    // W at 512), fewer when that would leave SMs idle
-    const int64_t items = static_cast<int64_t>(p.B) * tiles * p.heads;
-    p.per_cta = static_cast<int>(min(static_cast<int64_t>(8), max(static_cast<int64_t>(1), items / (2 * pool->num_sms))));
+    // Heads per CTA: the count whose waves of CTAs are done first, at ~4 units of time a
+    // head and ~6 for a CTA's start (its 128 gathered rows are read for all its heads).
+    const int64_t row_tiles = static_cast<int64_t>(p.B) * tiles;
+    int64_t best = 0;
+    p.per_cta = 1;
+    for (int n = 1; n <= p.heads; ++n) {
+        const int64_t waves = (row_tiles * ((p.heads + n - 1) / n) + pool->num_sms - 1) / pool->num_sms, cost = waves * (4 * n + 6);
+        if (n == 1 || cost < best) {
+            best = cost;
+            p.per_cta = n;
+        }
+    }
     latent_expand_kernel<T><<<dim3((p.heads + p.per_cta - 1) / p.per_cta, tiles, p.B), kLeThreads, smem, st>>>(pool->tmap16, tw, p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "latent_expand_kernel launch");
