@@ -2,6 +2,7 @@
 #pragma once
 
 #include "vk_ptx.cuh"
+#include "vk_rotary.cuh"
 
 namespace vk {
 
@@ -15,6 +16,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+
+// 0 in the place of each non-finite 16-bit element of a word.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_word(uint32_t w) {
+    constexpr uint32_t e = Elem<T>::kBf16 ? 0x7f80u : 0x7c00u;
+    if ((w & e) == e) w &= 0xffff0000u;
+    if ((w & (e << 16)) == (e << 16)) w &= 0x0000ffffu;
+    return w;
 }
 
 }  // namespace vk

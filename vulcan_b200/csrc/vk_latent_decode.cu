@@ -168,15 +168,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool l
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
-// 0 in the place of each non-finite 16-bit element of a word.
-template <typename T>
-__device__ __forceinline__ uint32_t finite_word(uint32_t w) {
-    constexpr uint32_t e = Elem<T>::kBf16 ? 0x7f80u : 0x7c00u;
-    if ((w & e) == e) w &= 0xffff0000u;
-    if ((w & (e << 16)) == (e << 16)) w &= 0x0000ffffu;
-    return w;
-}
-
 template <typename T, int LCH>  // LCH: latent_dim / 64
 __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __grid_constant__ CUtensorMap tmap,
                                                                       const __grid_constant__ LdParams p) {

@@ -11,7 +11,7 @@
 //
 //  * latent_expand_kernel: [128 cached tokens] x [one head's 256 rows of W] as a
 //    tcgen05 GEMM.  The 128 gathered latent rows stay in shared memory (128 KiB
-//    at 512) for all heads of the CTA; W streams through a ring of 32 KiB
+//    at 512) for all heads of the CTA; W streams through a ring of 16 KiB
 //    stages; two TMEM accumulators of 256 columns, so a head is stored while the
 //    next one multiplies.  Output rows [token][head][128 K | 128 V] in the
 //    workspace, rounded to the cache's 16-bit type (relative 2^-9 or 2^-12 of
@@ -80,13 +80,17 @@ __device__ __forceinline__ LpSeq lp_seq(const LpParams& p, int b, bool record) {
 
 // ------------------------------------------------------------------ expansion
 
-constexpr int kLeThreads = 192;   // 4 epilogue warps, TMA warp, MMA warp
-constexpr int kLeStage = 32768;   // 256 rows of W x 64
-constexpr int kLeMaxStages = 6;
+// A TMA load holds its issuing warp for ~500 cycles per 16 KiB (and a 2 KiB box
+// ~70), twice what the MMAs of the stage take: three warps issue.
+constexpr int kLeLoaders = 3;
+constexpr int kLeThreads = 384;   // 8 epilogue warps, MMA warp, three TMA warps
+constexpr int kLeStage = 16384;   // 128 rows of W x 64
+constexpr int kLeMaxStages = 10;
 
 template <typename T>
 __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __grid_constant__ CUtensorMap tmap,
                                                                       const __grid_constant__ CUtensorMap tmapw,
+                                                                      const __grid_constant__ CUtensorMap tmapkv,
                                                                       const __grid_constant__ LpParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -98,14 +102,15 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
     if (sq.n == 0 || kt * kLpKeys >= len) return;
     const int hfirst = blockIdx.x * p.per_cta, nh = min(p.per_cta, p.heads - hfirst);
     const int lch = p.latent >> 6;
-    const uint32_t s_b = sbase + lch * kLpUnit;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + lch * kLpUnit + p.stages * kLeStage);
+    const uint32_t s_b = sbase + lch * kLpUnit, s_out = s_b + p.stages * kLeStage;  // s_out: [K, V][128 rows][128 B]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + lch * kLpUnit + (p.stages + 2) * kLeStage);
     uint64_t* a_full = bars;             // [8]
     uint64_t* b_full = bars + 8;         // [stages]
     uint64_t* b_empty = b_full + kLeMaxStages;
     uint64_t* acc_full = b_empty + kLeMaxStages;  // [2]
     uint64_t* acc_empty = acc_full + 2;           // [2]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    uint8_t* bad_row = reinterpret_cast<uint8_t*>(bars) + 384;  // [2][128]
     if (threadIdx.x == 0) {
         for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&a_full[i]), 1);
         for (int i = 0; i < p.stages; ++i) {
@@ -114,11 +119,11 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&acc_full[i]), 1);
-            mbar_init(smem_u32(&acc_empty[i]), 4);
+            mbar_init(smem_u32(&acc_empty[i]), 8);
         }
         mbar_fence_init();
     }
-    if (warp == 5) {
+    if (warp == 9) {
         tmem_alloc(smem_u32(tmem_slot), 512);
         tmem_relinquish();
     }
@@ -127,7 +132,8 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 4) {
+    if (warp == 8 || warp >= 10) {
+        const int me = warp == 8 ? 0 : warp - 9;
         const uint64_t pol = l2_evict_last_policy();
         const int cnt = min(kLpKeys / p.P, (len + p.P - 1) / p.P - kt * (kLpKeys / p.P));
         int page = 0;
@@ -138,95 +144,129 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
                 page = 0;
             }
         }
+        // stages in the order (head, 64 columns of W, K rows then V rows), every third mine
         bool ok = true;
-        auto load_b = [&](int it) {
-            const int st = it % p.stages;
-            if (it >= p.stages) ok = mbar_wait(smem_u32(&b_empty[st]), (it / p.stages - 1) & 1, p.err);
+        int st = me, it = me;
+        uint32_t ph = 1;
+        const int total = nh * lch * 2, lead = min(p.stages, total);
+        auto load_b = [&](bool wait) {
+            if (wait) ok = mbar_wait(smem_u32(&b_empty[st]), ph, p.err);
             if (!ok) return;
             const uint32_t bar = smem_u32(&b_full[st]);
+            const int k = it >> 1, h = k / lch;
             mbar_expect_tx(bar, kLeStage);
-            tma_load_2d(s_b + st * kLeStage, &tmapw, (it % lch) * 64, (p.h0 + hfirst + it / lch) * 256, bar, pol);
-        };
-        const int total = nh * lch, lead = min(p.stages, total);
-        if (lane == 0) {
-            prefetch_tmap(&tmapw);
-            for (int it = 0; it < lead; ++it) load_b(it);
-            for (int c = 0; c < lch; ++c) mbar_expect_tx(smem_u32(&a_full[c]), cnt * p.P * 128);
-        }
-        __syncwarp();
-        for (int c = 0; c < lch; ++c)
-            if (lane < cnt)
-                tma_load_2d(sbase + c * kLpUnit + lane * p.P * 128, &tmap, c * 64, (p.layer * p.num_pages + page) * p.P,
-                            smem_u32(&a_full[c]), pol);
-        if (lane == 0)
-            for (int it = lead; it < total && ok; ++it) load_b(it);
-    } else if (warp == 5) {
-        if (lane == 0) {
-            constexpr uint32_t id = idesc_16(Elem<T>::kBf16, 128, 256, 0, 0);
-            bool ok = true;
-            int it = 0;
-            for (int h = 0; h < nh && ok; ++h) {
-                const int buf = h & 1;
-                if (h >= 2) ok = mbar_wait(smem_u32(&acc_empty[buf]), ((h >> 1) - 1) & 1, p.err);
-                for (int c = 0; c < lch && ok; ++c, ++it) {
-                    const int st = it % p.stages;
-                    if (h == 0) ok = mbar_wait(smem_u32(&a_full[c]), 0, p.err);
-                    ok = ok && mbar_wait(smem_u32(&b_full[st]), (it / p.stages) & 1, p.err);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t da = umma_desc_sw128(sbase + c * kLpUnit, 16, 1024);
-                    const uint64_t db = umma_desc_sw128(s_b + st * kLeStage, 16, 1024);
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)
-                        umma_ss(tmem + buf * 256, da + ((ks * 32) >> 4), db + ((ks * 32) >> 4), id, (c | ks) != 0);
-                    umma_commit(smem_u32(&b_empty[st]));
-                }
-                if (ok) umma_commit(smem_u32(&acc_full[buf]));
+            tma_load_2d(s_b + st * kLeStage, &tmapw, (k - h * lch) * 64, (p.h0 + hfirst + h) * 256 + (it & 1) * 128, bar, pol);
+            it += kLeLoaders;
+            st += kLeLoaders;
+            if (st >= p.stages) {
+                st -= p.stages;
+                ph ^= 1;
             }
+        };
+        if (lane == 0)
+            while (it < lead) load_b(false);
+        for (int k = me; k < lch; k += kLeLoaders) {
+            if (lane == 0) mbar_expect_tx(smem_u32(&a_full[k]), cnt * p.P * 128);
+            __syncwarp();
+            if (lane < cnt)
+                tma_load_2d(sbase + k * kLpUnit + lane * p.P * 128, &tmap, k * 64, (p.layer * p.num_pages + page) * p.P,
+                            smem_u32(&a_full[k]), pol);
+        }
+        if (lane == 0)
+            while (it < total && ok) load_b(true);
+    } else if (warp == 9) {
+        constexpr uint32_t id = idesc_16(Elem<T>::kBf16, 128, 128, 0, 0);
+        const bool lead = elect_lane();
+        const uint64_t d0 = umma_desc_sw128(sbase, 16, 1024);
+        const uint32_t hi = static_cast<uint32_t>(d0 >> 32), a_lo = static_cast<uint32_t>(d0), b_lo = a_lo + ((s_b - sbase) >> 4);
+        bool ok = true;
+        int st = 0, ph = 0;
+        for (int h = 0; h < nh && ok; ++h) {
+            const int buf = h & 1;
+            if (h >= 2) ok = wait_all(smem_u32(&acc_empty[buf]), ((h >> 1) - 1) & 1, p.err);
+            for (int c = 0; c < lch && ok; ++c) {
+                if (h == 0) ok = wait_all(smem_u32(&a_full[c]), 0, p.err);
+                for (int half = 0; half < 2; ++half) {
+                    ok = ok && wait_all(smem_u32(&b_full[st]), ph, p.err);
+                    if (ok && lead) {
+                        tc_fence_after();
+                        const uint32_t d = tmem + buf * 256 + half * 128, al = a_lo + c * (kLpUnit >> 4), bl = b_lo + st * (kLeStage >> 4);
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) umma_ss_lo(d, al + ks * 2, hi, bl + ks * 2, hi, id, ks ? 1 : c != 0);
+                        umma_commit(smem_u32(&b_empty[st]));
+                    }
+                    __syncwarp();
+                    if (++st == p.stages) {
+                        st = 0;
+                        ph ^= 1;
+                    }
+                }
+            }
+            if (ok && lead) umma_commit(smem_u32(&acc_full[buf]));
+            __syncwarp();
         }
     } else {
-        const int r = warp * 32 + lane;
+        // Epilogue: warps 0-3 the K columns, warps 4-7 the V columns, a row per thread,
+        // out through shared memory by TMA (rows stored straight from registers, 32
+        // bytes each at the workspace's pitch, kept the load/store queue busy for 2,000
+        // to 3,700 cycles a head, and MMAs and loads of those warps waited behind them).
+        const int half = warp >> 2, r = threadIdx.x & 127;
         const bool inside = kt * kLpKeys + r < len;
-        const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-        const int64_t row = static_cast<int64_t>(b) * p.lpad + kt * kLpKeys + r;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + half * 128;
+        const uint32_t stage = s_out + half * kLeStage;
+        constexpr uint32_t kExp = Elem<T>::kBf16 ? 0x7f807f80u : 0x7c007c00u;
+        bool ok = true;
         for (int h = 0; h < nh; ++h) {
             const int buf = h & 1;
-            if (!wait_all(smem_u32(&acc_full[buf]), (h >> 1) & 1, p.err)) break;
+            ok = ok && wait_all(smem_u32(&acc_full[buf]), (h >> 1) & 1, p.err);
             tc_fence_after();
-            char* dst = p.ws + 2 * ((row * p.heads + hfirst + h) * 256);
-            // a key whose every element is NaN or infinite comes from such a latent;
-            // rows that may not see it multiply its value by a weight of zero, so
-            // its value is stored as zeros (rows that see it get their NaN through S)
-            bool bad = true;
+            uint32_t w[64], all = kExp;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
+            for (int c = 0; c < 4; ++c) {
                 float v[32];
                 tmem_ld32(lane_base + buf * 256 + c * 32, v);
                 tmem_wait_ld();
-                if (c < 4) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) bad = bad && !(fabsf(v[i]) <= 3.4028234e38f);
-                } else if (bad) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = fabsf(v[i]) <= 3.4028234e38f ? v[i] : 0.f;
+                for (int i = 0; i < 16; ++i) {
+                    w[c * 16 + i] = inside ? Elem<T>::pack(v[2 * i], v[2 * i + 1]) : 0u;
+                    all &= w[c * 16 + i];
                 }
-                uint32_t w[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[i] = inside ? Elem<T>::pack(v[2 * i], v[2 * i + 1]) : 0u;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + c * 64 + i * 32),
-                                 "r"(w[8 * i]), "r"(w[8 * i + 1]), "r"(w[8 * i + 2]), "r"(w[8 * i + 3]), "r"(w[8 * i + 4]),
-                                 "r"(w[8 * i + 5]), "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
-                                 : "memory");
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&acc_empty[buf]));
+            // A key whose every element is NaN or infinite comes from such a latent; rows
+            // that may not see it multiply its value by a weight of zero, so the value's
+            // non-finite elements are stored as zeros (a row that sees the key gets its
+            // NaN through S).  Both halves meet at a named barrier each head; barriers
+            // count every warp, so a failed wait (recorded) leaves none behind.
+            if (half == 0) bad_row[buf * 128 + r] = (all & kExp) == kExp;
+            asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+            if (half == 1 && bad_row[buf * 128 + r]) {
+#pragma unroll
+                for (int i = 0; i < 64; ++i) w[i] = finite_word<T>(w[i]);
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {  // 64 columns at a time through this half's 16 KiB
+                if (r == 0) bulk_wait_read();
+                asm volatile("barrier.cta.sync %0, 128;" ::"r"(2 + half) : "memory");
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + swz128(r, i)), "r"(w[c * 32 + 4 * i]),
+                                 "r"(w[c * 32 + 4 * i + 1]), "r"(w[c * 32 + 4 * i + 2]), "r"(w[c * 32 + 4 * i + 3])
+                                 : "memory");
+                fence_async_smem();
+                asm volatile("barrier.cta.sync %0, 128;" ::"r"(2 + half) : "memory");
+                if (r == 0 && ok) {
+                    tma_store_2d(&tmapkv, stage, (hfirst + h) * 256 + half * 128 + c * 64, b * p.lpad + kt * kLpKeys);
+                    bulk_commit();
+                }
+            }
         }
+        if (r == 0) bulk_wait();
     }
     __syncthreads();
-    if (warp == 5) {
+    if (warp == 9) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -234,7 +274,7 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
 
 // ------------------------------------------------------------------ attention
 
-constexpr int kLaThreads = 320;
+constexpr int kLaThreads = 384;  // 8 softmax warps, MMA warp, three TMA warps
 constexpr int kLaQ = 0;                              // [2 tiles][3 chunks][128 rows][128 B]
 constexpr int kLaRing = 2 * 3 * kLpUnit;             // 96 KiB
 constexpr int kLaUnits = 8;
@@ -274,7 +314,13 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
     uint64_t* q_full = bars + 14;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 10; ++i) mbar_init(smem_u32(&bars[i]), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&k_full[i]), 3);  // the two units of W_k c and the rotary parts
+            mbar_init(smem_u32(&v_full[i]), 2);
+            mbar_init(smem_u32(&k_empty[i]), 1);
+            mbar_init(smem_u32(&v_empty[i]), 1);
+            mbar_init(smem_u32(&s_full[i]), 1);
+        }
         mbar_init(smem_u32(&p_full[0]), 4);
         mbar_init(smem_u32(&p_full[1]), 4);
         mbar_init(smem_u32(&o_full[0]), 1);
@@ -299,57 +345,67 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 8) {
-        // ------------------------------------------------------------ TMA producer
-        const uint64_t pol = l2_evict_last_policy();  // other row tiles read the same K and V
+    if (warp == 8 || warp == 10) {
+        // ------------------------------------------------------------ TMA: W c of K and V, one unit of each
+        // (a load holds its warp for ~500 cycles per 16 KiB: three warps share a tile)
+        // units 5j .. 5j+2 take the ring slots of tile j-2's last K unit and its V,
+        // units 5j+3, 5j+4 those of tile j-1's first two K units
+        if (lane == 0) {
+            const uint64_t pol = l2_evict_last_policy();  // other row tiles read the same K and V
+            const int wrow = b * p.lpad, u = warp == 8 ? 0 : 1;
+            bool ok = true;
+            for (int j = 0; j < ntiles; ++j) {
+                if (j >= 2) ok = ok && mbar_wait(smem_u32(&v_empty[j & 1]), ((j >> 1) - 1) & 1, p.err);
+                if (!ok) break;
+                const uint32_t kbar = smem_u32(&k_full[j & 1]), vbar = smem_u32(&v_full[j & 1]);
+                mbar_expect_tx(kbar, kLpUnit);
+                tma_load_2d(sbase + kLaRing + ((5 * j + u) & 7) * kLpUnit, &tmapkv, hl * 256 + u * 64, wrow + j * kLpKeys, kbar, pol);
+                if (j >= 1) ok = mbar_wait(smem_u32(&k_empty[(j - 1) & 1]), ((j - 1) >> 1) & 1, p.err);
+                if (!ok) break;
+                mbar_expect_tx(vbar, kLpUnit);
+                tma_load_2d(sbase + kLaRing + ((5 * j + 3 + u) & 7) * kLpUnit, &tmapkv, hl * 256 + kLpHead + u * 64,
+                            wrow + j * kLpKeys, vbar, pol);
+            }
+        }
+    } else if (warp == 11) {
+        // ------------------------------------------------------------ TMA: rotary parts from the pages
+        // (a warp of its own: eight 16-token pages take ~600 cycles to issue)
+        const uint64_t pol = l2_evict_last_policy();
         const int32_t* btrow = p.bt + static_cast<int64_t>(b) * p.bt_stride;
         const int npages = (kv_len + p.P - 1) / p.P, ppt = kLpKeys / p.P;
-        const int wrow = b * p.lpad;
-        bool ok = true;
-        for (int j = 0; j < ntiles && ok; ++j) {
-            int page = 0;  // a page of the tile's rotary parts per lane
-            const int cnt = min(ppt, npages - j * ppt);
-            if (lane < cnt) {
-                page = __ldg(btrow + j * ppt + lane);
-                if (page < 0 || page >= p.num_pages) {
-                    atomicOr(p.err, VK_ERR_PAGE_ID);
-                    page = 0;
-                }
+        auto page_of = [&](int j) {  // a page of the tile per lane
+            int page = lane < ppt && j * ppt + lane < npages ? __ldg(btrow + j * ppt + lane) : 0;
+            if (page < 0 || page >= p.num_pages) {
+                atomicOr(p.err, VK_ERR_PAGE_ID);
+                page = 0;
             }
-            // units 5j .. 5j+2 take the ring slots of tile j-2's last K unit and its V,
-            // units 5j+3, 5j+4 those of tile j-1's first two K units
+            return page;
+        };
+        bool ok = true;
+        int next = page_of(0);
+        for (int j = 0; j < ntiles; ++j) {
+            const int page = next, cnt = min(ppt, npages - j * ppt);
+            if (j + 1 < ntiles) next = page_of(j + 1);
             if (j >= 2) ok = wait_all(smem_u32(&v_empty[j & 1]), ((j >> 1) - 1) & 1, p.err);
             if (!ok) break;
             const uint32_t kbar = smem_u32(&k_full[j & 1]);
-            if (lane == 0) {
-                mbar_expect_tx(kbar, 2 * kLpUnit + cnt * p.P * 128);
-                for (int u = 0; u < 2; ++u)
-                    tma_load_2d(sbase + kLaRing + ((5 * j + u) & 7) * kLpUnit, &tmapkv, hl * 256 + u * 64, wrow + j * kLpKeys,
-                                kbar, pol);
-            }
-            __syncwarp();
+            if (lane == 0) mbar_expect_tx(kbar, cnt * p.P * 128);
             if (lane < cnt)
                 tma_load_2d(sbase + kLaRing + ((5 * j + 2) & 7) * kLpUnit + lane * p.P * 128, &tmap, p.latent,
                             (p.layer * p.num_pages + page) * p.P, kbar, pol);
-            if (j >= 1) ok = wait_all(smem_u32(&k_empty[(j - 1) & 1]), ((j - 1) >> 1) & 1, p.err);
-            if (ok && lane == 0) {
-                const uint32_t vbar = smem_u32(&v_full[j & 1]);
-                mbar_expect_tx(vbar, 2 * kLpUnit);
-                for (int u = 0; u < 2; ++u)
-                    tma_load_2d(sbase + kLaRing + ((5 * j + 3 + u) & 7) * kLpUnit, &tmapkv, hl * 256 + kLpHead + u * 64,
-                                wrow + j * kLpKeys, vbar, pol);
-            }
         }
     } else if (warp == 9) {
         // ------------------------------------------------------------ MMA issuer
-        // The whole warp waits and one lane issues: unrolled runs on 32-bit descriptor
-        // words, ~40 cycles an MMA (a lane alone on 64-bit descriptors took ~60, with
-        // the two 64-column halves of P V apart 28 MMAs a step: 35% tensor activity).
+        // S_A0, S_B0, PV_A0, S_A1, PV_B0, S_B1, ...: one thread, so its MMAs execute in
+        // order, P is read before the next S overwrites it, and each step's products
+        // are done as early as they can be (a second issuing warp, one per row tile,
+        // made the steps interleave and was 16% slower).  The warp waits as a whole and
+        // one lane issues, in unrolled runs on 32-bit descriptor words: ~40 cycles an
+        // MMA (60 on 64-bit descriptors from a lone lane).
         constexpr uint32_t id_s = idesc_16(Elem<T>::kBf16, 128, 128, 0, 0);
         constexpr uint32_t id_pv = idesc_16(Elem<T>::kBf16, 128, 128, 0, 1), id_half = idesc_16(Elem<T>::kBf16, 128, 64, 0, 1);
         const bool lead = elect_lane();
         bool ok = wait_all(smem_u32(q_full), 0, p.err);
-        const int nt[2] = {ntA, ntB};
         int k_waited = -1, v_waited = -1;
         const int rsteps = p.rope >> 4;
         const uint64_t dk0 = umma_desc_sw128(sbase + kLaRing, 16, 1024), dv0 = umma_desc_sw128(sbase + kLaRing, kLpUnit, 1024);
@@ -378,11 +434,11 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
             __syncwarp();
         };
         auto issue_pv = [&](int t, int j) {
-            ok = ok && wait_all(smem_u32(&p_full[t]), j & 1, p.err);
             if (j > v_waited) {
                 ok = ok && wait_all(smem_u32(&v_full[j & 1]), (j >> 1) & 1, p.err);
                 v_waited = j;
             }
+            ok = ok && wait_all(smem_u32(&p_full[t]), j & 1, p.err);
             if (ok && lead) {
                 tc_fence_after();
                 const uint32_t d = tmem + 256 + t * 128, a = tmem + t * 128, acc = j > 0;
@@ -408,12 +464,13 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
         issue_s(0, 0);
         if (ntB > 0) issue_s(1, 0);
         for (int j = 0; j < ntiles && ok; ++j) {
-#pragma unroll 1
-            for (int t = 0; t < 2; ++t) {
-                if (j < nt[t]) {
-                    issue_pv(t, j);
-                    if (j + 1 < nt[t]) issue_s(t, j + 1);
-                }
+            if (j < ntA) {
+                issue_pv(0, j);
+                if (j + 1 < ntA) issue_s(0, j + 1);
+            }
+            if (j < ntB) {
+                issue_pv(1, j);
+                if (j + 1 < ntB) issue_s(1, j + 1);
             }
         }
     } else {
@@ -542,8 +599,8 @@ static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensor
     }
     const int tiles = p.lpad / kLpKeys;
     const int lch = p.latent / 64;
-    p.stages = min(kLeMaxStages, (kLpSmemMax - 2048 - lch * kLpUnit) / kLeStage);
-    const size_t smem = static_cast<size_t>(lch) * kLpUnit + static_cast<size_t>(p.stages) * kLeStage + 2048;
+    p.stages = min(kLeMaxStages, (kLpSmemMax - 2048 - lch * kLpUnit) / kLeStage - 2);  // 4, 6, 8, 10 at 512 .. 128
+    const size_t smem = static_cast<size_t>(lch) * kLpUnit + static_cast<size_t>(p.stages + 2) * kLeStage + 2048;
     // Heads per CTA: the count whose waves of CTAs are done first, at ~4 units of time a
     // head and ~6 for a CTA's start (its 128 gathered rows are read for all its heads).
     const int64_t row_tiles = static_cast<int64_t>(p.B) * tiles;
@@ -556,7 +613,7 @@ static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensor
             p.per_cta = n;
         }
     }
-    latent_expand_kernel<T><<<dim3((p.heads + p.per_cta - 1) / p.per_cta, tiles, p.B), kLeThreads, smem, st>>>(pool->tmap16, tw, p);
+    latent_expand_kernel<T><<<dim3((p.heads + p.per_cta - 1) / p.per_cta, tiles, p.B), kLeThreads, smem, st>>>(pool->tmap16, tw, tkv, p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "latent_expand_kernel launch");
     const dim3 grid((p.max_tokens + 2 * kLpRows - 1) / (2 * kLpRows), p.heads, p.B);
@@ -647,7 +704,7 @@ extern "C" vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void*
     {
         const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.latent), static_cast<cuuint64_t>(num_heads) * 256};
         const cuuint64_t strides[1] = {static_cast<cuuint64_t>(w_stride) * 2};
-        const cuuint32_t box[2] = {64, 256};
+        const cuuint32_t box[2] = {64, 128};
         if (encode(&tw, type, 2, const_cast<void*>(w_kv), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return fail(VK_INVALID_ARG, "w_kv's shape or stride cannot be addressed by TMA");
