@@ -9,11 +9,13 @@
 // and head 2 * 256 * latent once for the expansion: from ~170 new tokens on the
 // expanded form does less.  Two kernels per group of heads:
 //
-//  * latent_expand_kernel: [128 cached tokens] x [one head's 256 rows of W] as a
-//    tcgen05 GEMM.  The 128 gathered latent rows stay in shared memory (128 KiB
-//    at 512) for all heads of the CTA; W streams through a ring of 16 KiB
-//    stages; two TMEM accumulators of 256 columns, so a head is stored while the
-//    next one multiplies.  Output rows [token][head][128 K | 128 V] in the
+//  * latent_expand_kernel: [256 cached tokens] x [128 rows of W] as a tcgen05 GEMM.
+//    What bounds it is the way from L2 into an SM (at most 64 bytes a cycle, and
+//    ~1,000 to 2,000 cycles long), so every byte of W serves two 128-row tiles: the
+//    gathered rows stay on the SM for all heads of the CTA, row tile 0 in shared
+//    memory (128 KiB at 512), row tile 1 in TMEM (256 columns), as the A operands of
+//    its MMAs.  With one row tile a CTA the same GEMM took 150 us at 8 x 2048 tokens
+//    and 32 heads.  Output rows [token][head][128 K | 128 V] in the
 //    workspace, rounded to the cache's 16-bit type (relative 2^-9 or 2^-12 of
 //    each element, as a cache of keys and values holds them); rows behind the
 //    sequence are stored as zeros, so the attention reads no stale bytes.
@@ -81,9 +83,10 @@ __device__ __forceinline__ LpSeq lp_seq(const LpParams& p, int b, bool record) {
 // ------------------------------------------------------------------ expansion
 
 // A TMA load holds its issuing warp for ~500 cycles per 16 KiB (and a 2 KiB box
-// ~70), twice what the MMAs of the stage take: three warps issue.
+// ~70), about what the MMAs of the stage take: three warps issue.
 constexpr int kLeLoaders = 3;
 constexpr int kLeThreads = 384;   // 8 epilogue warps, MMA warp, three TMA warps
+constexpr int kLeTokens = 256;    // cached rows of a CTA: row tiles 0 and 1 of 128
 constexpr int kLeStage = 16384;   // 128 rows of W x 64
 constexpr int kLeMaxStages = 10;
 
@@ -96,31 +99,33 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = blockIdx.z, kt = blockIdx.y;
-    const LpSeq sq = lp_seq(p, b, threadIdx.x == 0 && blockIdx.x == 0 && kt == 0 && p.h0 == 0);
+    const int b = blockIdx.z, key0 = blockIdx.y * kLeTokens;
+    const LpSeq sq = lp_seq(p, b, threadIdx.x == 0 && blockIdx.x == 0 && key0 == 0 && p.h0 == 0);
     const int len = sq.pos + sq.n;
-    if (sq.n == 0 || kt * kLpKeys >= len) return;
+    if (sq.n == 0 || key0 >= len) return;
+    const bool two = key0 + kLpKeys < len;  // row tile 1 has rows
     const int hfirst = blockIdx.x * p.per_cta, nh = min(p.per_cta, p.heads - hfirst);
     const int lch = p.latent >> 6;
-    const uint32_t s_b = sbase + lch * kLpUnit, s_out = s_b + p.stages * kLeStage;  // s_out: [K, V][128 rows][128 B]
+    const uint32_t s_b = sbase + lch * kLpUnit, s_out = s_b + p.stages * kLeStage;  // s_out: [row tile][128 rows][128 B]
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + lch * kLpUnit + (p.stages + 2) * kLeStage);
-    uint64_t* a_full = bars;             // [8]
-    uint64_t* b_full = bars + 8;         // [stages]
-    uint64_t* b_empty = b_full + kLeMaxStages;
-    uint64_t* acc_full = b_empty + kLeMaxStages;  // [2]
-    uint64_t* acc_empty = acc_full + 2;           // [2]
+    uint64_t* a_full = bars;                       // [2] row tile 1's, then row tile 0's latent rows landed
+    uint64_t* a_moved = bars + 2;                  // row tile 1's rows are in TMEM
+    uint64_t* b_full = bars + 3;                   // [stages]
+    uint64_t* b_empty = b_full + kLeMaxStages;     // [stages]
+    uint64_t* acc_full = b_empty + kLeMaxStages;   // [row tile]
+    uint64_t* acc_empty = acc_full + 2;            // [row tile]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
-    uint8_t* bad_row = reinterpret_cast<uint8_t*>(bars) + 384;  // [2][128]
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 8; ++i) mbar_init(smem_u32(&a_full[i]), 1);
         for (int i = 0; i < p.stages; ++i) {
             mbar_init(smem_u32(&b_full[i]), 1);
             mbar_init(smem_u32(&b_empty[i]), 1);
         }
         for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&a_full[i]), kLeLoaders);
             mbar_init(smem_u32(&acc_full[i]), 1);
-            mbar_init(smem_u32(&acc_empty[i]), 8);
+            mbar_init(smem_u32(&acc_empty[i]), 4);
         }
+        mbar_init(smem_u32(a_moved), 4);
         mbar_fence_init();
     }
     if (warp == 9) {
@@ -130,22 +135,14 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = *tmem_slot;  // columns 0..255: row tile 1's latent rows; 256, 384: the accumulators
 
     if (warp == 8 || warp >= 10) {
         const int me = warp == 8 ? 0 : warp - 9;
         const uint64_t pol = l2_evict_last_policy();
-        const int cnt = min(kLpKeys / p.P, (len + p.P - 1) / p.P - kt * (kLpKeys / p.P));
-        int page = 0;
-        if (lane < cnt) {
-            page = __ldg(p.bt + static_cast<int64_t>(b) * p.bt_stride + kt * (kLpKeys / p.P) + lane);
-            if (page < 0 || page >= p.num_pages) {
-                atomicOr(p.err, VK_ERR_PAGE_ID);
-                page = 0;
-            }
-        }
-        // stages in the order (head, 64 columns of W, K rows then V rows), every third mine
+        const int npages = (len + p.P - 1) / p.P, ppt = kLpKeys / p.P;
         bool ok = true;
+        // stages in the order (head, K rows then V rows, 64 columns of W), every third mine
         int st = me, it = me;
         uint32_t ph = 1;
         const int total = nh * lch * 2, lead = min(p.stages, total);
@@ -153,9 +150,9 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
             if (wait) ok = mbar_wait(smem_u32(&b_empty[st]), ph, p.err);
             if (!ok) return;
             const uint32_t bar = smem_u32(&b_full[st]);
-            const int k = it >> 1, h = k / lch;
+            const int hh = it / lch;  // half-head
             mbar_expect_tx(bar, kLeStage);
-            tma_load_2d(s_b + st * kLeStage, &tmapw, (k - h * lch) * 64, (p.h0 + hfirst + h) * 256 + (it & 1) * 128, bar, pol);
+            tma_load_2d(s_b + st * kLeStage, &tmapw, (it - hh * lch) * 64, (p.h0 + hfirst) * 256 + hh * 128, bar, pol);
             it += kLeLoaders;
             st += kLeLoaders;
             if (st >= p.stages) {
@@ -163,15 +160,31 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
                 ph ^= 1;
             }
         };
+        // the gathered rows: row tile 1 through the same shared memory first
+        auto load_a = [&](int tile) {
+            const int first = key0 / p.P + tile * ppt, cnt = min(ppt, npages - first);
+            int page = 0;
+            if (lane < cnt) {
+                page = __ldg(p.bt + static_cast<int64_t>(b) * p.bt_stride + first + lane);
+                if (page < 0 || page >= p.num_pages) {
+                    atomicOr(p.err, VK_ERR_PAGE_ID);
+                    page = 0;
+                }
+            }
+            const int mine = (lch - me + kLeLoaders - 1) / kLeLoaders;  // chunks me, me + 3, ...
+            const uint32_t bar = smem_u32(&a_full[tile ^ 1]);
+            if (lane == 0) mbar_expect_tx(bar, mine * cnt * p.P * 128);
+            __syncwarp();
+            for (int k = me; k < lch; k += kLeLoaders)
+                if (lane < cnt)
+                    tma_load_2d(sbase + k * kLpUnit + lane * p.P * 128, &tmap, k * 64, (p.layer * p.num_pages + page) * p.P, bar, pol);
+        };
+        if (two) load_a(1);
         if (lane == 0)
             while (it < lead) load_b(false);
-        for (int k = me; k < lch; k += kLeLoaders) {
-            if (lane == 0) mbar_expect_tx(smem_u32(&a_full[k]), cnt * p.P * 128);
-            __syncwarp();
-            if (lane < cnt)
-                tma_load_2d(sbase + k * kLpUnit + lane * p.P * 128, &tmap, k * 64, (p.layer * p.num_pages + page) * p.P,
-                            smem_u32(&a_full[k]), pol);
-        }
+        __syncwarp();
+        if (two) ok = wait_all(smem_u32(a_moved), 0, p.err);
+        if (ok) load_a(0);
         if (lane == 0)
             while (it < total && ok) load_b(true);
     } else if (warp == 9) {
@@ -181,84 +194,111 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
         const uint32_t hi = static_cast<uint32_t>(d0 >> 32), a_lo = static_cast<uint32_t>(d0), b_lo = a_lo + ((s_b - sbase) >> 4);
         bool ok = true;
         int st = 0, ph = 0;
-        for (int h = 0; h < nh && ok; ++h) {
-            const int buf = h & 1;
-            if (h >= 2) ok = wait_all(smem_u32(&acc_empty[buf]), ((h >> 1) - 1) & 1, p.err);
+        if (two) ok = wait_all(smem_u32(a_moved), 0, p.err);
+        ok = ok && wait_all(smem_u32(&a_full[1]), 0, p.err);
+        tc_fence_after();
+        for (int hh = 0; hh < 2 * nh && ok; ++hh) {  // K half, V half of each head
             for (int c = 0; c < lch && ok; ++c) {
-                if (h == 0) ok = wait_all(smem_u32(&a_full[c]), 0, p.err);
-                for (int half = 0; half < 2; ++half) {
-                    ok = ok && wait_all(smem_u32(&b_full[st]), ph, p.err);
+                ok = wait_all(smem_u32(&b_full[st]), ph, p.err);
+                if (c == 0 && hh > 0) ok = ok && wait_all(smem_u32(&acc_empty[0]), (hh - 1) & 1, p.err);
+                if (ok && lead) {
+                    tc_fence_after();
+                    const uint32_t al = a_lo + c * (kLpUnit >> 4), bl = b_lo + st * (kLeStage >> 4);
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) umma_ss_lo(tmem + 256, al + ks * 2, hi, bl + ks * 2, hi, id, ks ? 1 : c != 0);
+                    if (c == lch - 1) umma_commit(smem_u32(&acc_full[0]));
+                }
+                __syncwarp();
+                if (two) {
+                    if (c == 0 && hh > 0) ok = ok && wait_all(smem_u32(&acc_empty[1]), (hh - 1) & 1, p.err);
                     if (ok && lead) {
                         tc_fence_after();
-                        const uint32_t d = tmem + buf * 256 + half * 128, al = a_lo + c * (kLpUnit >> 4), bl = b_lo + st * (kLeStage >> 4);
+                        const uint32_t bl = b_lo + st * (kLeStage >> 4);
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) umma_ss_lo(d, al + ks * 2, hi, bl + ks * 2, hi, id, ks ? 1 : c != 0);
-                        umma_commit(smem_u32(&b_empty[st]));
+                        for (int ks = 0; ks < 4; ++ks) umma_ts_lo(tmem + 384, tmem + c * 32 + ks * 8, bl + ks * 2, hi, id, ks ? 1 : c != 0);
+                        if (c == lch - 1) umma_commit(smem_u32(&acc_full[1]));
                     }
                     __syncwarp();
-                    if (++st == p.stages) {
-                        st = 0;
-                        ph ^= 1;
-                    }
+                }
+                if (ok && lead) umma_commit(smem_u32(&b_empty[st]));
+                __syncwarp();
+                if (++st == p.stages) {
+                    st = 0;
+                    ph ^= 1;
                 }
             }
-            if (ok && lead) umma_commit(smem_u32(&acc_full[buf]));
-            __syncwarp();
         }
-    } else {
-        // Epilogue: warps 0-3 the K columns, warps 4-7 the V columns, a row per thread,
-        // out through shared memory by TMA (rows stored straight from registers, 32
-        // bytes each at the workspace's pitch, kept the load/store queue busy for 2,000
-        // to 3,700 cycles a head, and MMAs and loads of those warps waited behind them).
-        const int half = warp >> 2, r = threadIdx.x & 127;
-        const bool inside = kt * kLpKeys + r < len;
-        const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + half * 128;
-        const uint32_t stage = s_out + half * kLeStage;
+    } else if (warp < 4 || two) {
+        // Epilogue: warps 0-3 row tile 0, warps 4-7 row tile 1, a row per thread, out
+        // through shared memory by TMA (rows stored straight from registers, 32 bytes
+        // each at the workspace's pitch, kept the load/store queue busy for 2,000 to
+        // 3,700 cycles a head, and MMAs and loads of those warps waited behind them).
+        const int tile = warp >> 2, r = threadIdx.x & 127;
+        const bool inside = key0 + tile * kLpKeys + r < len;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const uint32_t stage = s_out + tile * kLeStage;
         constexpr uint32_t kExp = Elem<T>::kBf16 ? 0x7f807f80u : 0x7c007c00u;
         bool ok = true;
-        for (int h = 0; h < nh; ++h) {
-            const int buf = h & 1;
-            ok = ok && wait_all(smem_u32(&acc_full[buf]), (h >> 1) & 1, p.err);
+        if (tile) {  // row tile 1's latent rows, shared memory -> TMEM (two elements a column)
+            ok = wait_all(smem_u32(&a_full[0]), 0, p.err);
+            for (int c = 0; c < lch; ++c) {
+                float w[32];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(w[4 * i]), "=f"(w[4 * i + 1]), "=f"(w[4 * i + 2]), "=f"(w[4 * i + 3])
+                                 : "r"(sbase + c * kLpUnit + swz128(r, i)));
+                tmem_st32(lane_base + c * 32, w);
+            }
+            tmem_wait_st();
+            fence_async_smem();  // these reads before the next tile's TMA writes
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(a_moved));
+        }
+        bool bad = false;
+        for (int hh = 0; hh < 2 * nh; ++hh) {
+            ok = ok && wait_all(smem_u32(&acc_full[tile]), hh & 1, p.err);
             tc_fence_after();
             uint32_t w[64], all = kExp;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float v[32];
-                tmem_ld32(lane_base + buf * 256 + c * 32, v);
+            for (int c = 0; c < 2; ++c) {
+                float v[2][32];
+                tmem_ld32(lane_base + 256 + tile * 128 + c * 64, v[0]);
+                tmem_ld32(lane_base + 256 + tile * 128 + c * 64 + 32, v[1]);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    w[c * 16 + i] = inside ? Elem<T>::pack(v[2 * i], v[2 * i + 1]) : 0u;
-                    all &= w[c * 16 + i];
+                for (int i = 0; i < 32; ++i) {
+                    w[c * 32 + i] = inside ? Elem<T>::pack(v[i >> 4][2 * (i & 15)], v[i >> 4][2 * (i & 15) + 1]) : 0u;
+                    all &= w[c * 32 + i];
                 }
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&acc_empty[buf]));
+            if (lane == 0) mbar_arrive(smem_u32(&acc_empty[tile]));
             // A key whose every element is NaN or infinite comes from such a latent; rows
             // that may not see it multiply its value by a weight of zero, so the value's
             // non-finite elements are stored as zeros (a row that sees the key gets its
-            // NaN through S).  Both halves meet at a named barrier each head; barriers
-            // count every warp, so a failed wait (recorded) leaves none behind.
-            if (half == 0) bad_row[buf * 128 + r] = (all & kExp) == kExp;
-            asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
-            if (half == 1 && bad_row[buf * 128 + r]) {
+            // NaN through S).
+            if ((hh & 1) == 0) {
+                bad = (all & kExp) == kExp;
+            } else if (bad) {
 #pragma unroll
                 for (int i = 0; i < 64; ++i) w[i] = finite_word<T>(w[i]);
             }
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {  // 64 columns at a time through this half's 16 KiB
+            for (int c = 0; c < 2; ++c) {  // 64 columns at a time through this tile's 16 KiB
                 if (r == 0) bulk_wait_read();
-                asm volatile("barrier.cta.sync %0, 128;" ::"r"(2 + half) : "memory");
+                asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + tile) : "memory");
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + swz128(r, i)), "r"(w[c * 32 + 4 * i]),
                                  "r"(w[c * 32 + 4 * i + 1]), "r"(w[c * 32 + 4 * i + 2]), "r"(w[c * 32 + 4 * i + 3])
                                  : "memory");
                 fence_async_smem();
-                asm volatile("barrier.cta.sync %0, 128;" ::"r"(2 + half) : "memory");
+                asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + tile) : "memory");
                 if (r == 0 && ok) {
-                    tma_store_2d(&tmapkv, stage, (hfirst + h) * 256 + half * 128 + c * 64, b * p.lpad + kt * kLpKeys);
+                    tma_store_2d(&tmapkv, stage, hfirst * 256 + hh * 128 + c * 64, b * p.lpad + key0 + tile * kLpKeys);
                     bulk_commit();
                 }
             }
@@ -517,20 +557,27 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
                 m_ref = m_new;
             }
             const float mneg = m_ref == -INFINITY ? 0.f : -m_ref;
-            float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t sc2 = f2(sc, sc), mneg2 = f2(mneg, mneg);
+            uint64_t sum2[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int c = 0; c < kLpKeys / 32; ++c) {
                 uint32_t pk[16];
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
-                    const float a0 = ex2(fmaf(v[c][i], sc, mneg));
-                    const float a1 = ex2(fmaf(v[c][i + 1], sc, mneg));
-                    sum4[(i >> 1) & 3] += a0 + a1;
+                    float a0, a1;
+                    f2_get(f2_fma(f2(v[c][i], v[c][i + 1]), sc2, mneg2), a0, a1);
+                    a0 = ex2(a0);
+                    a1 = ex2(a1);
+                    sum2[(i >> 1) & 3] = f2_add(sum2[(i >> 1) & 3], f2(a0, a1));
                     pk[i >> 1] = Elem<T>::pack(a0, a1);
                 }
                 tmem_st16(lane_base + s_col + c * 16, pk);
             }
-            l = l * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+            {
+                float s0, s1;
+                f2_get(f2_add(f2_add(sum2[0], sum2[1]), f2_add(sum2[2], sum2[3])), s0, s1);
+                l = l * alpha + (s0 + s1);
+            }
             // after P is stored, when the S row's registers are dead
             if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
@@ -597,23 +644,23 @@ static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensor
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(latent prefill)");
         attr_set |= bit;
     }
-    const int tiles = p.lpad / kLpKeys;
     const int lch = p.latent / 64;
     p.stages = min(kLeMaxStages, (kLpSmemMax - 2048 - lch * kLpUnit) / kLeStage - 2);  // 4, 6, 8, 10 at 512 .. 128
     const size_t smem = static_cast<size_t>(lch) * kLpUnit + static_cast<size_t>(p.stages + 2) * kLeStage + 2048;
-    // Heads per CTA: the count whose waves of CTAs are done first, at ~4 units of time a
-    // head and ~6 for a CTA's start (its 128 gathered rows are read for all its heads).
-    const int64_t row_tiles = static_cast<int64_t>(p.B) * tiles;
+    // Heads per CTA: the count whose waves of CTAs are done first, at ~10 units of time a
+    // head and ~6 for a CTA's start (its gathered rows are read once for all its heads).
+    const int row_tiles = (p.lpad + kLeTokens - 1) / kLeTokens;
     int64_t best = 0;
     p.per_cta = 1;
     for (int n = 1; n <= p.heads; ++n) {
-        const int64_t waves = (row_tiles * ((p.heads + n - 1) / n) + pool->num_sms - 1) / pool->num_sms, cost = waves * (4 * n + 6);
+        const int64_t ctas = static_cast<int64_t>(p.B) * row_tiles * ((p.heads + n - 1) / n);
+        const int64_t cost = (ctas + pool->num_sms - 1) / pool->num_sms * (10 * n + 6);
         if (n == 1 || cost < best) {
             best = cost;
             p.per_cta = n;
         }
     }
-    latent_expand_kernel<T><<<dim3((p.heads + p.per_cta - 1) / p.per_cta, tiles, p.B), kLeThreads, smem, st>>>(pool->tmap16, tw, tkv, p);
+    latent_expand_kernel<T><<<dim3((p.heads + p.per_cta - 1) / p.per_cta, row_tiles, p.B), kLeThreads, smem, st>>>(pool->tmap16, tw, tkv, p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "latent_expand_kernel launch");
     const dim3 grid((p.max_tokens + 2 * kLpRows - 1) / (2 * kLpRows), p.heads, p.B);
