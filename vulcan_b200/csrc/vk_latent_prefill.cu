@@ -83,9 +83,9 @@ __device__ __forceinline__ LpSeq lp_seq(const LpParams& p, int b, bool record) {
 // ------------------------------------------------------------------ expansion
 
 // A TMA load holds its issuing warp for ~500 cycles per 16 KiB (and a 2 KiB box
-// ~70), about what the MMAs of the stage take: three warps issue.
-constexpr int kLeLoaders = 3;
-constexpr int kLeThreads = 384;   // 8 epilogue warps, MMA warp, three TMA warps
+// ~70), about what the MMAs of the stage take: two warps issue.
+constexpr int kLeLoaders = 2;
+constexpr int kLeThreads = 384;   // 8 epilogue warps, two MMA warps, two TMA warps
 constexpr int kLeTokens = 256;    // cached rows of a CTA: row tiles 0 and 1 of 128
 constexpr int kLeStage = 16384;   // 128 rows of W x 64
 constexpr int kLeMaxStages = 10;
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) {
             mbar_init(smem_u32(&b_full[i]), 1);
-            mbar_init(smem_u32(&b_empty[i]), 1);
+            mbar_init(smem_u32(&b_empty[i]), two ? 2 : 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&a_full[i]), kLeLoaders);
@@ -137,12 +137,12 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;  // columns 0..255: row tile 1's latent rows; 256, 384: the accumulators
 
-    if (warp == 8 || warp >= 10) {
-        const int me = warp == 8 ? 0 : warp - 9;
+    if (warp == 8 || warp == 10) {
+        const int me = warp == 8 ? 0 : 1;
         const uint64_t pol = l2_evict_last_policy();
         const int npages = (len + p.P - 1) / p.P, ppt = kLpKeys / p.P;
         bool ok = true;
-        // stages in the order (head, K rows then V rows, 64 columns of W), every third mine
+        // stages in the order (head, K rows then V rows, 64 columns of W), every other one mine
         int st = me, it = me;
         uint32_t ph = 1;
         const int total = nh * lch * 2, lead = min(p.stages, total);
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
                     page = 0;
                 }
             }
-            const int mine = (lch - me + kLeLoaders - 1) / kLeLoaders;  // chunks me, me + 3, ...
+            const int mine = (lch - me + kLeLoaders - 1) / kLeLoaders;  // chunks me, me + 2, ...
             const uint32_t bar = smem_u32(&a_full[tile ^ 1]);
             if (lane == 0) mbar_expect_tx(bar, mine * cnt * p.P * 128);
             __syncwarp();
@@ -187,44 +187,44 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
         if (ok) load_a(0);
         if (lane == 0)
             while (it < total && ok) load_b(true);
-    } else if (warp == 9) {
+    } else if (warp == 9 || warp == 11) {
+        // MMA issuers, one per row tile: an issuing thread is held until its last MMA is
+        // dispatched and then needs ~200 cycles to see the next stage's barrier, most of
+        // what four MMAs take; the other tile's MMAs fill that time (one warp for both
+        // took 980 cycles a stage, 512 of them MMAs).
         constexpr uint32_t id = idesc_16(Elem<T>::kBf16, 128, 128, 0, 0);
-        const bool lead = elect_lane();
-        const uint64_t d0 = umma_desc_sw128(sbase, 16, 1024);
-        const uint32_t hi = static_cast<uint32_t>(d0 >> 32), a_lo = static_cast<uint32_t>(d0), b_lo = a_lo + ((s_b - sbase) >> 4);
-        bool ok = true;
-        int st = 0, ph = 0;
-        if (two) ok = wait_all(smem_u32(a_moved), 0, p.err);
-        ok = ok && wait_all(smem_u32(&a_full[1]), 0, p.err);
-        tc_fence_after();
-        for (int hh = 0; hh < 2 * nh && ok; ++hh) {  // K half, V half of each head
-            for (int c = 0; c < lch && ok; ++c) {
-                ok = wait_all(smem_u32(&b_full[st]), ph, p.err);
-                if (c == 0 && hh > 0) ok = ok && wait_all(smem_u32(&acc_empty[0]), (hh - 1) & 1, p.err);
-                if (ok && lead) {
-                    tc_fence_after();
-                    const uint32_t al = a_lo + c * (kLpUnit >> 4), bl = b_lo + st * (kLeStage >> 4);
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) umma_ss_lo(tmem + 256, al + ks * 2, hi, bl + ks * 2, hi, id, ks ? 1 : c != 0);
-                    if (c == lch - 1) umma_commit(smem_u32(&acc_full[0]));
-                }
-                __syncwarp();
-                if (two) {
-                    if (c == 0 && hh > 0) ok = ok && wait_all(smem_u32(&acc_empty[1]), (hh - 1) & 1, p.err);
+        const int tile = warp == 9 ? 0 : 1;
+        if (tile == 0 || two) {
+            const bool lead = elect_lane();
+            const uint64_t d0 = umma_desc_sw128(sbase, 16, 1024);
+            const uint32_t hi = static_cast<uint32_t>(d0 >> 32), a_lo = static_cast<uint32_t>(d0), b_lo = a_lo + ((s_b - sbase) >> 4);
+            const uint32_t d = tmem + 256 + tile * 128;
+            int st = 0, ph = 0;
+            bool ok = wait_all(tile ? smem_u32(a_moved) : smem_u32(&a_full[1]), 0, p.err);
+            tc_fence_after();
+            for (int hh = 0; hh < 2 * nh && ok; ++hh) {  // K half, V half of each head
+                if (hh > 0) ok = wait_all(smem_u32(&acc_empty[tile]), (hh - 1) & 1, p.err);
+                for (int c = 0; c < lch && ok; ++c) {
+                    ok = wait_all(smem_u32(&b_full[st]), ph, p.err);
                     if (ok && lead) {
                         tc_fence_after();
                         const uint32_t bl = b_lo + st * (kLeStage >> 4);
+                        if (tile) {
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) umma_ts_lo(tmem + 384, tmem + c * 32 + ks * 8, bl + ks * 2, hi, id, ks ? 1 : c != 0);
-                        if (c == lch - 1) umma_commit(smem_u32(&acc_full[1]));
+                            for (int ks = 0; ks < 4; ++ks) umma_ts_lo(d, tmem + c * 32 + ks * 8, bl + ks * 2, hi, id, ks ? 1 : c != 0);
+                        } else {
+                            const uint32_t al = a_lo + c * (kLpUnit >> 4);
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks) umma_ss_lo(d, al + ks * 2, hi, bl + ks * 2, hi, id, ks ? 1 : c != 0);
+                        }
+                        umma_commit(smem_u32(&b_empty[st]));
+                        if (c == lch - 1) umma_commit(smem_u32(&acc_full[tile]));
                     }
                     __syncwarp();
-                }
-                if (ok && lead) umma_commit(smem_u32(&b_empty[st]));
-                __syncwarp();
-                if (++st == p.stages) {
-                    st = 0;
-                    ph ^= 1;
+                    if (++st == p.stages) {
+                        st = 0;
+                        ph ^= 1;
+                    }
                 }
             }
         }
