@@ -32,9 +32,12 @@ def _device(device) -> torch.device:
                         else int(device))
 
 
-def _stream_of(stream, device: torch.device) -> int:
+# The calls below take a few microseconds of GPU time at their smallest, so the
+# checks are kept to attribute reads.
+
+def _stream_of(stream, index: int) -> int:
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(index)
     return int(stream.cuda_stream) if hasattr(stream, "cuda_stream") else int(stream)
 
 
@@ -48,37 +51,42 @@ def _empty(shape, dtype, device: torch.device, stream) -> torch.Tensor:
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _on(t: torch.Tensor, dtype, name: str, device: torch.device) -> None:
-    if t.dtype != dtype:
+def _on(t: torch.Tensor, dtype, name: str, index: int) -> None:
+    if t.dtype is not dtype:
         raise TypeError("%s must be %s, got %s" % (name, dtype, t.dtype))
-    if t.device != device:
-        raise ValueError("%s must be on %s, got %s" % (name, device, t.device))
+    if t.get_device() != index:
+        raise ValueError("%s must be on cuda:%d, got %s" % (name, index, t.device))
 
 
-def _i32(t: torch.Tensor, name: str, device: torch.device, numel: int) -> int:
-    _on(t, torch.int32, name, device)
-    if not t.is_contiguous() or t.numel() != numel:
+def _i32(t: torch.Tensor, name: str, index: int, numel: int) -> int:
+    _on(t, torch.int32, name, index)
+    if t.numel() != numel or not t.is_contiguous():
         raise ValueError("%s must be contiguous with %d elements" % (name, numel))
     return t.data_ptr()
 
 
-def _tables(t: torch.Tensor, device: torch.device) -> int:
-    """Rows of the block tables; returns the batch."""
-    _on(t, torch.int32, "block_tables", device)
+def _tables(t: torch.Tensor, index: int) -> Tuple[int, int]:
+    """(batch, width) of the block tables."""
+    _on(t, torch.int32, "block_tables", index)
     if t.dim() != 2 or not t.is_contiguous():
         raise ValueError("block_tables must be a contiguous [batch, width] tensor")
-    return t.shape[0]
+    return t.shape
 
 
 def _token_head(t: torch.Tensor, name: str) -> Tuple[int, int]:
     """(token, head) strides of [tokens, heads, d] or [batch, tokens, heads, d] with unit stride along d and, in
     the second form, batches that follow one another."""
-    s, n = t.stride(), t.dim()
-    if n not in (3, 4) or (s[-1] != 1 and t.shape[-1] > 1):
+    s, shape = t.stride(), t.shape
+    n = len(s)
+    if n not in (3, 4) or (s[-1] != 1 and shape[-1] > 1):
         raise ValueError("%s must be [tokens, heads, d] or [batch, tokens, heads, d] with unit stride along d" % name)
-    if n == 4 and t.shape[0] > 1 and t.shape[1] > 1 and s[0] != s[1] * t.shape[1]:
+    if n == 3:
+        return s[0], s[1]
+    if shape[1] == 1:
+        return s[0], s[2]
+    if shape[0] > 1 and s[0] != s[1] * shape[1]:
         raise ValueError("%s: the batches of a 4-D view must follow one another (stride 0 = stride 1 * tokens)" % name)
-    return (s[0] if n == 4 and t.shape[1] == 1 else s[-3]), s[-2]
+    return s[1], s[2]
 
 
 class RotaryEmbedding:
@@ -103,7 +111,7 @@ class RotaryEmbedding:
         self.frequencies()
         self.handle = ctypes.c_void_p()
         self.device = _device(device) if torch.cuda.is_available() else torch.device("cpu")
-        self._cfg.device = self.device.index or 0
+        self._index = self._cfg.device = self.device.index or 0
         check(self._lib.vk_rotary_create(ctypes.byref(self._cfg), ctypes.byref(self.handle)), "vk_rotary_create")
 
     def frequencies(self) -> Tuple[List[float], float]:
@@ -118,33 +126,34 @@ class RotaryEmbedding:
         """q, k: [tokens, heads, D] (or [batch, tokens, heads, D]) fp16, bf16 or fp32, strided views allowed;
         positions: int32, one per token.  Returns the rotated q, or (q, k).  ``out``/``out_k`` may be q/k
         themselves: rotated in place."""
-        dev = self.device
-        if q.dtype not in DTYPES:
-            raise TypeError("q must be fp16, bf16 or fp32, got %s" % q.dtype)
-        d, tokens = q.shape[-1], q.numel() // max(1, q.shape[-1] * q.shape[-2]) if q.dim() > 2 else -1
-        got, views = [], []
-        for x, y, name in ((q, out, "q"), (k, out_k, "k")):
-            if x is None:
-                continue
-            v = _lib.VkRotaryView()
-            _on(x, q.dtype, name, dev)
-            v.x_token, v.x_head = _token_head(x, name)
-            if x.shape[-1] != d or x.shape[:-2] != q.shape[:-2]:
+        dev, index = self.device, self._index
+        dtype, shape = q.dtype, q.shape
+        if dtype not in DTYPES:
+            raise TypeError("q must be fp16, bf16 or fp32, got %s" % dtype)
+        d = shape[-1]
+        y, view = self._view(q, out, "q", dtype, dev, index, stream)
+        y_k = view_k = None
+        if k is not None:
+            if k.shape[:-2] != shape[:-2] or k.shape[-1] != d:
                 raise ValueError("q and k must have the same tokens and head dimension")
-            if y is None:
-                y = _empty(x.shape, x.dtype, dev, stream)
-            else:
-                _on(y, q.dtype, "out", dev)
-                if y.shape != x.shape:
-                    raise ValueError("out must have the shape of its input")
-            v.y_token, v.y_head = _token_head(y, "out")
-            v.x, v.y, v.heads = x.data_ptr(), y.data_ptr(), x.shape[-2]
-            got.append(y)
-            views.append(v)
-        check(self._lib.vk_rotary_apply(self.handle, DTYPES[q.dtype], views[0], views[1] if k is not None else None, d,
-                                        _i32(positions, "positions", dev, tokens), tokens, _stream_of(stream, dev)),
-              "vk_rotary_apply")
-        return got[0] if k is None else tuple(got)
+            y_k, view_k = self._view(k, out_k, "k", dtype, dev, index, stream)
+        tokens = shape[0] if len(shape) == 3 else shape[0] * shape[1]
+        check(self._lib.vk_rotary_apply(self.handle, DTYPES[dtype], view, view_k, d, _i32(positions, "positions", index, tokens),
+                                        tokens, _stream_of(stream, index)), "vk_rotary_apply")
+        return y if k is None else (y, y_k)
+
+    @staticmethod
+    def _view(x, y, name, dtype, dev, index, stream):
+        _on(x, dtype, name, index)
+        token, head = _token_head(x, name)
+        if y is None:
+            y = torch.empty_like(x) if stream is None and x.is_contiguous() else _empty(x.shape, dtype, dev, stream)
+        else:
+            _on(y, dtype, "out", index)
+            if y.shape != x.shape:
+                raise ValueError("out must have the shape of its input")
+        y_token, y_head = _token_head(y, "out")
+        return y, _lib.VkRotaryView(x.data_ptr(), y.data_ptr(), token, head, y_token, y_head, x.shape[-2])
 
     def close(self) -> None:
         if getattr(self, "handle", None) is not None and self.handle.value:
@@ -174,6 +183,7 @@ class LatentKVPool(PagedKVPool):
             raise TypeError("dtype must be torch.float16 or torch.bfloat16")
         self.handle = None
         self.device = storage.device if storage is not None else _device(device)
+        self._index = self.device.index
         self.num_layers, self.num_pages, self.page_tokens, self.dtype = num_layers, num_pages, page_tokens, dtype
         self.latent_dim, self.rope_dim, self.width = latent_dim, rope_dim, latent_dim + rope_dim
         self.num_kv_heads, self.head_dim, self.kv, self.kv_format = 1, self.width, False, "latent"
@@ -207,24 +217,24 @@ class LatentKVPool(PagedKVPool):
         """latent [tokens, latent_dim], k_rope [tokens, rope_dim] (row-strided views); sequence b takes the rows
         offsets[b]..offsets[b+1]-1 (None: the same number each) from position positions[b] on.  ``norm_weight``: root
         mean square norm of the latent first; ``rope``: k_rope rotated at its position."""
-        dev = self.device
-        batch = _tables(block_tables, dev)
+        dev, index = self.device, self._index
+        batch, width = _tables(block_tables, index)
         for t, name, d in ((latent, "latent", self.latent_dim), (k_rope, "k_rope", self.rope_dim)):
-            _on(t, self.dtype, name, dev)
+            _on(t, self.dtype, name, index)
             if t.dim() != 2 or t.shape[1] != d or t.stride(1) != 1:
                 raise ValueError("%s must be [tokens, %d] with unit stride along its rows" % (name, d))
         tokens = latent.shape[0]
         if k_rope.shape[0] != tokens:
             raise ValueError("latent and k_rope must have the same tokens")
         if norm_weight is not None:
-            _on(norm_weight, self.dtype, "norm_weight", dev)
+            _on(norm_weight, self.dtype, "norm_weight", index)
             if norm_weight.numel() != self.latent_dim or not norm_weight.is_contiguous():
                 raise ValueError("norm_weight must be contiguous with %d elements" % self.latent_dim)
         check(self._lib.vk_latent_append(
             self.handle, layer, latent.data_ptr(), latent.stride(0), k_rope.data_ptr(), k_rope.stride(0),
             None if norm_weight is None else norm_weight.data_ptr(), eps, None if rope is None else rope.handle,
-            block_tables.data_ptr(), block_tables.shape[1], _i32(positions, "positions", dev, batch),
-            None if offsets is None else _i32(offsets, "offsets", dev, batch + 1), batch, tokens, _stream_of(stream, dev)),
+            block_tables.data_ptr(), width, _i32(positions, "positions", index, batch),
+            None if offsets is None else _i32(offsets, "offsets", index, batch + 1), batch, tokens, _stream_of(stream, index)),
             "vk_latent_append")
 
     def decode_workspace_size(self, batch: int, tokens_per_seq: int, num_heads: int) -> int:
@@ -236,35 +246,36 @@ class LatentKVPool(PagedKVPool):
         """Absorbed form.  q_latent [B, H, latent_dim] or [B, T, H, latent_dim], q_rope likewise with rope_dim
         (rotated; strided views allowed); seq_lens [B] int32: rows to attend, the T new ones included (query token t
         sees seq_lens[b] - (T-1-t)).  Returns out like q_latent, or (out, lse)."""
-        dev = self.device
-        batch = _tables(block_tables, dev)
-        _on(q_latent, self.dtype, "q_latent", dev)
-        _on(q_rope, self.dtype, "q_rope", dev)
-        if q_latent.dim() not in (3, 4) or q_latent.shape[:-1] != q_rope.shape[:-1] or q_latent.shape[0] != batch or \
-                q_latent.shape[-1] != self.latent_dim or q_rope.shape[-1] != self.rope_dim:
+        dev, index = self.device, self._index
+        batch, width = _tables(block_tables, index)
+        _on(q_latent, self.dtype, "q_latent", index)
+        _on(q_rope, self.dtype, "q_rope", index)
+        shape = q_latent.shape
+        if len(shape) not in (3, 4) or shape[:-1] != q_rope.shape[:-1] or shape[0] != batch or shape[-1] != self.latent_dim or \
+                q_rope.shape[-1] != self.rope_dim:
             raise ValueError("q_latent must be [B, (T,) H, %d] and q_rope [B, (T,) H, %d]" % (self.latent_dim, self.rope_dim))
-        tokens, heads = (q_latent.shape[1] if q_latent.dim() == 4 else 1), q_latent.shape[-2]
+        tokens, heads = (shape[1] if len(shape) == 4 else 1), shape[-2]
         lt, lh = _token_head(q_latent, "q_latent")
         rt, rh = _token_head(q_rope, "q_rope")
         if out is None:
-            out = _empty(q_latent.shape, self.dtype, dev, stream)
+            out = torch.empty_like(q_latent) if stream is None and q_latent.is_contiguous() else _empty(shape, self.dtype, dev, stream)
         else:
-            _on(out, self.dtype, "out", dev)
-            if out.shape != q_latent.shape or not out.is_contiguous():
+            _on(out, self.dtype, "out", index)
+            if out.shape != shape or not out.is_contiguous():
                 raise ValueError("out must be contiguous with the shape of q_latent")
         if lse is not None:
-            _on(lse, torch.float32, "lse", dev)
-            if lse.shape != q_latent.shape[:-1] or not lse.is_contiguous():
+            _on(lse, torch.float32, "lse", index)
+            if lse.shape != shape[:-1] or not lse.is_contiguous():
                 raise ValueError("lse must be contiguous [B, (T,) H]")
         elif return_lse:
-            lse = _empty(q_latent.shape[:-1], torch.float32, dev, stream)
+            lse = _empty(shape[:-1], torch.float32, dev, stream)
         ws = workspace if workspace is not None else _empty((self.decode_workspace_size(batch, tokens, heads),), torch.uint8,
                                                             dev, stream)
         check(self._lib.vk_latent_decode(
             self.handle, layer, q_latent.data_ptr(), lt, lh, q_rope.data_ptr(), rt, rh, out.data_ptr(),
-            None if lse is None else lse.data_ptr(), block_tables.data_ptr(), block_tables.shape[1],
-            _i32(seq_lens, "seq_lens", dev, batch), batch, tokens, heads, scale, ws.data_ptr(),
-            ws.numel() * ws.element_size(), _stream_of(stream, dev)), "vk_latent_decode")
+            None if lse is None else lse.data_ptr(), block_tables.data_ptr(), width,
+            _i32(seq_lens, "seq_lens", index, batch), batch, tokens, heads, scale, ws.data_ptr(),
+            ws.numel() * ws.element_size(), _stream_of(stream, index)), "vk_latent_decode")
         return (out, lse) if return_lse else out
 
     def prefill_workspace_size(self, batch: int, max_seq_len: int, num_heads: int) -> int:
@@ -280,10 +291,10 @@ class LatentKVPool(PagedKVPool):
         ``max_tokens`` bounds the longest chunk (default: without offsets the chunk, with them all tokens),
         ``max_seq_len`` the longest sequence after the chunk (default: what the tables hold).  Returns
         [..., H, 128]."""
-        dev = self.device
-        batch = _tables(block_tables, dev)
-        _on(q, self.dtype, "q", dev)
-        _on(w_kv, self.dtype, "w_kv", dev)
+        dev, index = self.device, self._index
+        batch, width = _tables(block_tables, index)
+        _on(q, self.dtype, "q", index)
+        _on(w_kv, self.dtype, "w_kv", index)
         qt, qh = _token_head(q, "q")
         heads = q.shape[-2]
         if q.shape[-1] != 128 + self.rope_dim:
@@ -299,16 +310,16 @@ class LatentKVPool(PagedKVPool):
         if out is None:
             out = _empty(shape, self.dtype, dev, stream)
         else:
-            _on(out, self.dtype, "out", dev)
+            _on(out, self.dtype, "out", index)
             if out.shape != shape or not out.is_contiguous():
                 raise ValueError("out must be contiguous with shape %s" % (tuple(shape),))
         ws = workspace if workspace is not None else _empty((self.prefill_workspace_size(batch, max_seq_len, heads),),
                                                             torch.uint8, dev, stream)
         check(self._lib.vk_latent_prefill(
             self.handle, layer, q.data_ptr(), qt, qh, w_kv.data_ptr(), w_kv.stride(0), out.data_ptr(),
-            block_tables.data_ptr(), block_tables.shape[1], _i32(positions, "positions", dev, batch),
-            None if offsets is None else _i32(offsets, "offsets", dev, batch + 1), batch, tokens, max_tokens, max_seq_len,
-            heads, scale, ws.data_ptr(), ws.numel() * ws.element_size(), _stream_of(stream, dev)), "vk_latent_prefill")
+            block_tables.data_ptr(), width, _i32(positions, "positions", index, batch),
+            None if offsets is None else _i32(offsets, "offsets", index, batch + 1), batch, tokens, max_tokens, max_seq_len,
+            heads, scale, ws.data_ptr(), ws.numel() * ws.element_size(), _stream_of(stream, index)), "vk_latent_prefill")
         return out
 
     def plan(self, *args, **kwargs):
