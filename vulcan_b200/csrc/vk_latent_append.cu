@@ -27,115 +27,151 @@ struct LatentAppendParams {
     float eps;
 };
 
-constexpr int kLaWarps = 4;  // tokens per block: 16k tokens still give every SM several blocks
+constexpr int kLaWarps = 4;
 
-// The sequence of a row: the last b with offsets[b] <= row, or -1 behind the end.
-__device__ __forceinline__ int sequence_of(const int32_t* offsets, int B, int row) {
-    if (row >= __ldg(offsets + B)) return -1;
-    int lo = 0, hi = B - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (__ldg(offsets + mid) <= row) lo = mid;
-        else hi = mid - 1;
+// The sequence of a row, the last b with offsets[b] <= row, and that offset, by a
+// 32-ary search of the warp (one round of loads for up to 32 sequences); -1 behind
+// the last sequence.
+__device__ __forceinline__ int sequence_of(const int32_t* offsets, int B, int row, int lane, int* first) {
+    const int end = __ldg(offsets + B);
+    int lo = 0, n = B, at = 0;
+    do {
+        const int step = (n + 31) >> 5;
+        const int v = lane * step < n ? __ldg(offsets + lo + lane * step) : 0;
+        const unsigned le = __ballot_sync(0xffffffffu, lane * step < n && v <= row);
+        const int k = le ? 31 - __clz(le) : 0;
+        at = __shfl_sync(0xffffffffu, v, k);
+        lo += k * step;
+        n = min(step, n - k * step);
+    } while (n > 1);
+    *first = at;
+    return row < end ? lo : -1;
+}
+
+// A warp takes ROWS consecutive rows.  Every row's loads go out first; then lane t
+// looks up where row t goes (three dependent loads: sequence, position, page), all
+// rows at once, and hands it to the warp.
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(kLaWarps * 32) latent_append_kernel(const __grid_constant__ RotaryTable rot,
+                                                                      const __grid_constant__ LatentAppendParams p) {
+    const int64_t row0 = (static_cast<int64_t>(blockIdx.x) * kLaWarps + (threadIdx.x >> 5)) * ROWS;
+    const int lane = threadIdx.x & 31;
+    if (row0 >= p.tokens) return;
+    const int vecs = p.latent_dim >> 3;  // 16-byte vectors of the latent: 16..64, two a lane at most
+    // of the rotary part a lane has one pair (rope_dim <= 64): elements 2i and 2i+1, or
+    // i and i + rope_dim/2 in the half layout
+    const int pairs = p.rope_dim >> 1;
+    const bool half = rot.pairs && rot.half;
+    uint4 c[ROWS][2], wv[2];
+    uint32_t k[ROWS];
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) {
+        const int64_t row = row0 + t < p.tokens ? row0 + t : row0;
+        const uint4* src = reinterpret_cast<const uint4*>(p.latent + 2 * (row * p.latent_stride));
+        const char* ksrc = p.k_rope + 2 * (row * p.rope_stride);
+        k[t] = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            c[t][i] = lane + 32 * i < vecs ? __ldg(src + lane + 32 * i) : make_uint4(0, 0, 0, 0);
+        if (lane < pairs) {
+            if (half)
+                k[t] = __ldg(reinterpret_cast<const uint16_t*>(ksrc) + lane) |
+                       static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(ksrc) + lane + pairs)) << 16;
+            else
+                k[t] = __ldg(reinterpret_cast<const uint32_t*>(ksrc) + lane);
+        }
     }
-    return lo;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        wv[i] = p.weight && lane + 32 * i < vecs ? __ldg(reinterpret_cast<const uint4*>(p.weight) + lane + 32 * i) : make_uint4(0, 0, 0, 0);
+
+    int b = -1, first = 0;
+    if (p.offsets) {
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t) {
+            int f;
+            const int s = sequence_of(p.offsets, p.B, static_cast<int>(row0) + t, lane, &f);
+            if (lane == t) {
+                b = s;
+                first = f;
+            }
+        }
+    } else {
+        const int per = p.tokens / p.B;
+        b = static_cast<int>((row0 + lane) / per);
+        first = b * per;
+    }
+    int64_t slot = -1;  // lane t: row of the layer that row0 + t goes to
+    int my_pos = 0;
+    if (lane < ROWS && row0 + lane < p.tokens && b >= 0) {
+        const int64_t pos = static_cast<int64_t>(__ldg(p.pos + b)) + (row0 + lane - first);
+        if (row0 + lane < first || pos < 0 || pos / p.P >= p.bt_stride) {
+            atomicOr(p.err, VK_ERR_TABLE_INDEX);
+        } else {
+            const int32_t page = __ldg(p.bt + static_cast<int64_t>(b) * p.bt_stride + pos / p.P);
+            if (page < 0 || page >= p.num_pages) {
+                atomicOr(p.err, VK_ERR_PAGE_ID);
+            } else {
+                slot = static_cast<int64_t>(page) * p.P + pos % p.P;
+                my_pos = static_cast<int>(pos);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) {
+        const int64_t to = __shfl_sync(0xffffffffu, slot, t);
+        if (to < 0) continue;
+        uint4* dst = reinterpret_cast<uint4*>(p.base + 2 * to * (p.latent_dim + p.rope_dim));
+        if (p.weight) {
+            float x[2][8], sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                unpack16<T>(c[t][i], x[i]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum = fmaf(x[i][j], x[i][j], sum);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float inv = 1.f / sqrtf(sum / p.latent_dim + p.eps);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float w[8];
+                unpack16<T>(wv[i], w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[i][j] = x[i][j] * inv * w[j];
+                c[t][i] = pack16<T>(x[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (lane + 32 * i < vecs) dst[lane + 32 * i] = c[t][i];
+        const int pos = __shfl_sync(0xffffffffu, my_pos, t);
+        if (lane < pairs) {
+            if (rot.pairs) {
+                const float2 x = Elem<T>::unpack(k[t]);
+                const float2 r = rotary_turn(x.x, x.y, rotary_cos_sin(rot, lane, pos));
+                k[t] = Elem<T>::pack(r.x, r.y);
+            }
+            char* kdst = reinterpret_cast<char*>(dst + vecs);
+            if (half) {
+                reinterpret_cast<uint16_t*>(kdst)[lane] = static_cast<uint16_t>(k[t]);
+                reinterpret_cast<uint16_t*>(kdst)[lane + pairs] = static_cast<uint16_t>(k[t] >> 16);
+            } else {
+                reinterpret_cast<uint32_t*>(kdst)[lane] = k[t];
+            }
+        }
+    }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLaWarps * 32) latent_append_kernel(const __grid_constant__ RotaryTable rot,
-                                                                      const LatentAppendParams p) {
-    const int row = blockIdx.x * kLaWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (row >= p.tokens) return;
-    // the row's loads go out first; the page lookup runs behind them
-    const int vecs = p.latent_dim >> 3;  // 16-byte vectors of the latent: 16..64, two a lane at most
-    const uint4* src = reinterpret_cast<const uint4*>(p.latent + 2 * (row * p.latent_stride));
-    uint4 c[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        c[i] = lane + 32 * i < vecs ? __ldg(src + lane + 32 * i) : make_uint4(0, 0, 0, 0);
-    const uint4* ksrc = reinterpret_cast<const uint4*>(p.k_rope + 2 * (row * p.rope_stride));
-    const int kvecs = p.rope_dim >> 3;
-    // half layout: a lane takes vector j of both halves; else vector j alone
-    const int half = rot.pairs && rot.half ? kvecs >> 1 : 0;
-    const int kitems = half ? half : kvecs;
-    uint4 k0 = make_uint4(0, 0, 0, 0), k1 = k0;
-    if (lane < kitems) {
-        k0 = __ldg(ksrc + lane);
-        if (half) k1 = __ldg(ksrc + lane + half);
-    }
-    int b, t;
-    if (p.offsets) {
-        b = sequence_of(p.offsets, p.B, row);
-        if (b < 0) return;
-        t = row - __ldg(p.offsets + b);
-    } else {
-        const int per = p.tokens / p.B;
-        b = row / per;
-        t = row % per;
-    }
-    const int64_t pos = static_cast<int64_t>(__ldg(p.pos + b)) + t;
-    if (t < 0 || pos < 0 || pos / p.P >= p.bt_stride) {
-        if (lane == 0) atomicOr(p.err, VK_ERR_TABLE_INDEX);
-        return;
-    }
-    const int32_t page = __ldg(p.bt + static_cast<int64_t>(b) * p.bt_stride + pos / p.P);
-    if (page < 0 || page >= p.num_pages) {
-        if (lane == 0) atomicOr(p.err, VK_ERR_PAGE_ID);
-        return;
-    }
-    const int width = p.latent_dim + p.rope_dim;
-    uint4* dst = reinterpret_cast<uint4*>(p.base + 2 * (static_cast<uint64_t>(page) * p.P + pos % p.P) * width);
-    if (p.weight) {
-        float x[2][8], sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            unpack16<T>(c[i], x[i]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(x[i][j], x[i][j], sum);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = 1.f / sqrtf(sum / p.latent_dim + p.eps);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (lane + 32 * i >= vecs) continue;
-            float w[8];
-            unpack16<T>(__ldg(reinterpret_cast<const uint4*>(p.weight) + lane + 32 * i), w);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[i][j] = x[i][j] * inv * w[j];
-            c[i] = pack16<T>(x[i]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (lane + 32 * i < vecs) dst[lane + 32 * i] = c[i];
-    if (lane < kitems) {
-        if (rot.pairs) {
-            float u[8];
-            unpack16<T>(k0, u);
-            if (half) {
-                float w[8];
-                unpack16<T>(k1, w);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float2 r = rotary_turn(u[j], w[j], rotary_cos_sin(rot, lane * 8 + j, static_cast<int>(pos)));
-                    u[j] = r.x;
-                    w[j] = r.y;
-                }
-                k1 = pack16<T>(w);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    const float2 r = rotary_turn(u[j], u[j + 1], rotary_cos_sin(rot, lane * 4 + (j >> 1), static_cast<int>(pos)));
-                    u[j] = r.x;
-                    u[j + 1] = r.y;
-                }
-            }
-            k0 = pack16<T>(u);
-        }
-        dst[vecs + lane] = k0;
-        if (half) dst[vecs + lane + half] = k1;
-    }
+static void launch_latent_append(const RotaryTable& rot, const LatentAppendParams& p, int num_sms, cudaStream_t st) {
+    // one row a warp is the shortest way through for a decode step; chunks take two, so
+    // that one row's loads and lookups overlap the other's
+    const bool many = p.tokens >= 16 * num_sms;
+    const int64_t per = kLaWarps * (many ? 2 : 1);
+    const unsigned blocks = static_cast<unsigned>((p.tokens + per - 1) / per);
+    if (many) latent_append_kernel<T, 2><<<blocks, kLaWarps * 32, 0, st>>>(rot, p);
+    else latent_append_kernel<T, 1><<<blocks, kLaWarps * 32, 0, st>>>(rot, p);
 }
 
 }  // namespace vk
@@ -181,11 +217,8 @@ extern "C" vk_status vk_latent_append(vk_pool* pool, int32_t layer, const void* 
     p.num_pages = pool->num_pages;
     p.eps = eps;
     DeviceGuard g(pool->device);
-    const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(tokens) + kLaWarps - 1) / kLaWarps);
-    if (pool->kv_format == VK_KV_LATENT_BF16)
-        latent_append_kernel<__nv_bfloat16><<<blocks, kLaWarps * 32, 0, as_stream(stream)>>>(*rot, p);
-    else
-        latent_append_kernel<__half><<<blocks, kLaWarps * 32, 0, as_stream(stream)>>>(*rot, p);
+    if (pool->kv_format == VK_KV_LATENT_BF16) launch_latent_append<__nv_bfloat16>(*rot, p, pool->num_sms, as_stream(stream));
+    else launch_latent_append<__half>(*rot, p, pool->num_sms, as_stream(stream));
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? VK_OK : cuda_fail(e, "latent_append_kernel launch");
 }

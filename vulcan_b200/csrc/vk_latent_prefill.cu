@@ -99,6 +99,9 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the attention may start its launch: it reads what this kernel writes only behind
+    // griddepcontrol.wait
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int b = blockIdx.z, key0 = blockIdx.y * kLeTokens;
     const LpSeq sq = lp_seq(p, b, threadIdx.x == 0 && blockIdx.x == 0 && key0 == 0 && p.h0 == 0);
     const int len = sq.pos + sq.n;
@@ -334,7 +337,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
     const int b = blockIdx.z, hl = blockIdx.y, h = p.h0 + hl;
     const LpSeq sq = lp_seq(p, b, false);
     const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * kLpRows;  // most keys first
-    if (q0 >= sq.n) return;
+    if (q0 >= sq.n) {  // (this grid must not end before the expansion does)
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     const int pos0 = sq.pos;
     const int rowsA = min(kLpRows, sq.n - q0), rowsB = max(0, min(kLpRows, sq.n - q0 - kLpRows));
     const int lenA = pos0 + q0 + rowsA, lenB = rowsB > 0 ? pos0 + q0 + kLpRows + rowsB : 0;
@@ -394,6 +400,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
             const uint64_t pol = l2_evict_last_policy();  // other row tiles read the same K and V
             const int wrow = b * p.lpad, u = warp == 8 ? 0 : 1;
             bool ok = true;
+            asm volatile("griddepcontrol.wait;" ::: "memory");
             for (int j = 0; j < ntiles; ++j) {
                 if (j >= 2) ok = ok && mbar_wait(smem_u32(&v_empty[j & 1]), ((j >> 1) - 1) & 1, p.err);
                 if (!ok) break;
@@ -664,8 +671,17 @@ static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensor
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "latent_expand_kernel launch");
     const dim3 grid((p.max_tokens + 2 * kLpRows - 1) / (2 * kLpRows), p.heads, p.B);
-    latent_prefill_kernel<T><<<grid, kLaThreads, kLaSmem, st>>>(pool->tmap16, tq, tkv, p);
-    e = cudaGetLastError();
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kLaThreads);
+    cfg.dynamicSmemBytes = kLaSmem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, latent_prefill_kernel<T>, pool->tmap16, tq, tkv, p);
     if (e != cudaSuccess) return cuda_fail(e, "latent_prefill_kernel launch");
     return VK_OK;
 }

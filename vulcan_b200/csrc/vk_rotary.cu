@@ -37,35 +37,44 @@ struct RotaryParams {
     int slices;     // blocks per token
 };
 
-constexpr int kRotThreads = 256;
+constexpr int kRotThreads = 128;
 
 // Block (token, slice of its items): the token's cos and sin once into shared
 // memory (sincospi of each pair, shared by every head), then one item per
-// thread.  An item is 16 bytes of one head (interleaved), the two 16-byte
-// halves of 4 or 8 pairs (half layout), or 16 bytes behind rotary_dim to copy;
-// with VEC 0 a single pair or element, for pointers and strides that are not
-// 16-byte multiples.  The loads go out before the cos/sin are computed.
+// thread (two or four in flight measured the same or slower).  An item is 16 bytes of one head (interleaved), the two 16-byte halves of 4 or 8
+// pairs (half layout), or 16 bytes behind rotary_dim to copy; with VEC 0 a single
+// pair or element, for pointers and strides that are not 16-byte multiples.  The
+// loads go out before the cos/sin are computed.
 template <typename T, int HALF, int VEC>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotaryTable tab, const RotaryParams p) {
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_constant__ RotaryTable tab,
+                                                             const __grid_constant__ RotaryParams p) {
     __shared__ float2 cs[kRotaryMaxPairs];
     const int token = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
-    const int item = slice * kRotThreads + threadIdx.x;
+    const int item = slice * kRotThreads + threadIdx.x, half = tab.pairs;
     const bool live = item < p.items;
-    const int head = live ? item / p.per_head : 0, j = live ? item % p.per_head : 0;
-    const RotaryView& v = head >= p.v[0].heads ? p.v[1] : p.v[0];
-    const int h = head >= p.v[0].heads ? head - p.v[0].heads : head;
-    const T* x = reinterpret_cast<const T*>(v.x) + token * v.x_token + h * v.x_head;
-    T* y = reinterpret_cast<T*>(v.y) + token * v.y_token + h * v.y_head;
-    const bool rot = j < p.rotated;
-    const int half = tab.pairs;
+    const T* x = nullptr;
+    T* y = nullptr;
+    int j = 0;
+    bool rot = false;
+    if (live) {
+        const int head = item / p.per_head;
+        j = item % p.per_head;
+        rot = j < p.rotated;
+        const bool is_k = head >= p.v[0].heads;
+        const RotaryView& v = is_k ? p.v[1] : p.v[0];
+        const int h = is_k ? head - p.v[0].heads : head;
+        x = reinterpret_cast<const T*>(v.x) + token * v.x_token + h * v.x_head;
+        y = reinterpret_cast<T*>(v.y) + token * v.y_token + h * v.y_head;
+    }
     if constexpr (VEC != 0) {
         constexpr int N = Elem<T>::kVec;
-        // element offsets of the item's first and (half layout, rotated) second vector
-        const int e0 = rot ? j * N : (HALF ? 2 * half + (j - p.rotated) * N : j * N);
-        uint4 a = make_uint4(0, 0, 0, 0), b = a;
+        // element of the item's first vector; (half layout, rotated) the second is `half` on
+        const int e0 = rot || !HALF ? j * N : 2 * half + (j - p.rotated) * N;
+        uint4 a, b;
         if (live) {
             a = *reinterpret_cast<const uint4*>(x + e0);
             if (HALF && rot) b = *reinterpret_cast<const uint4*>(x + half + e0);
+            y += e0;
         }
         for (int i = threadIdx.x; i < half; i += kRotThreads) cs[i] = rotary_cos_sin(tab, i, __ldg(p.pos + token));
         __syncthreads();
@@ -82,7 +91,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
                     u[i] = r.x;
                     w[i] = r.y;
                 }
-                *reinterpret_cast<uint4*>(y + half + e0) = pack16<T>(w);
+                *reinterpret_cast<uint4*>(y + half) = pack16<T>(w);
             } else {
 #pragma unroll
                 for (int i = 0; i < N; i += 2) {
@@ -93,7 +102,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
             }
             a = pack16<T>(u);
         }
-        *reinterpret_cast<uint4*>(y + e0) = a;
+        *reinterpret_cast<uint4*>(y) = a;
     } else {
         for (int i = threadIdx.x; i < half; i += kRotThreads) cs[i] = rotary_cos_sin(tab, i, __ldg(p.pos + token));
         __syncthreads();
@@ -112,18 +121,13 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const __grid_consta
 
 const RotaryTable* rotary_table(const vk_rotary* r) { return &r->table; }
 
-template <typename T>
+template <typename T, int HALF>
 static vk_status launch_rotary(const vk_rotary* r, const RotaryParams& p, bool vec, cudaStream_t st) {
     const int64_t blocks = static_cast<int64_t>(p.tokens) * p.slices;
     if (blocks > 0x7fffffff) return fail(VK_INVALID_ARG, "rotary: too many tokens for one launch");
     const dim3 grid(static_cast<unsigned>(blocks));
-    if (r->table.half) {
-        if (vec) rotary_kernel<T, 1, 1><<<grid, kRotThreads, 0, st>>>(r->table, p);
-        else rotary_kernel<T, 1, 0><<<grid, kRotThreads, 0, st>>>(r->table, p);
-    } else {
-        if (vec) rotary_kernel<T, 0, 1><<<grid, kRotThreads, 0, st>>>(r->table, p);
-        else rotary_kernel<T, 0, 0><<<grid, kRotThreads, 0, st>>>(r->table, p);
-    }
+    if (vec) rotary_kernel<T, HALF, 1><<<grid, kRotThreads, 0, st>>>(r->table, p);
+    else rotary_kernel<T, HALF, 0><<<grid, kRotThreads, 0, st>>>(r->table, p);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? VK_OK : cuda_fail(e, "rotary_kernel launch");
 }
@@ -260,7 +264,10 @@ extern "C" vk_status vk_rotary_apply(const vk_rotary* r, int32_t dtype, const vk
     p.head_dim = head_dim;
     DeviceGuard g(r->device);
     cudaStream_t st = as_stream(stream);
-    if (dtype == VK_F16) return launch_rotary<__half>(r, p, vec, st);
-    if (dtype == VK_BF16) return launch_rotary<__nv_bfloat16>(r, p, vec, st);
-    return launch_rotary<float>(r, p, vec, st);
+    const bool half = r->table.half;
+    switch (dtype) {
+        case VK_F16: return half ? launch_rotary<__half, 1>(r, p, vec, st) : launch_rotary<__half, 0>(r, p, vec, st);
+        case VK_BF16: return half ? launch_rotary<__nv_bfloat16, 1>(r, p, vec, st) : launch_rotary<__nv_bfloat16, 0>(r, p, vec, st);
+        default: return half ? launch_rotary<float, 1>(r, p, vec, st) : launch_rotary<float, 0>(r, p, vec, st);
+    }
 }
