@@ -4,10 +4,13 @@
 //
 //   row = [ c / sqrt(mean(c^2) + eps) * w  |  R(pos) k ]
 //
-// Bound by memory for chunks (2 * (latent + rope) * 2 bytes a token) and by
-// latency for a decode step.  One warp per token: the row stays in registers
-// between the sum of squares (fp32, one shuffle tree) and the scaled store, so
-// it is read once and written once, in 16-byte vectors.
+// Floor: 2 * (latent + rope) * 2 bytes a token.  One warp per token: the row stays in
+// registers between the sum of squares (fp32, one shuffle tree) and the scaled
+// store, so it is read once and written once, the latent in 16-byte vectors.
+// Bound by latency: 2.8 us for a decode step; 17.6k tokens of 512 + 64 take 13.6 us,
+// 3.0 TB/s (the memory alone 6.3): ~20% of the time is the launch, the rest four
+// dependent loads a warp at 44 registers (two and four rows a warp measured 14.0 and
+// 14.6 us, blocks of two and eight warps 14.0 and 14.7).
 #include "vk_internal.h"
 #include "vk_rotary.cuh"
 
@@ -23,8 +26,8 @@ struct LatentAppendParams {
     const int32_t* pos;
     const int32_t* offsets;
     uint32_t* err;
-    int bt_stride, B, tokens, latent_dim, rope_dim, P, num_pages;
-    float eps;
+    int bt_stride, B, tokens, latent_dim, rope_dim, P_log2, num_pages;
+    float eps, inv_dim;
 };
 
 constexpr int kLaWarps = 4;
@@ -48,130 +51,94 @@ __device__ __forceinline__ int sequence_of(const int32_t* offsets, int B, int ro
     return row < end ? lo : -1;
 }
 
-// A warp takes ROWS consecutive rows.  Every row's loads go out first; then lane t
-// looks up where row t goes (three dependent loads: sequence, position, page), all
-// rows at once, and hands it to the warp.
-template <typename T, int ROWS>
+template <typename T>
 __global__ void __launch_bounds__(kLaWarps * 32) latent_append_kernel(const __grid_constant__ RotaryTable rot,
                                                                       const __grid_constant__ LatentAppendParams p) {
-    const int64_t row0 = (static_cast<int64_t>(blockIdx.x) * kLaWarps + (threadIdx.x >> 5)) * ROWS;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kLaWarps + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    if (row0 >= p.tokens) return;
+    if (row >= p.tokens) return;
+    // the row's loads go out first; the lookups (three dependent loads: sequence,
+    // position, page) run behind them
     const int vecs = p.latent_dim >> 3;  // 16-byte vectors of the latent: 16..64, two a lane at most
     // of the rotary part a lane has one pair (rope_dim <= 64): elements 2i and 2i+1, or
     // i and i + rope_dim/2 in the half layout
     const int pairs = p.rope_dim >> 1;
     const bool half = rot.pairs && rot.half;
-    uint4 c[ROWS][2], wv[2];
-    uint32_t k[ROWS];
+    const uint4* src = reinterpret_cast<const uint4*>(p.latent + 2 * (row * p.latent_stride));
+    const char* ksrc = p.k_rope + 2 * (row * p.rope_stride);
+    uint4 c[2], wv[2];
+    uint32_t k = 0;
 #pragma unroll
-    for (int t = 0; t < ROWS; ++t) {
-        const int64_t row = row0 + t < p.tokens ? row0 + t : row0;
-        const uint4* src = reinterpret_cast<const uint4*>(p.latent + 2 * (row * p.latent_stride));
-        const char* ksrc = p.k_rope + 2 * (row * p.rope_stride);
-        k[t] = 0;
+    for (int i = 0; i < 2; ++i) {
+        const bool in = lane + 32 * i < vecs;
+        c[i] = in ? __ldg(src + lane + 32 * i) : make_uint4(0, 0, 0, 0);
+        wv[i] = in && p.weight ? __ldg(reinterpret_cast<const uint4*>(p.weight) + lane + 32 * i) : make_uint4(0, 0, 0, 0);
+    }
+    if (lane < pairs) {
+        if (half)
+            k = __ldg(reinterpret_cast<const uint16_t*>(ksrc) + lane) |
+                static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(ksrc) + lane + pairs)) << 16;
+        else
+            k = __ldg(reinterpret_cast<const uint32_t*>(ksrc) + lane);
+    }
+    int b, first;
+    if (p.offsets) {
+        b = sequence_of(p.offsets, p.B, static_cast<int>(row), lane, &first);
+        if (b < 0) return;
+    } else {
+        const int per = p.tokens / p.B;
+        b = static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(per));
+        first = b * per;
+    }
+    const int64_t pos = static_cast<int64_t>(__ldg(p.pos + b)) + (row - first);
+    if (row < first || pos < 0 || (pos >> p.P_log2) >= p.bt_stride) {
+        if (lane == 0) atomicOr(p.err, VK_ERR_TABLE_INDEX);
+        return;
+    }
+    const int32_t page = __ldg(p.bt + static_cast<int64_t>(b) * p.bt_stride + (pos >> p.P_log2));
+    if (page < 0 || page >= p.num_pages) {
+        if (lane == 0) atomicOr(p.err, VK_ERR_PAGE_ID);
+        return;
+    }
+    const int64_t slot = (static_cast<int64_t>(page) << p.P_log2) + (pos & ((1 << p.P_log2) - 1));
+    uint4* dst = reinterpret_cast<uint4*>(p.base + 2 * slot * (p.latent_dim + p.rope_dim));
+    if (p.weight) {
+        float x[2][8], sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            c[t][i] = lane + 32 * i < vecs ? __ldg(src + lane + 32 * i) : make_uint4(0, 0, 0, 0);
-        if (lane < pairs) {
-            if (half)
-                k[t] = __ldg(reinterpret_cast<const uint16_t*>(ksrc) + lane) |
-                       static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(ksrc) + lane + pairs)) << 16;
-            else
-                k[t] = __ldg(reinterpret_cast<const uint32_t*>(ksrc) + lane);
+        for (int i = 0; i < 2; ++i) {
+            unpack16<T>(c[i], x[i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum = fmaf(x[i][j], x[i][j], sum);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = rsqrtf(sum * p.inv_dim + p.eps);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float w[8];
+            unpack16<T>(wv[i], w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[i][j] = x[i][j] * inv * w[j];
+            c[i] = pack16<T>(x[i]);
         }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-        wv[i] = p.weight && lane + 32 * i < vecs ? __ldg(reinterpret_cast<const uint4*>(p.weight) + lane + 32 * i) : make_uint4(0, 0, 0, 0);
-
-    int b = -1, first = 0;
-    if (p.offsets) {
-#pragma unroll
-        for (int t = 0; t < ROWS; ++t) {
-            int f;
-            const int s = sequence_of(p.offsets, p.B, static_cast<int>(row0) + t, lane, &f);
-            if (lane == t) {
-                b = s;
-                first = f;
-            }
+        if (lane + 32 * i < vecs) dst[lane + 32 * i] = c[i];
+    if (lane < pairs) {
+        if (rot.pairs) {
+            const float2 x = Elem<T>::unpack(k);
+            const float2 r = rotary_turn(x.x, x.y, rotary_cos_sin(rot, lane, static_cast<int>(pos)));
+            k = Elem<T>::pack(r.x, r.y);
         }
-    } else {
-        const int per = p.tokens / p.B;
-        b = static_cast<int>((row0 + lane) / per);
-        first = b * per;
-    }
-    int64_t slot = -1;  // lane t: row of the layer that row0 + t goes to
-    int my_pos = 0;
-    if (lane < ROWS && row0 + lane < p.tokens && b >= 0) {
-        const int64_t pos = static_cast<int64_t>(__ldg(p.pos + b)) + (row0 + lane - first);
-        if (row0 + lane < first || pos < 0 || pos / p.P >= p.bt_stride) {
-            atomicOr(p.err, VK_ERR_TABLE_INDEX);
+        char* kdst = reinterpret_cast<char*>(dst + vecs);
+        if (half) {
+            reinterpret_cast<uint16_t*>(kdst)[lane] = static_cast<uint16_t>(k);
+            reinterpret_cast<uint16_t*>(kdst)[lane + pairs] = static_cast<uint16_t>(k >> 16);
         } else {
-            const int32_t page = __ldg(p.bt + static_cast<int64_t>(b) * p.bt_stride + pos / p.P);
-            if (page < 0 || page >= p.num_pages) {
-                atomicOr(p.err, VK_ERR_PAGE_ID);
-            } else {
-                slot = static_cast<int64_t>(page) * p.P + pos % p.P;
-                my_pos = static_cast<int>(pos);
-            }
+            reinterpret_cast<uint32_t*>(kdst)[lane] = k;
         }
     }
-#pragma unroll
-    for (int t = 0; t < ROWS; ++t) {
-        const int64_t to = __shfl_sync(0xffffffffu, slot, t);
-        if (to < 0) continue;
-        uint4* dst = reinterpret_cast<uint4*>(p.base + 2 * to * (p.latent_dim + p.rope_dim));
-        if (p.weight) {
-            float x[2][8], sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                unpack16<T>(c[t][i], x[i]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum = fmaf(x[i][j], x[i][j], sum);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const float inv = 1.f / sqrtf(sum / p.latent_dim + p.eps);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float w[8];
-                unpack16<T>(wv[i], w);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[i][j] = x[i][j] * inv * w[j];
-                c[t][i] = pack16<T>(x[i]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (lane + 32 * i < vecs) dst[lane + 32 * i] = c[t][i];
-        const int pos = __shfl_sync(0xffffffffu, my_pos, t);
-        if (lane < pairs) {
-            if (rot.pairs) {
-                const float2 x = Elem<T>::unpack(k[t]);
-                const float2 r = rotary_turn(x.x, x.y, rotary_cos_sin(rot, lane, pos));
-                k[t] = Elem<T>::pack(r.x, r.y);
-            }
-            char* kdst = reinterpret_cast<char*>(dst + vecs);
-            if (half) {
-                reinterpret_cast<uint16_t*>(kdst)[lane] = static_cast<uint16_t>(k[t]);
-                reinterpret_cast<uint16_t*>(kdst)[lane + pairs] = static_cast<uint16_t>(k[t] >> 16);
-            } else {
-                reinterpret_cast<uint32_t*>(kdst)[lane] = k[t];
-            }
-        }
-    }
-}
-
-template <typename T>
-static void launch_latent_append(const RotaryTable& rot, const LatentAppendParams& p, int num_sms, cudaStream_t st) {
-    // one row a warp is the shortest way through for a decode step; chunks take two, so
-    // that one row's loads and lookups overlap the other's
-    const bool many = p.tokens >= 16 * num_sms;
-    const int64_t per = kLaWarps * (many ? 2 : 1);
-    const unsigned blocks = static_cast<unsigned>((p.tokens + per - 1) / per);
-    if (many) latent_append_kernel<T, 2><<<blocks, kLaWarps * 32, 0, st>>>(rot, p);
-    else latent_append_kernel<T, 1><<<blocks, kLaWarps * 32, 0, st>>>(rot, p);
 }
 
 }  // namespace vk
@@ -213,12 +180,16 @@ extern "C" vk_status vk_latent_append(vk_pool* pool, int32_t layer, const void* 
     p.tokens = tokens;
     p.latent_dim = pool->latent_dim;
     p.rope_dim = pool->rope_dim;
-    p.P = pool->cfg.page_tokens;
+    p.P_log2 = pool->cfg.page_tokens == 16 ? 4 : pool->cfg.page_tokens == 32 ? 5 : 6;
     p.num_pages = pool->num_pages;
     p.eps = eps;
+    p.inv_dim = 1.f / static_cast<float>(pool->latent_dim);
     DeviceGuard g(pool->device);
-    if (pool->kv_format == VK_KV_LATENT_BF16) launch_latent_append<__nv_bfloat16>(*rot, p, pool->num_sms, as_stream(stream));
-    else launch_latent_append<__half>(*rot, p, pool->num_sms, as_stream(stream));
+    const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(tokens) + kLaWarps - 1) / kLaWarps);
+    if (pool->kv_format == VK_KV_LATENT_BF16)
+        latent_append_kernel<__nv_bfloat16><<<blocks, kLaWarps * 32, 0, as_stream(stream)>>>(*rot, p);
+    else
+        latent_append_kernel<__half><<<blocks, kLaWarps * 32, 0, as_stream(stream)>>>(*rot, p);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? VK_OK : cuda_fail(e, "latent_append_kernel launch");
 }
