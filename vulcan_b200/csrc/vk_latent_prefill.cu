@@ -49,6 +49,9 @@ struct LpParams {
     char* ws;     // [B * lpad][heads][256]
     char* out;    // [tokens][H][128]
     int bt_stride, B, tokens, H, heads, h0, layer, num_pages, P, latent, rope, lpad, max_tokens, max_len, stages, per_cta;
+    int q_tiles, splits;   // attention: 256-row tiles of the longest chunk, key ranges a CTA's tile is cut into
+    float* part_o;         // splits > 1: [q tile of (b, head)][split][256][128] unnormalised O
+    float2* part_ml;       // and its (maximum, sum) [..][256]
     float scale_log2;
 };
 
@@ -325,7 +328,7 @@ constexpr int kLaBar = kLaRing + kLaUnits * kLpUnit;  // 224 KiB
 constexpr int kLaSmem = kLaBar + 256 + 1024;
 static_assert(kLaSmem <= kLpSmemMax, "latent prefill shared memory");
 
-template <typename T>
+template <typename T, bool SPLIT>  // SPLIT: the CTA has one of p.splits ranges of the keys
 __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __grid_constant__ CUtensorMap tmap,
                                                                        const __grid_constant__ CUtensorMap tmapq,
                                                                        const __grid_constant__ CUtensorMap tmapkv,
@@ -334,9 +337,9 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = blockIdx.z, hl = blockIdx.y, h = p.h0 + hl;
+    const int b = SPLIT ? blockIdx.z / p.splits : blockIdx.z, split = SPLIT ? blockIdx.z % p.splits : 0, hl = blockIdx.y, h = p.h0 + hl;
     const LpSeq sq = lp_seq(p, b, false);
-    const int q0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * kLpRows;  // most keys first
+    const int qt = p.q_tiles - 1 - static_cast<int>(blockIdx.x), q0 = qt * 2 * kLpRows;  // most keys first
     if (q0 >= sq.n) {  // (this grid must not end before the expansion does)
         asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
@@ -344,8 +347,12 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
     const int pos0 = sq.pos;
     const int rowsA = min(kLpRows, sq.n - q0), rowsB = max(0, min(kLpRows, sq.n - q0 - kLpRows));
     const int lenA = pos0 + q0 + rowsA, lenB = rowsB > 0 ? pos0 + q0 + kLpRows + rowsB : 0;
-    const int ntA = (lenA + kLpKeys - 1) / kLpKeys, ntB = (lenB + kLpKeys - 1) / kLpKeys;
-    const int kv_len = max(lenA, lenB), ntiles = max(ntA, ntB);
+    // this CTA's key tiles kt0 .. kt0 + ntiles - 1; row tile A (B) sees the first ntA (ntB)
+    const int kv_len = max(lenA, lenB), all = (kv_len + kLpKeys - 1) / kLpKeys;
+    const int kt0 = SPLIT ? static_cast<int>(static_cast<int64_t>(split) * all / p.splits) : 0;
+    const int ntiles = SPLIT ? static_cast<int>(static_cast<int64_t>(split + 1) * all / p.splits) - kt0 : all;
+    const int ntA = max(0, min(ntiles, (lenA + kLpKeys - 1) / kLpKeys - kt0));
+    const int ntB = max(0, min(ntiles, (lenB + kLpKeys - 1) / kLpKeys - kt0));
 
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kLaBar);
     uint64_t* k_full = bars;       // [2] the three K units of a tile landed
@@ -398,7 +405,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
         // units 5j+3, 5j+4 those of tile j-1's first two K units
         if (lane == 0) {
             const uint64_t pol = l2_evict_last_policy();  // other row tiles read the same K and V
-            const int wrow = b * p.lpad, u = warp == 8 ? 0 : 1;
+            const int wrow = b * p.lpad + kt0 * kLpKeys, u = warp == 8 ? 0 : 1;
             bool ok = true;
             asm volatile("griddepcontrol.wait;" ::: "memory");
             for (int j = 0; j < ntiles; ++j) {
@@ -406,7 +413,8 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
                 if (!ok) break;
                 const uint32_t kbar = smem_u32(&k_full[j & 1]), vbar = smem_u32(&v_full[j & 1]);
                 mbar_expect_tx(kbar, kLpUnit);
-                tma_load_2d(sbase + kLaRing + ((5 * j + u) & 7) * kLpUnit, &tmapkv, hl * 256 + u * 64, wrow + j * kLpKeys, kbar, pol);
+                tma_load_2d(sbase + kLaRing + ((5 * j + u) & 7) * kLpUnit, &tmapkv, hl * 256 + u * 64, wrow + j * kLpKeys,
+                            kbar, pol);
                 if (j >= 1) ok = mbar_wait(smem_u32(&k_empty[(j - 1) & 1]), ((j - 1) >> 1) & 1, p.err);
                 if (!ok) break;
                 mbar_expect_tx(vbar, kLpUnit);
@@ -418,8 +426,8 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
         // ------------------------------------------------------------ TMA: rotary parts from the pages
         // (a warp of its own: eight 16-token pages take ~600 cycles to issue)
         const uint64_t pol = l2_evict_last_policy();
-        const int32_t* btrow = p.bt + static_cast<int64_t>(b) * p.bt_stride;
-        const int npages = (kv_len + p.P - 1) / p.P, ppt = kLpKeys / p.P;
+        const int ppt = kLpKeys / p.P, npages = (kv_len + p.P - 1) / p.P - kt0 * ppt;  // from the first tile's on
+        const int32_t* btrow = p.bt + static_cast<int64_t>(b) * p.bt_stride + kt0 * ppt;
         auto page_of = [&](int j) {  // a page of the tile per lane
             int page = lane < ppt && j * ppt + lane < npages ? __ldg(btrow + j * ppt + lane) : 0;
             if (page < 0 || page >= p.num_pages) {
@@ -508,7 +516,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
             }
             __syncwarp();
         };
-        issue_s(0, 0);
+        if (ntA > 0) issue_s(0, 0);
         if (ntB > 0) issue_s(1, 0);
         for (int j = 0; j < ntiles && ok; ++j) {
             if (j < ntA) {
@@ -533,7 +541,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
         for (int j = 0; j < ntt; ++j) {
             if (!wait_all(smem_u32(&s_full[t]), j & 1, p.err)) { alive = false; break; }
             tc_fence_after();
-            const int key0 = j * kLpKeys;
+            const int key0 = (kt0 + j) * kLpKeys;
             float v[kLpKeys / 32][32];
 #pragma unroll
             for (int c = 0; c < kLpKeys / 32; ++c) tmem_ld32(lane_base + s_col + c * 32, v[c]);
@@ -560,7 +568,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
             float alpha = 1.f;
             if (mx > m_ref + 8.f || m_ref == -INFINITY) {
                 const float m_new = fmaxf(m_ref, mx);
-                alpha = ex2(m_ref - m_new);
+                alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - m_new);
                 m_ref = m_new;
             }
             const float mneg = m_ref == -INFINITY ? 0.f : -m_ref;
@@ -602,16 +610,24 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&p_full[t]));
         }
+        const int64_t part = SPLIT ? ((((static_cast<int64_t>(b) * p.heads + hl) * p.q_tiles + qt) * p.splits + split) * 256 + t * kLpRows + r) : 0;
+        if (SPLIT) p.part_ml[part] = make_float2(m_ref, l);  // (-inf, 0) where no key is seen
         if (alive && ntt > 0 && wait_all(smem_u32(&o_full[t]), (ntt - 1) & 1, p.err)) {
             tc_fence_after();
             const float inv = 1.f / l;
-            char* dst = p.out + 2 * ((static_cast<int64_t>(sq.row0) + (valid_row ? qrow : 0)) * p.H + h) * kLpHead;
+            char* dst = SPLIT ? reinterpret_cast<char*>(p.part_o + part * kLpHead)
+                              : p.out + 2 * ((static_cast<int64_t>(sq.row0) + (valid_row ? qrow : 0)) * p.H + h) * kLpHead;
 #pragma unroll
             for (int c = 0; c < kLpHead / 32; ++c) {
                 float o[32];
                 tmem_ld32(lane_base + o_col + c * 32, o);
                 tmem_wait_ld();
-                if (valid_row) {
+                if (!valid_row) continue;
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4*>(dst + 4 * (c * 32 + i)) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                } else {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8)
                         *reinterpret_cast<uint4*>(dst + 2 * (c * 32 + i)) =
@@ -629,8 +645,41 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
     }
 }
 
+// Joins the key ranges of a query row: a warp per (row, head), four elements a lane.
+template <typename T>
+__global__ void __launch_bounds__(128) latent_prefill_merge_kernel(const __grid_constant__ LpParams p) {
+    const int lane = threadIdx.x & 31, b = blockIdx.z, hl = blockIdx.y, qrow = blockIdx.x * 4 + (threadIdx.x >> 5);
+    const LpSeq sq = lp_seq(p, b, false);
+    if (qrow >= sq.n) return;
+    const int64_t part0 = ((static_cast<int64_t>(b) * p.heads + hl) * p.q_tiles + (qrow >> 8)) * p.splits;
+    float2 ml = make_float2(-INFINITY, 0.f);  // lane s: split s (at most 16)
+    if (lane < p.splits) ml = p.part_ml[(part0 + lane) * 256 + (qrow & 255)];
+    float m = ml.x;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = __shfl_sync(0xffffffffu, m, 0);
+    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+    float l = f * ml.y;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    l = __shfl_sync(0xffffffffu, l, 0);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.splits; ++s) {
+        const float w = __shfl_sync(0xffffffffu, f, s);
+        if (w == 0.f) continue;  // a range that the row does not see has no O
+        const float4 x = *reinterpret_cast<const float4*>(p.part_o + ((part0 + s) * 256 + (qrow & 255)) * kLpHead + lane * 4);
+        acc = make_float4(fmaf(w, x.x, acc.x), fmaf(w, x.y, acc.y), fmaf(w, x.z, acc.z), fmaf(w, x.w, acc.w));
+    }
+    const float inv = 1.f / l;
+    char* dst = p.out + 2 * ((static_cast<int64_t>(sq.row0) + qrow) * p.H + p.h0 + hl) * kLpHead;
+    *reinterpret_cast<uint2*>(dst + lane * 8) = make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
+}
+
 // Heads whose keys and values the workspace holds at once: all, up to 1 GiB.
 constexpr uint64_t kLpWorkspace = 1ull << 30;
+constexpr int kLpMaxSplits = 16;
+// Partials of split query tiles: at most one CTA per SM.
+static size_t lp_part_bytes(const vk_pool* pool) { return static_cast<size_t>(pool->num_sms) * 256 * (kLpHead * 4 + 8); }
 static int lp_heads(int64_t rows, int H) {
     const uint64_t per_head = static_cast<uint64_t>(rows) * 512;
     const int64_t fit = static_cast<int64_t>(kLpWorkspace / per_head);
@@ -647,7 +696,9 @@ static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensor
     if (!(attr_set & bit)) {
         cudaError_t e = cudaFuncSetAttribute(latent_expand_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLpSmemMax);
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(latent_prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLaSmem);
+            e = cudaFuncSetAttribute(latent_prefill_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLaSmem);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(latent_prefill_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLaSmem);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(latent prefill)");
         attr_set |= bit;
     }
@@ -670,7 +721,14 @@ static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensor
     latent_expand_kernel<T><<<dim3((p.heads + p.per_cta - 1) / p.per_cta, row_tiles, p.B), kLeThreads, smem, st>>>(pool->tmap16, tw, tkv, p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "latent_expand_kernel launch");
-    const dim3 grid((p.max_tokens + 2 * kLpRows - 1) / (2 * kLpRows), p.heads, p.B);
+    // Too few CTAs for the GPU: each (query tile, head, sequence) is cut along its keys,
+    // into ranges of six key tiles or more (200 new tokens behind 30k, 8 heads: 598 us
+    // without, 134 with; 1,030 behind none in two ranges: 44 instead of 35).
+    p.q_tiles = (p.max_tokens + 2 * kLpRows - 1) / (2 * kLpRows);
+    const int64_t base = static_cast<int64_t>(p.q_tiles) * p.heads * p.B;
+    p.splits = static_cast<int>(max(static_cast<int64_t>(1), min(min(static_cast<int64_t>(kLpMaxSplits), pool->num_sms / base),
+                                                                  static_cast<int64_t>(p.max_len / (6 * kLpKeys)))));
+    const dim3 grid(p.q_tiles, p.heads, p.B * p.splits);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -681,8 +739,14 @@ static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensor
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, latent_prefill_kernel<T>, pool->tmap16, tq, tkv, p);
+    e = p.splits > 1 ? cudaLaunchKernelEx(&cfg, latent_prefill_kernel<T, true>, pool->tmap16, tq, tkv, p)
+                     : cudaLaunchKernelEx(&cfg, latent_prefill_kernel<T, false>, pool->tmap16, tq, tkv, p);
     if (e != cudaSuccess) return cuda_fail(e, "latent_prefill_kernel launch");
+    if (p.splits > 1) {
+        latent_prefill_merge_kernel<T><<<dim3((p.max_tokens + 3) / 4, p.heads, p.B), 128, 0, st>>>(p);
+        e = cudaGetLastError();
+        if (e != cudaSuccess) return cuda_fail(e, "latent_prefill_merge_kernel launch");
+    }
     return VK_OK;
 }
 
@@ -694,7 +758,7 @@ extern "C" size_t vk_latent_prefill_workspace_size(const vk_pool* pool, int32_t 
     if (!pool || !is_latent(pool) || batch <= 0 || max_seq_len <= 0 || num_heads <= 0) return 0;
     const int64_t rows = static_cast<int64_t>(batch) * ((static_cast<int64_t>(max_seq_len) + kLpKeys - 1) / kLpKeys * kLpKeys);
     if (rows >= (1ll << 31)) return 0;
-    return static_cast<size_t>(rows) * 512 * lp_heads(rows, num_heads);
+    return static_cast<size_t>(rows) * 512 * lp_heads(rows, num_heads) + lp_part_bytes(pool);
 }
 
 extern "C" vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -747,6 +811,8 @@ extern "C" vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void*
     p.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(width))) * 1.4426950408889634f;
     const int64_t rows = static_cast<int64_t>(batch) * p.lpad;
     const int group = lp_heads(rows, num_heads);
+    p.part_o = reinterpret_cast<float*>(p.ws + static_cast<size_t>(rows) * 512 * group);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(pool->num_sms) * 256 * kLpHead);
 
     const CUtensorMapDataType type = pool->kv_format == VK_KV_LATENT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     alignas(64) CUtensorMap tq, tw, tkv;
