@@ -71,13 +71,13 @@ struct LdParams {
     float4* ws_o;    // partial O: ld_part()
     float2* ws_ml;   // [2 * CTAs][64]: maximum (log2 domain), sum
     int2* ws_unit;   // [units]: first and last CTA of a split unit, or (-1, -1)
-    int bt_stride, B, T, H, groups, layer, num_pages, P, latent, rope, nch, stages;
+    int bt_stride, B, T, H, groups, layer, num_pages, P, latent, rope, nch, stages, capacity;
     float scale_log2;
 };
 
 __device__ __forceinline__ int ld_len(const LdParams& p, int b) {
     const int len = __ldg(p.lens + b);
-    return len < 0 || len > static_cast<int64_t>(p.bt_stride) * p.P ? 0 : len;
+    return len < 0 || len > p.capacity ? 0 : len;
 }
 
 // n CTAs share `total`: the first `rem` take q + 1, the others q.  (64-bit
@@ -885,6 +885,8 @@ extern "C" vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* 
     p.layer = layer;
     p.num_pages = pool->num_pages;
     p.P = pool->cfg.page_tokens;
+    const int64_t capacity = static_cast<int64_t>(bt_stride) * p.P;
+    p.capacity = static_cast<int>(capacity < 0x7fffff00 ? capacity : 0x7fffff00);  // (rounded up to tiles in int32)
     p.latent = pool->latent_dim;
     p.rope = pool->rope_dim;
     p.nch = p.latent / 64 + 1;

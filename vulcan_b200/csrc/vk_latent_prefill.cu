@@ -774,8 +774,10 @@ extern "C" vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void*
     if (batch == 0 || tokens == 0) return VK_OK;
     if (!q || !w_kv || !out || !block_tables || !positions) return fail(VK_INVALID_ARG, "NULL array");
     if (!offsets && tokens % batch) return fail(VK_INVALID_ARG, "without offsets, tokens must be a multiple of batch");
-    if (max_tokens <= 0 || max_seq_len < max_tokens) return fail(VK_INVALID_ARG, "max_tokens must be > 0 and max_seq_len >= max_tokens");
-    if (!offsets && max_tokens < tokens / batch) return fail(VK_INVALID_ARG, "max_tokens is smaller than the chunk");
+    if (max_tokens <= 0 || max_seq_len <= 0) return fail(VK_INVALID_ARG, "max_tokens and max_seq_len must be > 0");
+    if (!offsets && (max_tokens < tokens / batch || max_seq_len < tokens / batch))
+        return fail(VK_INVALID_ARG, "max_tokens or max_seq_len is smaller than the chunk");
+    if (max_tokens > max_seq_len) max_tokens = max_seq_len;  // no chunk is longer than its sequence
     if (max_seq_len > static_cast<int64_t>(bt_stride) * pool->cfg.page_tokens)
         return fail(VK_INVALID_ARG, "max_seq_len exceeds the block table capacity");
     if (batch > 65535 || num_heads > 65535) return fail(VK_INVALID_ARG, "batch and num_heads must be <= 65535");

@@ -358,7 +358,11 @@ vk_status vk_latent_pool_create(const vk_latent_cfg* c, void* device_mem, size_t
         }
         if (e != cudaSuccess) s = cuda_fail(e, "cudaMalloc(latent pool)");
     }
-    if (s == VK_OK) s = finish_create(p, out_pool);
+    try {
+        if (s == VK_OK) s = finish_create(p, out_pool);
+    } catch (const std::bad_alloc&) {
+        s = fail(VK_INVALID_ARG, "out of host memory");
+    }
     if (s != VK_OK) {
         if (p->d_err) cudaFree(p->d_err);
         if (p->owns_mem) cudaFree(p->base);

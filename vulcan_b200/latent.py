@@ -58,6 +58,15 @@ def _on(t: torch.Tensor, dtype, name: str, index: int) -> None:
         raise ValueError("%s must be on cuda:%d, got %s" % (name, index, t.device))
 
 
+def _workspace(given, need: int, device: torch.device, index: int, stream) -> Tuple[torch.Tensor, int]:
+    """(the call's scratch, its bytes): the caller's, or memory of its own."""
+    if given is None:
+        return _empty((need,), torch.uint8, device, stream), need
+    if given.get_device() != index or not given.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on cuda:%d" % index)
+    return given, given.numel() * given.element_size()
+
+
 def _i32(t: torch.Tensor, name: str, index: int, numel: int) -> int:
     _on(t, torch.int32, name, index)
     if t.numel() != numel or not t.is_contiguous():
@@ -230,6 +239,8 @@ class LatentKVPool(PagedKVPool):
             _on(norm_weight, self.dtype, "norm_weight", index)
             if norm_weight.numel() != self.latent_dim or not norm_weight.is_contiguous():
                 raise ValueError("norm_weight must be contiguous with %d elements" % self.latent_dim)
+        if rope is not None and not rope.handle.value:
+            raise ValueError("rope is closed")
         check(self._lib.vk_latent_append(
             self.handle, layer, latent.data_ptr(), latent.stride(0), k_rope.data_ptr(), k_rope.stride(0),
             None if norm_weight is None else norm_weight.data_ptr(), eps, None if rope is None else rope.handle,
@@ -269,13 +280,12 @@ class LatentKVPool(PagedKVPool):
                 raise ValueError("lse must be contiguous [B, (T,) H]")
         elif return_lse:
             lse = _empty(shape[:-1], torch.float32, dev, stream)
-        ws = workspace if workspace is not None else _empty((self.decode_workspace_size(batch, tokens, heads),), torch.uint8,
-                                                            dev, stream)
+        ws, ws_bytes = _workspace(workspace, self.decode_workspace_size(batch, tokens, heads), dev, index, stream)
         check(self._lib.vk_latent_decode(
             self.handle, layer, q_latent.data_ptr(), lt, lh, q_rope.data_ptr(), rt, rh, out.data_ptr(),
             None if lse is None else lse.data_ptr(), block_tables.data_ptr(), width,
-            _i32(seq_lens, "seq_lens", index, batch), batch, tokens, heads, scale, ws.data_ptr(),
-            ws.numel() * ws.element_size(), _stream_of(stream, index)), "vk_latent_decode")
+            _i32(seq_lens, "seq_lens", index, batch), batch, tokens, heads, scale, ws.data_ptr(), ws_bytes,
+            _stream_of(stream, index)), "vk_latent_decode")
         return (out, lse) if return_lse else out
 
     def prefill_workspace_size(self, batch: int, max_seq_len: int, num_heads: int) -> int:
@@ -313,13 +323,12 @@ class LatentKVPool(PagedKVPool):
             _on(out, self.dtype, "out", index)
             if out.shape != shape or not out.is_contiguous():
                 raise ValueError("out must be contiguous with shape %s" % (tuple(shape),))
-        ws = workspace if workspace is not None else _empty((self.prefill_workspace_size(batch, max_seq_len, heads),),
-                                                            torch.uint8, dev, stream)
+        ws, ws_bytes = _workspace(workspace, self.prefill_workspace_size(batch, max_seq_len, heads), dev, index, stream)
         check(self._lib.vk_latent_prefill(
             self.handle, layer, q.data_ptr(), qt, qh, w_kv.data_ptr(), w_kv.stride(0), out.data_ptr(),
             block_tables.data_ptr(), width, _i32(positions, "positions", index, batch),
             None if offsets is None else _i32(offsets, "offsets", index, batch + 1), batch, tokens, max_tokens, max_seq_len,
-            heads, scale, ws.data_ptr(), ws.numel() * ws.element_size(), _stream_of(stream, index)), "vk_latent_prefill")
+            heads, scale, ws.data_ptr(), ws_bytes, _stream_of(stream, index)), "vk_latent_prefill")
         return out
 
     def plan(self, *args, **kwargs):
