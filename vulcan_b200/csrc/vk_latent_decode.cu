@@ -17,8 +17,9 @@
 //    rows, 128-byte swizzle) into a ring of as many stages as fit (2 at 512 + 64);
 //  * warp 5 issues  S[64 rows x 64 keys] = Q K^T  (tcgen05.mma, M 64, K-major
 //    both) and warp 6  O^T[latent x 64 rows] += V^T P^T  as M = 128 blocks of
-//    latent elements: an MMA costs its thread 40-60 cycles to issue, more than the
-//    tensor core takes, so two threads issue.  The transposed output keeps all 128 lanes at work with 64
+//    latent elements: an MMA costs its thread ~40 cycles to issue, more than the
+//    tensor core takes, so two threads issue (one lane each: waits and issue by the
+//    whole warp were 6% slower).  The transposed output keeps all 128 lanes at work with 64
 //    rows (O itself would be M = 64 at half the rate) and needs 256 TMEM columns
 //    instead of 512, so S has two buffers beside it: S of tile i+1 is issued
 //    before O of tile i and the tensor core works through the softmax.  V^T is
@@ -366,42 +367,41 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         const uint32_t k_hi = static_cast<uint32_t>(dk0 >> 32), k_lo = static_cast<uint32_t>(dk0);
         const uint32_t q_lo = k_lo + ((s_q - sbase) >> 4);
         const int rsteps = p.rope >> 4;
-        const bool lead = elect_lane();
-        while (ok && w.next_real(p, c)) {
-            ok = wait_all(smem_u32(q_full), piece & 1, p.err);
-            ++piece;
-            for (int t = c.t0; t < c.t1 && ok; ++t, ++si) {
-                if (si >= 2) ok = wait_all(smem_u32(&p_full[si & 1]), ((si >> 1) - 1) & 1, p.err);  // S's buffer has been read
-                const uint32_t kl = k_lo + st * (stage_bytes >> 4);
-                const uint32_t d = tmem + 256 + (si & 1) * 64;
+        if (elect_lane()) {
+            while (ok && w.next_real(p, c)) {
+                ok = mbar_wait(smem_u32(q_full), piece & 1, p.err);
+                ++piece;
+                for (int t = c.t0; t < c.t1 && ok; ++t, ++si) {
+                    if (si >= 2) ok = mbar_wait(smem_u32(&p_full[si & 1]), ((si >> 1) - 1) & 1, p.err);  // S's buffer has been read
+                    const uint32_t kl = k_lo + st * (stage_bytes >> 4);
+                    const uint32_t d = tmem + 256 + (si & 1) * 64;
 #pragma unroll
-                for (int g = 0; g < LCH / 2; ++g) {
-                    ok = ok && wait_all(smem_u32(&k_full[st * kLdParts + g]), ph, p.err);
-                    if (ok && lead) {
-                        tc_fence_after();
+                    for (int g = 0; g < LCH / 2; ++g) {
+                        ok = ok && mbar_wait(smem_u32(&k_full[st * kLdParts + g]), ph, p.err);
+                        if (ok) {
+                            tc_fence_after();
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const uint32_t off = ((2 * g + (k >> 2)) * kLdChunk + (k & 3) * 32) >> 4;
-                            umma_ss_lo(d, q_lo + off, k_hi, kl + off, k_hi, id_s, (g | k) != 0);
+                            for (int k = 0; k < 8; ++k) {
+                                const uint32_t off = ((2 * g + (k >> 2)) * kLdChunk + (k & 3) * 32) >> 4;
+                                umma_ss_lo(d, q_lo + off, k_hi, kl + off, k_hi, id_s, (g | k) != 0);
+                            }
                         }
                     }
-                    __syncwarp();
-                }
-                ok = ok && wait_all(smem_u32(&k_full[st * kLdParts + LCH / 2]), ph, p.err);
-                if (ok && lead) {
-                    tc_fence_after();
+                    ok = ok && mbar_wait(smem_u32(&k_full[st * kLdParts + LCH / 2]), ph, p.err);
+                    if (ok) {
+                        tc_fence_after();
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        const uint32_t off = (LCH * kLdChunk + ks * 32) >> 4;
-                        if (ks < rsteps) umma_ss_lo(d, q_lo + off, k_hi, kl + off, k_hi, id_s, 1);
+                        for (int ks = 0; ks < 4; ++ks) {
+                            const uint32_t off = (LCH * kLdChunk + ks * 32) >> 4;
+                            if (ks < rsteps) umma_ss_lo(d, q_lo + off, k_hi, kl + off, k_hi, id_s, 1);
+                        }
+                        umma_commit(smem_u32(&s_full[si & 1]));
+                        umma_commit(smem_u32(&k_empty[st * kLdParts + LCH / 2]));
                     }
-                    umma_commit(smem_u32(&s_full[si & 1]));
-                    umma_commit(smem_u32(&k_empty[st * kLdParts + LCH / 2]));
-                }
-                __syncwarp();
-                if (++st == p.stages) {
-                    st = 0;
-                    ph ^= 1;
+                    if (++st == p.stages) {
+                        st = 0;
+                        ph ^= 1;
+                    }
                 }
             }
         }
@@ -413,31 +413,31 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
         const uint64_t dv0 = umma_desc_sw128(sbase, kLdChunk, 1024), dp0 = umma_desc_sw128(s_p, 16, 1024);
         const uint32_t v_hi = static_cast<uint32_t>(dv0 >> 32), v_lo = static_cast<uint32_t>(dv0);
         const uint32_t p_hi = static_cast<uint32_t>(dp0 >> 32), p_lo = static_cast<uint32_t>(dp0);
-        const bool lead = elect_lane();
-        while (ok && w.next_real(p, c)) {
-            for (int t = c.t0; t < c.t1 && ok; ++t, ++pi) {
+        if (elect_lane()) {
+            while (ok && w.next_real(p, c)) {
+                for (int t = c.t0; t < c.t1 && ok; ++t, ++pi) {
 #pragma unroll
-                for (int g = 0; g < LCH / 2; ++g)  // long complete: S has read them
-                    ok = ok && wait_all(smem_u32(&k_full[st * kLdParts + g]), ph, p.err);
-                ok = ok && wait_all(smem_u32(&p_full[pi & 1]), (pi >> 1) & 1, p.err);
-                if (ok && lead) {
-                    tc_fence_after();
-                    const uint32_t vl = v_lo + st * (stage_bytes >> 4);
-                    const uint32_t acc = t != c.t0;
+                    for (int g = 0; g < LCH / 2; ++g)  // long complete: S has read them
+                        ok = ok && mbar_wait(smem_u32(&k_full[st * kLdParts + g]), ph, p.err);
+                    ok = ok && mbar_wait(smem_u32(&p_full[pi & 1]), (pi >> 1) & 1, p.err);
+                    if (ok) {
+                        tc_fence_after();
+                        const uint32_t vl = v_lo + st * (stage_bytes >> 4);
+                        const uint32_t acc = t != c.t0;
 #pragma unroll
-                    for (int mb = 0; mb < LCH / 2; ++mb) {
+                        for (int mb = 0; mb < LCH / 2; ++mb) {
 #pragma unroll
-                        for (int ks = 0; ks < kLdKeys / 16; ++ks)
-                            umma_ss_lo(tmem + mb * 64, vl + ((mb * 2 * kLdChunk + ks * 2048) >> 4), v_hi, p_lo + ks * 2, p_hi, id_pv,
-                                       ks ? 1 : acc);
-                        umma_commit(smem_u32(&k_empty[st * kLdParts + mb]));
+                            for (int ks = 0; ks < kLdKeys / 16; ++ks)
+                                umma_ss_lo(tmem + mb * 64, vl + ((mb * 2 * kLdChunk + ks * 2048) >> 4), v_hi, p_lo + ks * 2, p_hi, id_pv,
+                                           ks ? 1 : acc);
+                            umma_commit(smem_u32(&k_empty[st * kLdParts + mb]));
+                        }
+                        umma_commit(smem_u32(pv_done));
                     }
-                    umma_commit(smem_u32(pv_done));
-                }
-                __syncwarp();
-                if (++st == p.stages) {
-                    st = 0;
-                    ph ^= 1;
+                    if (++st == p.stages) {
+                        st = 0;
+                        ph ^= 1;
+                    }
                 }
             }
         }

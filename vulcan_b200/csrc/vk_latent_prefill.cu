@@ -200,19 +200,18 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
         // took 980 cycles a stage, 512 of them MMAs).
         constexpr uint32_t id = idesc_16(Elem<T>::kBf16, 128, 128, 0, 0);
         const int tile = warp == 9 ? 0 : 1;
-        if (tile == 0 || two) {
-            const bool lead = elect_lane();
+        if ((tile == 0 || two) && elect_lane()) {
             const uint64_t d0 = umma_desc_sw128(sbase, 16, 1024);
             const uint32_t hi = static_cast<uint32_t>(d0 >> 32), a_lo = static_cast<uint32_t>(d0), b_lo = a_lo + ((s_b - sbase) >> 4);
             const uint32_t d = tmem + 256 + tile * 128;
             int st = 0, ph = 0;
-            bool ok = wait_all(tile ? smem_u32(a_moved) : smem_u32(&a_full[1]), 0, p.err);
+            bool ok = mbar_wait(tile ? smem_u32(a_moved) : smem_u32(&a_full[1]), 0, p.err);
             tc_fence_after();
             for (int hh = 0; hh < 2 * nh && ok; ++hh) {  // K half, V half of each head
-                if (hh > 0) ok = wait_all(smem_u32(&acc_empty[tile]), (hh - 1) & 1, p.err);
+                if (hh > 0) ok = mbar_wait(smem_u32(&acc_empty[tile]), (hh - 1) & 1, p.err);
                 for (int c = 0; c < lch && ok; ++c) {
-                    ok = wait_all(smem_u32(&b_full[st]), ph, p.err);
-                    if (ok && lead) {
+                    ok = mbar_wait(smem_u32(&b_full[st]), ph, p.err);
+                    if (ok) {
                         tc_fence_after();
                         const uint32_t bl = b_lo + st * (kLeStage >> 4);
                         if (tile) {
@@ -226,7 +225,6 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
                         umma_commit(smem_u32(&b_empty[st]));
                         if (c == lch - 1) umma_commit(smem_u32(&acc_full[tile]));
                     }
-                    __syncwarp();
                     if (++st == p.stages) {
                         st = 0;
                         ph ^= 1;
@@ -454,78 +452,76 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
         // S_A0, S_B0, PV_A0, S_A1, PV_B0, S_B1, ...: one thread, so its MMAs execute in
         // order, P is read before the next S overwrites it, and each step's products
         // are done as early as they can be (a second issuing warp, one per row tile,
-        // made the steps interleave and was 16% slower).  The warp waits as a whole and
-        // one lane issues, in unrolled runs on 32-bit descriptor words: ~40 cycles an
-        // MMA (60 on 64-bit descriptors from a lone lane).
+        // made the steps interleave and was 16% slower).  Unrolled runs on 32-bit
+        // descriptor words: ~40 cycles an MMA (60 on 64-bit ones).
         constexpr uint32_t id_s = idesc_16(Elem<T>::kBf16, 128, 128, 0, 0);
         constexpr uint32_t id_pv = idesc_16(Elem<T>::kBf16, 128, 128, 0, 1), id_half = idesc_16(Elem<T>::kBf16, 128, 64, 0, 1);
-        const bool lead = elect_lane();
-        bool ok = wait_all(smem_u32(q_full), 0, p.err);
-        int k_waited = -1, v_waited = -1;
-        const int rsteps = p.rope >> 4;
-        const uint64_t dk0 = umma_desc_sw128(sbase + kLaRing, 16, 1024), dv0 = umma_desc_sw128(sbase + kLaRing, kLpUnit, 1024);
-        const uint32_t k_hi = static_cast<uint32_t>(dk0 >> 32), k_lo = static_cast<uint32_t>(dk0);
-        const uint32_t v_hi = static_cast<uint32_t>(dv0 >> 32), v_lo = static_cast<uint32_t>(dv0);
-        const uint32_t q_lo = k_lo - (kLaRing >> 4);
-        constexpr uint32_t kUnit16 = kLpUnit >> 4;
-        auto issue_s = [&](int t, int j) {
-            if (j > k_waited) {
-                ok = ok && wait_all(smem_u32(&k_full[j & 1]), (j >> 1) & 1, p.err);
-                k_waited = j;
-            }
-            if (ok && lead) {
-                tc_fence_after();
-                const uint32_t ql = q_lo + t * 3 * kUnit16, d = tmem + t * 128;
-#pragma unroll
-                for (int u = 0; u < 3; ++u) {
-                    const uint32_t kl = k_lo + ((5 * j + u) & 7) * kUnit16;
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)
-                        if (u < 2 || ks < rsteps) umma_ss_lo(d, ql + u * kUnit16 + ks * 2, k_hi, kl + ks * 2, k_hi, id_s, (u | ks) != 0);
+        if (elect_lane()) {
+            bool ok = mbar_wait(smem_u32(q_full), 0, p.err);
+            int k_waited = -1, v_waited = -1;
+            const int rsteps = p.rope >> 4;
+            const uint64_t dk0 = umma_desc_sw128(sbase + kLaRing, 16, 1024), dv0 = umma_desc_sw128(sbase + kLaRing, kLpUnit, 1024);
+            const uint32_t k_hi = static_cast<uint32_t>(dk0 >> 32), k_lo = static_cast<uint32_t>(dk0);
+            const uint32_t v_hi = static_cast<uint32_t>(dv0 >> 32), v_lo = static_cast<uint32_t>(dv0);
+            const uint32_t q_lo = k_lo - (kLaRing >> 4);
+            constexpr uint32_t kUnit16 = kLpUnit >> 4;
+            auto issue_s = [&](int t, int j) {
+                if (j > k_waited) {
+                    ok = ok && mbar_wait(smem_u32(&k_full[j & 1]), (j >> 1) & 1, p.err);
+                    k_waited = j;
                 }
-                umma_commit(smem_u32(&s_full[t]));
-                if (t == 1 || j >= ntB) umma_commit(smem_u32(&k_empty[j & 1]));
-            }
-            __syncwarp();
-        };
-        auto issue_pv = [&](int t, int j) {
-            if (j > v_waited) {
-                ok = ok && wait_all(smem_u32(&v_full[j & 1]), (j >> 1) & 1, p.err);
-                v_waited = j;
-            }
-            ok = ok && wait_all(smem_u32(&p_full[t]), j & 1, p.err);
-            if (ok && lead) {
-                tc_fence_after();
-                const uint32_t d = tmem + 256 + t * 128, a = tmem + t * 128, acc = j > 0;
-                const int slot = (5 * j + 3) & 7;
-                if (slot < 7) {  // both 64-column units side by side: one MMA spans them
-                    const uint32_t vl = v_lo + slot * kUnit16;
+                if (ok) {
+                    tc_fence_after();
+                    const uint32_t ql = q_lo + t * 3 * kUnit16, d = tmem + t * 128;
 #pragma unroll
-                    for (int ks = 0; ks < kLpKeys / 16; ++ks) umma_ts_lo(d, a + ks * 8, vl + ks * 128, v_hi, id_pv, ks ? 1 : acc);
-                } else {
-#pragma unroll 1
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t vl = v_lo + ((slot + u) & 7) * kUnit16;
+                    for (int u = 0; u < 3; ++u) {
+                        const uint32_t kl = k_lo + ((5 * j + u) & 7) * kUnit16;
 #pragma unroll
-                        for (int ks = 0; ks < kLpKeys / 16; ++ks)
-                            umma_ts_lo(d + u * 64, a + ks * 8, vl + ks * 128, v_hi, id_half, ks ? 1 : acc);
+                        for (int ks = 0; ks < 4; ++ks)
+                            if (u < 2 || ks < rsteps) umma_ss_lo(d, ql + u * kUnit16 + ks * 2, k_hi, kl + ks * 2, k_hi, id_s, (u | ks) != 0);
                     }
+                    umma_commit(smem_u32(&s_full[t]));
+                    if (t == 1 || j >= ntB) umma_commit(smem_u32(&k_empty[j & 1]));
                 }
-                umma_commit(smem_u32(&o_full[t]));
-                if (t == 1 || j >= ntB) umma_commit(smem_u32(&v_empty[j & 1]));
-            }
-            __syncwarp();
-        };
-        if (ntA > 0) issue_s(0, 0);
-        if (ntB > 0) issue_s(1, 0);
-        for (int j = 0; j < ntiles && ok; ++j) {
-            if (j < ntA) {
-                issue_pv(0, j);
-                if (j + 1 < ntA) issue_s(0, j + 1);
-            }
-            if (j < ntB) {
-                issue_pv(1, j);
-                if (j + 1 < ntB) issue_s(1, j + 1);
+            };
+            auto issue_pv = [&](int t, int j) {
+                if (j > v_waited) {
+                    ok = ok && mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, p.err);
+                    v_waited = j;
+                }
+                ok = ok && mbar_wait(smem_u32(&p_full[t]), j & 1, p.err);
+                if (ok) {
+                    tc_fence_after();
+                    const uint32_t d = tmem + 256 + t * 128, a = tmem + t * 128, acc = j > 0;
+                    const int slot = (5 * j + 3) & 7;
+                    if (slot < 7) {  // both 64-column units side by side: one MMA spans them
+                        const uint32_t vl = v_lo + slot * kUnit16;
+#pragma unroll
+                        for (int ks = 0; ks < kLpKeys / 16; ++ks) umma_ts_lo(d, a + ks * 8, vl + ks * 128, v_hi, id_pv, ks ? 1 : acc);
+                    } else {
+#pragma unroll 1
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t vl = v_lo + ((slot + u) & 7) * kUnit16;
+#pragma unroll
+                            for (int ks = 0; ks < kLpKeys / 16; ++ks)
+                                umma_ts_lo(d + u * 64, a + ks * 8, vl + ks * 128, v_hi, id_half, ks ? 1 : acc);
+                        }
+                    }
+                    umma_commit(smem_u32(&o_full[t]));
+                    if (t == 1 || j >= ntB) umma_commit(smem_u32(&v_empty[j & 1]));
+                }
+            };
+            if (ntA > 0) issue_s(0, 0);
+            if (ntB > 0) issue_s(1, 0);
+            for (int j = 0; j < ntiles && ok; ++j) {
+                if (j < ntA) {
+                    issue_pv(0, j);
+                    if (j + 1 < ntA) issue_s(0, j + 1);
+                }
+                if (j < ntB) {
+                    issue_pv(1, j);
+                    if (j + 1 < ntB) issue_s(1, j + 1);
+                }
             }
         }
     } else {
