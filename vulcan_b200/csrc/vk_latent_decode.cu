@@ -358,6 +358,13 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                 }
             }
         }
+        if (!ok)  // a wait gave up: no copy of this warp may land behind the CTA's end (bounded as well)
+            for (int k = 0; k < p.stages; ++k)
+                if (k < st || filled) {
+                    const uint32_t par = k < st ? ph ^ 1 : ph;
+                    mbar_wait(smem_u32(&k_full[k * kLdParts + g]), par, p.err);
+                    if (g == 0) mbar_wait(smem_u32(&k_full[k * kLdParts + LCH / 2]), par, p.err);
+                }
     } else if (warp == 5) {
         // ------------------------------------------------------------ S = Q K^T
         int si = 0, piece = 0, st = 0, ph = 0;

@@ -191,8 +191,14 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
         __syncwarp();
         if (two) ok = wait_all(smem_u32(a_moved), 0, p.err);
         if (ok) load_a(0);
-        if (lane == 0)
+        if (lane == 0) {
             while (it < total && ok) load_b(true);
+            if (!ok) {  // a wait gave up: no copy of this warp may land behind the CTA's end (bounded as well)
+                if (two) mbar_wait(smem_u32(&a_full[0]), 0, p.err);
+                for (int k = max(me, it - p.stages); k < it; ++k)
+                    if ((k - me) % kLeLoaders == 0) mbar_wait(smem_u32(&b_full[k % p.stages]), (k / p.stages) & 1, p.err);
+            }
+        }
     } else if (warp == 9 || warp == 11) {
         // MMA issuers, one per row tile: an issuing thread is held until its last MMA is
         // dispatched and then needs ~200 cycles to see the next stage's barrier, most of
@@ -404,6 +410,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
         if (lane == 0) {
             const uint64_t pol = l2_evict_last_policy();  // other row tiles read the same K and V
             const int wrow = b * p.lpad + kt0 * kLpKeys, u = warp == 8 ? 0 : 1;
+            int landed = -1;  // the last tile whose K and V are on their way
             bool ok = true;
             asm volatile("griddepcontrol.wait;" ::: "memory");
             for (int j = 0; j < ntiles; ++j) {
@@ -418,7 +425,13 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
                 mbar_expect_tx(vbar, kLpUnit);
                 tma_load_2d(sbase + kLaRing + ((5 * j + 3 + u) & 7) * kLpUnit, &tmapkv, hl * 256 + kLpHead + u * 64,
                             wrow + j * kLpKeys, vbar, pol);
+                landed = j;
             }
+            if (!ok)  // a wait gave up: no copy of this warp may land behind the CTA's end (bounded as well)
+                for (int j = max(0, landed - 1); j <= min(landed + 1, ntiles - 1); ++j) {
+                    mbar_wait(smem_u32(&k_full[j & 1]), (j >> 1) & 1, p.err);
+                    if (j <= landed) mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, p.err);
+                }
         }
     } else if (warp == 11) {
         // ------------------------------------------------------------ TMA: rotary parts from the pages
