@@ -7,10 +7,12 @@
 // Floor: 2 * (latent + rope) * 2 bytes a token.  One warp per token: the row stays in
 // registers between the sum of squares (fp32, one shuffle tree) and the scaled
 // store, so it is read once and written once, the latent in 16-byte vectors.
-// Bound by latency: 2.8 us for a decode step; 17.6k tokens of 512 + 64 take 13.6 us,
-// 3.0 TB/s (the memory alone 6.3): ~20% of the time is the launch, the rest four
-// dependent loads a warp at 44 registers (two and four rows a warp measured 14.0 and
-// 14.6 us, blocks of two and eight warps 14.0 and 14.7).
+// Bound by latency: 2.6 us for a decode step; 17.6k tokens of 512 + 64 take 11.3 us,
+// 3.6 TB/s (the memory alone 6.3): ~20% of the time is the launch, the rest three
+// dependent loads a warp (sequence and position, page; the row meanwhile).  At 32
+// registers (one spilled) all 64 warps fit an SM: 11.3 us against 11.8 at 44.  Blocks of
+// 8 and 16 warps measured 12.0 and 12.2 us, two and four rows a warp 14.0 and 14.6
+// where one took 13.6.
 #include "vk_internal.h"
 #include "vk_rotary.cuh"
 
@@ -35,27 +37,36 @@ constexpr int kLaWarps = 4;
 // The sequence of a row, the last b with offsets[b] <= row, and that offset, by a
 // 32-ary search of the warp (one round of loads for up to 32 sequences); -1 behind
 // the last sequence.
-__device__ __forceinline__ int sequence_of(const int32_t* offsets, int B, int row, int lane, int* first) {
+__device__ __forceinline__ int sequence_of(const int32_t* offsets, const int32_t* positions, int B, int row, int lane, int* first,
+                                           int* position) {
     const int end = __ldg(offsets + B);
-    int lo = 0, n = B, at = 0;
+    int lo = 0, n = B, at = 0, pos = 0;
     do {
         const int step = (n + 31) >> 5;
         const int v = lane * step < n ? __ldg(offsets + lo + lane * step) : 0;
+        const int pv = lane * step < n ? __ldg(positions + lo + lane * step) : 0;  // beside it: one load less in the chain
         const unsigned le = __ballot_sync(0xffffffffu, lane * step < n && v <= row);
         const int k = le ? 31 - __clz(le) : 0;
         at = __shfl_sync(0xffffffffu, v, k);
+        pos = __shfl_sync(0xffffffffu, pv, k);
         lo += k * step;
         n = min(step, n - k * step);
     } while (n > 1);
     *first = at;
+    *position = pos;
     return row < end ? lo : -1;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLaWarps * 32) latent_append_kernel(const __grid_constant__ RotaryTable rot,
-                                                                      const __grid_constant__ LatentAppendParams p) {
+__global__ void __launch_bounds__(kLaWarps * 32, 64 / kLaWarps) latent_append_kernel(
+    const __grid_constant__ RotaryTable rot, const __grid_constant__ LatentAppendParams p) {
     const int64_t row = static_cast<int64_t>(blockIdx.x) * kLaWarps + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
+    // the turns of the pairs, read from the kernel's parameters once a block: a warp's 32
+    // addresses in the constant cache are served one after another (a read per warp: 13.0 us)
+    __shared__ uint64_t turn[32];
+    if (threadIdx.x < rot.pairs) turn[threadIdx.x] = rot.turn[threadIdx.x];
+    __syncthreads();
     if (row >= p.tokens) return;
     // the row's loads go out first; the lookups (three dependent loads: sequence,
     // position, page) run behind them
@@ -81,16 +92,17 @@ __global__ void __launch_bounds__(kLaWarps * 32) latent_append_kernel(const __gr
         else
             k = __ldg(reinterpret_cast<const uint32_t*>(ksrc) + lane);
     }
-    int b, first;
+    int b, first, start;
     if (p.offsets) {
-        b = sequence_of(p.offsets, p.B, static_cast<int>(row), lane, &first);
+        b = sequence_of(p.offsets, p.pos, p.B, static_cast<int>(row), lane, &first, &start);
         if (b < 0) return;
     } else {
         const int per = p.tokens / p.B;
         b = static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(per));
         first = b * per;
+        start = __ldg(p.pos + b);
     }
-    const int64_t pos = static_cast<int64_t>(__ldg(p.pos + b)) + (row - first);
+    const int64_t pos = static_cast<int64_t>(start) + (row - first);
     if (row < first || pos < 0 || (pos >> p.P_log2) >= p.bt_stride) {
         if (lane == 0) atomicOr(p.err, VK_ERR_TABLE_INDEX);
         return;
@@ -128,7 +140,7 @@ __global__ void __launch_bounds__(kLaWarps * 32) latent_append_kernel(const __gr
     if (lane < pairs) {
         if (rot.pairs) {
             const float2 x = Elem<T>::unpack(k);
-            const float2 r = rotary_turn(x.x, x.y, rotary_cos_sin(rot, lane, static_cast<int>(pos)));
+            const float2 r = rotary_turn(x.x, x.y, rotary_cos_sin(turn[lane], rot.magnitude, static_cast<int>(pos)));
             k = Elem<T>::pack(r.x, r.y);
         }
         char* kdst = reinterpret_cast<char*>(dst + vecs);

@@ -27,12 +27,16 @@ struct RotaryTable {
     int half;                        // 0: pairs (2i, 2i+1); 1: pairs (i, i + rotary_dim/2)
 };
 
-__device__ __forceinline__ float2 rotary_cos_sin(const RotaryTable& t, int pair, int pos) {
-    const uint64_t phase = static_cast<uint64_t>(static_cast<int64_t>(pos)) * t.turn[pair];
+__device__ __forceinline__ float2 rotary_cos_sin(uint64_t turn, float magnitude, int pos) {
+    const uint64_t phase = static_cast<uint64_t>(static_cast<int64_t>(pos)) * turn;
     const float turns2 = static_cast<float>(static_cast<int32_t>(phase >> 32)) * 0x1p-31f;  // 2 * turns, in [-1, 1]
     float s, c;
     sincospif(turns2, &s, &c);
-    return make_float2(c * t.magnitude, s * t.magnitude);
+    return make_float2(c * magnitude, s * magnitude);
+}
+
+__device__ __forceinline__ float2 rotary_cos_sin(const RotaryTable& t, int pair, int pos) {
+    return rotary_cos_sin(t.turn[pair], t.magnitude, pos);
 }
 
 __device__ __forceinline__ float2 rotary_turn(float a, float b, float2 cs) {
