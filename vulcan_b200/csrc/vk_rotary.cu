@@ -6,6 +6,11 @@
 //
 // with (a_i, b_i) = (2i, 2i+1) or (i, i + rotary_dim/2), angle = pos * f_i, cos
 // and sin times the magnitude; computed in fp32, rounded once to the type.
+//
+// Floor: 4 bytes an element of a 16-bit tensor.  16,384 tokens of 32 + 32 heads of 128
+// take 92 us, 0.90 of the measured copy rate (101 in a long run); blocks of 128 threads,
+// one vector (a pair of vectors in the half layout) a thread, were the fastest of 64 to
+// 512 threads and 1 to 4 vectors.  64 tokens: 2.5 us, the launch.
 #include <algorithm>
 #include <cmath>
 #include <new>
