@@ -97,6 +97,29 @@ def test_rotary_apply_refusals(lib):
     lib.vk_rotary_destroy(out)
 
 
+def test_rotary_outputs_that_share_elements(lib):
+    out = ctypes.c_void_p()
+    cfg = _rotary_cfg()
+    assert lib.vk_rotary_create(ctypes.byref(cfg), ctypes.byref(out)) == _lib.VK_OK
+
+    def apply(yt, yh, heads=2, tokens=3, in_place=False):
+        v = _lib.VkRotaryView(FAKE, FAKE if in_place else FAKE + (1 << 20), yt if in_place else 128, yh if in_place else 64, yt, yh,
+                              heads)
+        # without positions a call whose strides pass is refused for that instead
+        status = lib.vk_rotary_apply(out, 0, v, None, 64, None, tokens, None)
+        assert status == _lib.VK_INVALID_ARG
+        return b"share" in lib.vk_last_error_string()
+
+    for in_place in (False, True):
+        for yt, yh in ((128, 0), (0, 64), (0, 0), (64, 64), (127, 64), (96, 64), (128, 63), (63, 256), (64, 191)):
+            assert apply(yt, yh, in_place=in_place), (yt, yh)
+        for yt, yh in ((128, 64), (1024, 72), (64, 192), (72, 300), (-128, 64), (128, -64)):
+            assert not apply(yt, yh, in_place=in_place), (yt, yh)
+    assert not apply(0, 64, tokens=1) and not apply(64, 0, heads=1)
+    assert apply(0, 0, tokens=1) and apply(0, 0, heads=1)
+    lib.vk_rotary_destroy(out)
+
+
 @pytest.mark.parametrize("rotary_dim", [2, 64, 128, 256])
 def test_frequencies_plain_and_linear(lib, rotary_dim):
     f, m = _frequencies(lib, _rotary_cfg(rotary_dim))

@@ -169,6 +169,16 @@ static vk_status rotary_frequencies(const vk_rotary_cfg& c, double* f, double* m
     return VK_OK;
 }
 
+// Whether two (token, head) rows of n elements may lie on one another: rows of either
+// index apart by n or more, and those of one index within one step of the other.
+static bool rotary_shares(int64_t token, int64_t tokens, int64_t head, int64_t heads, int64_t n) {
+    token = token < 0 ? -token : token;
+    head = head < 0 ? -head : head;
+    if (tokens <= 1) return heads > 1 && head < n;
+    if (heads <= 1) return token < n;
+    return head < n || token < n || ((token - n) / head < heads - 1 && (head - n) / token < tokens - 1);
+}
+
 static vk_status check_rotary_cfg(const vk_rotary_cfg* c) {
     if (!c) return fail(VK_INVALID_ARG, "rotary: cfg is NULL");
     if (c->rotary_dim <= 0 || (c->rotary_dim & 1) || c->rotary_dim > 2 * kRotaryMaxPairs)
@@ -246,6 +256,8 @@ extern "C" vk_status vk_rotary_apply(const vk_rotary* r, int32_t dtype, const vk
             return fail(VK_INVALID_ARG, "x and y must be aligned to their elements");
         if (v->x == v->y && (v->x_token != v->y_token || v->x_head != v->y_head))
             return fail(VK_INVALID_ARG, "in place needs equal strides of x and y");
+        if (rotary_shares(v->y_token, tokens, v->y_head, v->heads, head_dim))
+            return fail(VK_INVALID_ARG, "the heads and tokens of y may not share elements");
         vec = vec && !((reinterpret_cast<uintptr_t>(v->x) | reinterpret_cast<uintptr_t>(v->y)) & 15) && v->x_token % n == 0 &&
               v->x_head % n == 0 && v->y_token % n == 0 && v->y_head % n == 0;
         copies = copies || v->x != v->y;
