@@ -415,6 +415,48 @@ def test_prefill_cut_along_keys(vk, new, prefix, heads, batch):
     prefill_check(c, g, [new, max(1, new // 2)][:batch], heads, scale=0.05)
 
 
+def test_prefill_graph_and_streams(vk):
+    """Append and prefill captured together replay with other chunks; calls on several streams run side by side."""
+    g = gen(41)
+    c = Cache(vk, [400, 700, 90], seed=3)
+    total, heads = 330, 4
+    q, w = rnd(g, total, heads, 192), rnd(g, heads * 256, 512, std=512 ** -0.5)
+    lat, kr = rnd(g, total, 512), rnd(g, total, 64)
+    pos, offsets = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+
+    def chunk(new):
+        offsets.copy_(torch.tensor([0, new[0], new[0] + new[1], sum(new)], dtype=torch.int32))
+        pos.copy_(c.seq_lens - torch.tensor(new, dtype=torch.int32, device="cuda"))
+
+    def run(out, stream=None):
+        c.pool.append(1, lat, kr, c.tables, pos, offsets=offsets, stream=stream)
+        return c.pool.prefill(1, q, w, c.tables, pos, offsets=offsets, max_tokens=200, max_seq_len=704, out=out, stream=stream)
+
+    out = torch.empty(total, heads, 128, device="cuda").half()
+    chunk([10, 20, 30])
+    run(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(out)
+    for new in ([100, 200, 30], [1, 0, 90], [0, 0, 0], [17, 129, 1]):
+        chunk(new)
+        want = run(torch.full_like(out, 4))
+        out.fill_(4)
+        graph.replay()
+        assert c.check() == 0
+        assert torch.equal(out, want), new
+        assert (out[sum(new):] == 4).all()
+    chunk([100, 200, 30])
+    want = run(torch.empty_like(out))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = [c.pool.prefill(1, q, w, c.tables, pos, offsets=offsets, max_tokens=200, max_seq_len=704, stream=s)
+           for _ in range(3) for s in streams]
+    torch.cuda.synchronize()
+    assert c.check() == 0
+    assert all(torch.equal(x, want) for x in got)
+
+
 def test_prefill_head_groups(vk):
     """A bound on the lengths that makes the workspace hold a part of the heads at a time."""
     g = gen(23)
