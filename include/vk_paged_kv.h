@@ -502,7 +502,9 @@ vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* q_latent, i
  * w_kv: [num_heads * 256, latent_dim], row stride w_stride, per head the 128
  * rows of W_k,h, then the 128 of W_v,h (an [out, in] projection weight as it
  * is); out: [tokens, num_heads, 128].  All of the pool's type, 16-byte aligned,
- * strides multiples of 8.
+ * strides multiples of 8.  Keys and values are rounded to the pool's type (beyond
+ * its range: to its largest number); a NaN or infinite latent reaches the rows that
+ * see it, as NaN, and no others.
  * max_tokens and max_seq_len bound the longest chunk and the longest sequence
  * after it, on the host (they size the launches and the workspace); a sequence
  * beyond them, or beyond its table, records VK_ERR_SEQ_LEN and is left out.

@@ -482,6 +482,23 @@ def test_prefill_non_finite_latents(vk):
         assert torch.isnan(got[70:]).all()
 
 
+def test_prefill_values_beyond_the_type(vk):
+    """A finite latent whose value overflows fp16 leaves the rows that may not see it as they were."""
+    g = gen(25)
+    c = Cache(vk, [100], layers=1, layer=0)
+    q, w = rnd(g, 100, 2, 192), rnd(g, 512, 512, std=512 ** -0.5)
+    pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+    want = c.pool.prefill(0, q, w, c.tables, pos)
+    row = 6000 * torch.sign(w[128])  # the first value element of head 0
+    assert float((row.double() * w[128].double()).sum()) > 70000
+    assert float((w[:128].double() @ row.double()).abs().max()) < 60000
+    c.pool.latent_view()[0, int(c.tables[0, 70 // 16]), 70 % 16, :512] = row
+    got = c.pool.prefill(0, q, w, c.tables, pos)
+    assert c.check() == 0
+    assert torch.equal(got[:70], want[:70])
+    assert torch.isfinite(got).all()
+
+
 def test_prefill_records_what_is_out_of_bounds(vk):
     """Sequences beyond the given bounds are recorded and left out; the others are computed."""
     g = gen(25)

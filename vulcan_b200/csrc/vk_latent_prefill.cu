@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
         const bool inside = key0 + tile * kLpKeys + r < len;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t stage = s_out + tile * kLeStage;
-        constexpr uint32_t kExp = Elem<T>::kBf16 ? 0x7f807f80u : 0x7c007c00u;
+        constexpr uint32_t kExp = 0x7f800000u;
         bool ok = true;
         if (tile) {  // row tile 1's latent rows, shared memory -> TMEM (two elements a column)
             ok = wait_all(smem_u32(&a_full[0]), 0, p.err);
@@ -289,22 +289,24 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
                 tmem_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    w[c * 32 + i] = inside ? Elem<T>::pack(v[i >> 4][2 * (i & 15)], v[i >> 4][2 * (i & 15) + 1]) : 0u;
-                    all &= w[c * 32 + i];
+                    const float x = v[i >> 4][2 * (i & 15)], y = v[i >> 4][2 * (i & 15) + 1];
+                    w[c * 32 + i] = inside ? Elem<T>::pack_sat(x, y) : 0u;
+                    all &= __float_as_uint(x) & __float_as_uint(y);
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&acc_empty[tile]));
-            // A key whose every element is NaN or infinite comes from such a latent; rows
-            // that may not see it multiply its value by a weight of zero, so the value's
-            // non-finite elements are stored as zeros (a row that sees the key gets its
-            // NaN through S).
-            if ((hh & 1) == 0) {
-                bad = (all & kExp) == kExp;
-            } else if (bad) {
+            // A key whose every element is NaN or infinite comes from such a latent.  Rows
+            // that may not see it multiply its value by a weight of zero, so the value is
+            // stored as zeros and the key as NaN: a row that sees it gets its NaN through
+            // S.  (For the same reason a finite value beyond the type's range is stored as
+            // the largest number, not as infinity.)
+            if ((hh & 1) == 0) bad = inside && (all & kExp) == kExp;
+            if (bad) {
+                const uint32_t fill = hh & 1 ? 0u : 0x7fff7fffu;
 #pragma unroll
-                for (int i = 0; i < 64; ++i) w[i] = finite_word<T>(w[i]);
+                for (int i = 0; i < 64; ++i) w[i] = fill;
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {  // 64 columns at a time through this tile's 16 KiB

@@ -57,6 +57,12 @@ struct Elem<__half> {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
+    // beyond the type's range: its largest number
+    static __device__ __forceinline__ uint32_t pack_sat(float a, float b) {
+        uint32_t w;
+        asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+        return w;
+    }
     static __device__ __forceinline__ float2 unpack(uint32_t w) {
         return __half22float2(*reinterpret_cast<const __half2*>(&w));
     }
@@ -70,6 +76,11 @@ struct Elem<__nv_bfloat16> {
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ uint32_t pack_sat(float a, float b) {
+        uint32_t w;
+        asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+        return w;
     }
     static __device__ __forceinline__ float2 unpack(uint32_t w) {
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
