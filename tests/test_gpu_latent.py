@@ -712,3 +712,53 @@ def test_a_layer_serves(vk, dtype):
         # far inside the bound on average: a wrong row or mask would not be
         assert float(err.norm() / want[:, now].norm()) < 8 * e
         at += n
+
+
+def test_scheduler_over_a_latent_pool(vk):
+    """Sequences admitted, grown, evicted to the host, restored and compacted keep their rows: each decode equals one over
+    rows kept aside."""
+    from vulcan_b200.scheduler import PagedKVScheduler
+    g, page = gen(61), 64
+    pool = vk.LatentKVPool(1, 256, 32, 9, page_tokens=page)
+    host = torch.empty(8 * pool.page_bytes, dtype=torch.uint8).pin_memory()
+    sched = PagedKVScheduler(pool, host, 8)
+    rows = {}
+
+    def tables(ids):
+        return torch.from_numpy(sched.block_table(ids)).cuda(), torch.from_numpy(sched.lengths(ids)).cuda()
+
+    def append(sid, n):
+        new = rnd(g, n, 288)
+        bt, _ = tables([sid])
+        at = 0 if sid not in rows else len(rows[sid])
+        rows[sid] = new if not at else torch.cat([rows[sid], new])
+        pool.append(0, new[:, :256], new[:, 256:], bt, torch.tensor([at], dtype=torch.int32, device="cuda"))
+
+    def check(ids):
+        bt, lens = tables(ids)
+        ql, qr = rnd(g, len(ids), 4, 256), rnd(g, len(ids), 4, 32)
+        out, lse = pool.decode(0, ql, qr, bt, lens, 0.06, return_lse=True)
+        torch.cuda.synchronize()
+        assert pool.error_bits() == 0
+        c = type("Rows", (), dict(lens=[len(rows[i]) for i in ids], rows=[rows[i] for i in ids], dtype=torch.float16, latent=256, rope=32))
+        decode_bound_check(c, ql[:, None], qr[:, None], out[:, None], lse[:, None], 0.06, 1)
+
+    for sid, n in ((0, 130), (1, 64), (2, 190)):
+        assert sched.admit(sid, n)
+        append(sid, n)
+    assert [len(sched.seqs[i].pages) for i in range(3)] == [3, 1, 3]
+    check([0, 1, 2])
+    assert sched.grow(1)
+    append(1, 1)
+    assert sched.evict(0)
+    assert sched.admit(3, 200)  # pages that were sequence 0's
+    append(3, 200)
+    check([1, 2, 3])
+    torch.cuda.synchronize()
+    sched.release(2)
+    ids = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    assert sched.compact(lambda src, dst: pool.copy_pages(ids(src), ids(dst))) > 0
+    check([3, 1])
+    assert sched.restore(0)
+    torch.cuda.synchronize()
+    check([3, 0, 1])

@@ -180,3 +180,31 @@ def test_python_refusals_without_a_gpu():
         vk.LatentKVPool(1, 512, 64, 4, dtype=torch.float32)
     f, m = vk.RotaryEmbedding(64, theta=10000.0).frequencies()
     assert len(f) == 32 and f[0] == 1.0 and m == 1.0
+
+
+def test_scheduler_counts_a_pools_own_page_size():
+    from vulcan_b200.scheduler import PagedKVScheduler
+
+    class Pool:
+        page_bytes, page_tokens = 4, 64
+
+        def __init__(self):
+            self.left = list(range(6))
+
+        def pages_available(self):
+            return len(self.left)
+
+        def alloc(self, n):
+            got, self.left = self.left[:n], self.left[n:]
+            return got
+
+        def free(self, ids):
+            self.left += ids
+
+    sched = PagedKVScheduler(Pool())
+    assert sched.admit(0, 130) and len(sched.seqs[0].pages) == 3
+    for _ in range(62):
+        assert sched.grow(0)
+    assert sched.seqs[0].length == 192 and len(sched.seqs[0].pages) == 3
+    assert sched.grow(0) and len(sched.seqs[0].pages) == 4
+    assert PagedKVScheduler.pages_for(17) == 2

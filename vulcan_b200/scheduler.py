@@ -12,7 +12,8 @@ page reuse ordered.
 
 The pool is used through the methods ``alloc``, ``free``, ``pages_available``,
 ``swap_out``, ``swap_in``, ``compact_plan``, ``copy_pages`` and the attribute
-``page_bytes``, so tests can substitute a host-only model.
+``page_bytes`` (and ``page_tokens``, 16 without it), so tests can substitute a
+host-only model.
 """
 from __future__ import annotations
 
@@ -80,6 +81,7 @@ class PagedKVScheduler:
         bytes (or None for no swapping).  ``on_swap(kind, pages, fn)`` may wrap the
         swap calls (used by benchmarks to time them)."""
         self.pool = pool
+        self.page_tokens = getattr(pool, "page_tokens", PAGE_TOKENS)  # latent pools: 16, 32 or 64
         self.host = host_buffer
         self.arena = HostArena(host_slots)
         self.seqs: Dict[int, Sequence] = {}
@@ -92,8 +94,8 @@ class PagedKVScheduler:
 
     # ------------------------------------------------------------------ helpers
     @staticmethod
-    def pages_for(tokens: int) -> int:
-        return (tokens + PAGE_TOKENS - 1) // PAGE_TOKENS
+    def pages_for(tokens: int, page_tokens: int = PAGE_TOKENS) -> int:
+        return (tokens + page_tokens - 1) // page_tokens
 
     def _touch(self, sid: int) -> None:
         self.lru.pop(sid, None)
@@ -115,7 +117,7 @@ class PagedKVScheduler:
     def admit(self, sid: int, length: int) -> bool:
         """New sequence with ``length`` cached tokens (pages allocated, contents
         supplied by the caller's prefill).  Evicts LRU sequences if needed."""
-        need = self.pages_for(length)
+        need = self.pages_for(length, self.page_tokens)
         if not self._make_room(need):
             return False
         s = Sequence(sid, length, self.pool.alloc(need) if need else [])
@@ -126,7 +128,7 @@ class PagedKVScheduler:
     def grow(self, sid: int, protect=()) -> bool:
         """Makes room for one more token of a resident sequence."""
         s = self.seqs[sid]
-        if self.pages_for(s.length + 1) > len(s.pages):
+        if self.pages_for(s.length + 1, self.page_tokens) > len(s.pages):
             if not self._make_room(1, protect=set(protect) | {sid}):
                 return False
             s.pages += self.pool.alloc(1)
