@@ -378,10 +378,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
     uint64_t* k_empty = bars + 4;  // [2] both row tiles' S of a key tile done
     uint64_t* v_empty = bars + 6;  // [2]
     uint64_t* s_full = bars + 8;   // [row tile]
-    uint64_t* p_full = bars + 10;  // [row tile]
-    uint64_t* o_full = bars + 12;  // [row tile]
-    uint64_t* q_full = bars + 14;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+    uint64_t* p_full = bars + 10;  // [row tile][half of the keys] P written, before the first O rescaled
+    uint64_t* o_full = bars + 14;  // [row tile]
+    uint64_t* q_full = bars + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&k_full[i]), 3);  // the two units of W_k c and the rotary parts
@@ -390,8 +390,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
             mbar_init(smem_u32(&v_empty[i]), 1);
             mbar_init(smem_u32(&s_full[i]), 1);
         }
-        mbar_init(smem_u32(&p_full[0]), 4);
-        mbar_init(smem_u32(&p_full[1]), 4);
+        for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&p_full[i]), 4);
         mbar_init(smem_u32(&o_full[0]), 1);
         mbar_init(smem_u32(&o_full[1]), 1);
         mbar_init(smem_u32(q_full), 1);
@@ -514,27 +513,32 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
                     ok = ok && mbar_wait(smem_u32(&v_full[j & 1]), (j >> 1) & 1, p.err);
                     v_waited = j;
                 }
-                ok = ok && mbar_wait(smem_u32(&p_full[t]), j & 1, p.err);
-                if (ok) {
+                // in two halves of the keys: the first runs behind the second's exponentials
+                const uint32_t d = tmem + 256 + t * 128, a = tmem + t * 128;
+                const int slot = (5 * j + 3) & 7;
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    ok = ok && mbar_wait(smem_u32(&p_full[2 * t + hf]), j & 1, p.err);
+                    if (!ok) return;
                     tc_fence_after();
-                    const uint32_t d = tmem + 256 + t * 128, a = tmem + t * 128, acc = j > 0;
-                    const int slot = (5 * j + 3) & 7;
+                    const uint32_t acc = j > 0 || hf > 0;
                     if (slot < 7) {  // both 64-column units side by side: one MMA spans them
                         const uint32_t vl = v_lo + slot * kUnit16;
 #pragma unroll
-                        for (int ks = 0; ks < kLpKeys / 16; ++ks) umma_ts_lo(d, a + ks * 8, vl + ks * 128, v_hi, id_pv, ks ? 1 : acc);
+                        for (int ks = 4 * hf; ks < 4 * hf + 4; ++ks)
+                            umma_ts_lo(d, a + ks * 8, vl + ks * 128, v_hi, id_pv, ks & 3 ? 1 : acc);
                     } else {
 #pragma unroll 1
                         for (int u = 0; u < 2; ++u) {
                             const uint32_t vl = v_lo + ((slot + u) & 7) * kUnit16;
 #pragma unroll
-                            for (int ks = 0; ks < kLpKeys / 16; ++ks)
-                                umma_ts_lo(d + u * 64, a + ks * 8, vl + ks * 128, v_hi, id_half, ks ? 1 : acc);
+                            for (int ks = 4 * hf; ks < 4 * hf + 4; ++ks)
+                                umma_ts_lo(d + u * 64, a + ks * 8, vl + ks * 128, v_hi, id_half, ks & 3 ? 1 : acc);
                         }
                     }
-                    umma_commit(smem_u32(&o_full[t]));
-                    if (t == 1 || j >= ntB) umma_commit(smem_u32(&v_empty[j & 1]));
                 }
+                umma_commit(smem_u32(&o_full[t]));
+                if (t == 1 || j >= ntB) umma_commit(smem_u32(&v_empty[j & 1]));
             };
             if (ntA > 0) issue_s(0, 0);
             if (ntB > 0) issue_s(1, 0);
@@ -596,40 +600,43 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
             const uint64_t sc2 = f2(sc, sc), mneg2 = f2(mneg, mneg);
             uint64_t sum2[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < kLpKeys / 32; ++c) {
-                uint32_t pk[16];
+            for (int hf = 0; hf < 2; ++hf) {
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    float a0, a1;
-                    f2_get(f2_fma(f2(v[c][i], v[c][i + 1]), sc2, mneg2), a0, a1);
-                    a0 = ex2(a0);
-                    a1 = ex2(a1);
-                    sum2[(i >> 1) & 3] = f2_add(sum2[(i >> 1) & 3], f2(a0, a1));
-                    pk[i >> 1] = Elem<T>::pack(a0, a1);
+                for (int c = 2 * hf; c < 2 * hf + 2; ++c) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        float a0, a1;
+                        f2_get(f2_fma(f2(v[c][i], v[c][i + 1]), sc2, mneg2), a0, a1);
+                        a0 = ex2(a0);
+                        a1 = ex2(a1);
+                        sum2[(i >> 1) & 3] = f2_add(sum2[(i >> 1) & 3], f2(a0, a1));
+                        pk[i >> 1] = Elem<T>::pack(a0, a1);
+                    }
+                    tmem_st16(lane_base + s_col + c * 16, pk);
                 }
-                tmem_st16(lane_base + s_col + c * 16, pk);
+                // with half of the S row's registers dead
+                if (hf == 0 && j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+                    for (int c = 0; c < kLpHead / 32; ++c) {
+                        float o[32];
+                        tmem_ld32(lane_base + o_col + c * 32, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] *= alpha;
+                        tmem_st32(lane_base + o_col + c * 32, o);
+                    }
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&p_full[2 * t + hf]));
             }
             {
                 float s0, s1;
                 f2_get(f2_add(f2_add(sum2[0], sum2[1]), f2_add(sum2[2], sum2[3])), s0, s1);
                 l = l * alpha + (s0 + s1);
             }
-            // after P is stored, when the S row's registers are dead
-            if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
-                for (int c = 0; c < kLpHead / 32; ++c) {
-                    float o[32];
-                    tmem_ld32(lane_base + o_col + c * 32, o);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] *= alpha;
-                    tmem_st32(lane_base + o_col + c * 32, o);
-                }
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&p_full[t]));
         }
         const int64_t part = SPLIT ? ((((static_cast<int64_t>(b) * p.heads + hl) * p.q_tiles + qt) * p.splits + split) * 256 + t * kLpRows + r) : 0;
         if (SPLIT) p.part_ml[part] = make_float2(m_ref, l);  // (-inf, 0) where no key is seen
