@@ -375,22 +375,22 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
     uint64_t* v_full = bars + 2;   // [2]
     // even and odd key tiles have barriers of their own: the tile after the one the
     // producer waits for may complete first, and one barrier would then be a phase ahead
-    uint64_t* k_empty = bars + 4;  // [2] both row tiles' S of a key tile done
-    uint64_t* v_empty = bars + 6;  // [2]
-    uint64_t* s_full = bars + 8;   // [row tile]
+    uint64_t* v_empty = bars + 4;  // [2] both row tiles' P V of a key tile done
+    uint64_t* s_full = bars + 6;   // [row tile][2] S done; row tile B's (or the last to see the keys): K has been read too
     uint64_t* p_full = bars + 10;  // [row tile][half of the keys] P written, before the first O rescaled
-    uint64_t* o_full = bars + 14;  // [row tile]
+    uint64_t* o_full = bars + 14;  // [row tile] the last P V done
     uint64_t* q_full = bars + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&k_full[i]), 3);  // the two units of W_k c and the rotary parts
             mbar_init(smem_u32(&v_full[i]), 2);
-            mbar_init(smem_u32(&k_empty[i]), 1);
             mbar_init(smem_u32(&v_empty[i]), 1);
-            mbar_init(smem_u32(&s_full[i]), 1);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&p_full[i]), 4);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&p_full[i]), 4);
+        }
         mbar_init(smem_u32(&o_full[0]), 1);
         mbar_init(smem_u32(&o_full[1]), 1);
         mbar_init(smem_u32(q_full), 1);
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
                 mbar_expect_tx(kbar, kLpUnit);
                 tma_load_2d(sbase + kLaRing + ((5 * j + u) & 7) * kLpUnit, &tmapkv, hl * 256 + u * 64, wrow + j * kLpKeys,
                             kbar, pol);
-                if (j >= 1) ok = mbar_wait(smem_u32(&k_empty[(j - 1) & 1]), ((j - 1) >> 1) & 1, p.err);
+                if (j >= 1) ok = mbar_wait(smem_u32(&s_full[(j - 1 < ntB ? 2 : 0) + ((j - 1) & 1)]), ((j - 1) >> 1) & 1, p.err);
                 if (!ok) break;
                 mbar_expect_tx(vbar, kLpUnit);
                 tma_load_2d(sbase + kLaRing + ((5 * j + 3 + u) & 7) * kLpUnit, &tmapkv, hl * 256 + kLpHead + u * 64,
@@ -504,8 +504,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
                         for (int ks = 0; ks < 4; ++ks)
                             if (u < 2 || ks < rsteps) umma_ss_lo(d, ql + u * kUnit16 + ks * 2, k_hi, kl + ks * 2, k_hi, id_s, (u | ks) != 0);
                     }
-                    umma_commit(smem_u32(&s_full[t]));
-                    if (t == 1 || j >= ntB) umma_commit(smem_u32(&k_empty[j & 1]));
+                    umma_commit(smem_u32(&s_full[2 * t + (j & 1)]));
                 }
             };
             auto issue_pv = [&](int t, int j) {
@@ -537,8 +536,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
                         }
                     }
                 }
-                umma_commit(smem_u32(&o_full[t]));
+                // a commit costs this thread ~200 cycles, the second of two in a row more:
+                // three a step (six took 3,700 cycles a step)
                 if (t == 1 || j >= ntB) umma_commit(smem_u32(&v_empty[j & 1]));
+                if (j == (t ? ntB : ntA) - 1) umma_commit(smem_u32(&o_full[t]));
             };
             if (ntA > 0) issue_s(0, 0);
             if (ntB > 0) issue_s(1, 0);
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
         float m_ref = -INFINITY, l = 0.f;
         bool alive = true;
         for (int j = 0; j < ntt; ++j) {
-            if (!wait_all(smem_u32(&s_full[t]), j & 1, p.err)) { alive = false; break; }
+            if (!wait_all(smem_u32(&s_full[2 * t + (j & 1)]), (j >> 1) & 1, p.err)) { alive = false; break; }
             tc_fence_after();
             const int key0 = (kt0 + j) * kLpKeys;
             float v[kLpKeys / 32][32];
@@ -640,7 +641,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
         }
         const int64_t part = SPLIT ? ((((static_cast<int64_t>(b) * p.heads + hl) * p.q_tiles + qt) * p.splits + split) * 256 + t * kLpRows + r) : 0;
         if (SPLIT) p.part_ml[part] = make_float2(m_ref, l);  // (-inf, 0) where no key is seen
-        if (alive && ntt > 0 && wait_all(smem_u32(&o_full[t]), (ntt - 1) & 1, p.err)) {
+        if (alive && ntt > 0 && wait_all(smem_u32(&o_full[t]), 0, p.err)) {
             tc_fence_after();
             const float inv = 1.f / l;
             char* dst = SPLIT ? reinterpret_cast<char*>(p.part_o + part * kLpHead)
