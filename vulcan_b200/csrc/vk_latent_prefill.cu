@@ -28,15 +28,16 @@
 //    of whole 32 + 16 KiB tiles would not fit twice beside 96 KiB of queries;
 //    units let the next K load while the last V is read.
 //
-// Measured, 512 + 64, 32 heads: 8 chunks of 2048 tokens 521 us (614 in a long run under
-// the 1000 W cap), 141 of them the expansion and 380 the attention; the tensor pipe is
-// active for 59% and 46% of the cycles.  The expansion is bound by shared memory: a
-// stage of 64 latent elements takes 660 cycles, 640 of them reads of operands at 128
-// bytes a cycle.  A step of the attention (a key tile against two row tiles) takes
-// ~4,300 cycles, 2,560 of them MMAs: a softmax of ~1,900 cycles a tile (maximum 285,
-// exponentials and P 1,430, TMEM the rest) and the order S, softmax, P V of each row
-// tile leave the rest.  Not kept: a share of the exponentials by a polynomial on the
-// FMA pipe (no gain), two issuing threads (16% slower).
+// Measured, 512 + 64, 32 heads: 8 chunks of 2048 tokens 498 us (about 600 in a long run
+// under the 1000 W cap), 141 of them the expansion and 357 the attention.  The
+// expansion is bound by shared memory: a stage of 64 latent elements takes 660 cycles,
+// 640 of them reads of operands at 128 bytes a cycle.  A step of the attention (a key
+// tile against two row tiles) takes ~3,700 cycles, 2,300 to 2,560 of them MMAs: each row
+// tile's S, softmax (~1,900 cycles: maximum 285, exponentials and P 1,430, TMEM the
+// rest) and P V follow one another, and the issuing thread pays 150 to 200 cycles for
+// every barrier and commit between them.  Not kept: a share of the exponentials by a
+// polynomial on the FMA pipe (no gain), two issuing threads (16% slower), waiting for
+// the next tile's loads between the halves of P V (3% slower).
 #include "vk_internal.h"
 #include "vk_latent.cuh"
 #include "vk_ptx.cuh"
