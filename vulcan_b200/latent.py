@@ -228,24 +228,28 @@ class LatentKVPool(PagedKVPool):
         """latent [tokens, latent_dim], k_rope [tokens, rope_dim] (row-strided views); sequence b takes the rows
         offsets[b]..offsets[b+1]-1 (None: the same number each) from position positions[b] on.  ``norm_weight``: root
         mean square norm of the latent first; ``rope``: k_rope rotated at its position."""
-        dev, index = self.device, self._index
+        index, dtype = self._index, self.dtype
         batch, width = _tables(block_tables, index)
-        for t, name, d in ((latent, "latent", self.latent_dim), (k_rope, "k_rope", self.rope_dim)):
-            _on(t, self.dtype, name, index)
-            if t.dim() != 2 or t.shape[1] != d or t.stride(1) != 1:
+        latent_rows, rope_rows = latent.stride(), k_rope.stride()
+        for t, name, d, rows in ((latent, "latent", self.latent_dim, latent_rows), (k_rope, "k_rope", self.rope_dim, rope_rows)):
+            if t.dtype is not dtype or t.get_device() != index:
+                _on(t, dtype, name, index)
+            if len(rows) != 2 or rows[1] != 1 or t.shape[1] != d:
                 raise ValueError("%s must be [tokens, %d] with unit stride along its rows" % (name, d))
         tokens = latent.shape[0]
         if k_rope.shape[0] != tokens:
             raise ValueError("latent and k_rope must have the same tokens")
+        weight = None
         if norm_weight is not None:
-            _on(norm_weight, self.dtype, "norm_weight", index)
+            _on(norm_weight, dtype, "norm_weight", index)
             if norm_weight.numel() != self.latent_dim or not norm_weight.is_contiguous():
                 raise ValueError("norm_weight must be contiguous with %d elements" % self.latent_dim)
+            weight = norm_weight.data_ptr()
         if rope is not None and not rope.handle.value:
             raise ValueError("rope is closed")
         check(self._lib.vk_latent_append(
-            self.handle, layer, latent.data_ptr(), latent.stride(0), k_rope.data_ptr(), k_rope.stride(0),
-            None if norm_weight is None else norm_weight.data_ptr(), eps, None if rope is None else rope.handle,
+            self.handle, layer, latent.data_ptr(), latent_rows[0], k_rope.data_ptr(), rope_rows[0], weight, eps,
+            None if rope is None else rope.handle,
             block_tables.data_ptr(), width, _i32(positions, "positions", index, batch),
             None if offsets is None else _i32(offsets, "offsets", index, batch + 1), batch, tokens, _stream_of(stream, index)),
             "vk_latent_append")
