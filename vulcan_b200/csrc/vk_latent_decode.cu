@@ -53,6 +53,7 @@
 // key gets its NaN through S.
 #include "vk_internal.h"
 #include "vk_latent.cuh"
+#include "vk_latent_deal.h"
 #include "vk_ptx.cuh"
 #include "vk_rotary.cuh"
 #include "vk_tc.cuh"
@@ -69,9 +70,6 @@ constexpr int kLdSmemMax = 232448;
 // A unit's prologue and epilogue (q load, output) in tiles, for the deal (2 to 4 are
 // within 2% of one another, 1 and 6 slower).
 constexpr int kLdUnitCost = 3;
-// Least cost of a CTA's range (1 x 200 tokens: 12.5 us with 1, 14.7 with 4: tiles in
-// parallel and a merge beat tiles in turn)
-constexpr int kLdMinRange = 1;
 
 struct LdParams {
     const char* ql;
@@ -85,7 +83,7 @@ struct LdParams {
     float4* ws_o;    // partial O: ld_part()
     float2* ws_ml;   // [2 * CTAs][64]: maximum (log2 domain), sum
     int2* ws_unit;   // [units]: first and last CTA of a split unit, or (-1, -1)
-    int bt_stride, B, T, H, groups, layer, num_pages, P, latent, rope, nch, stages, capacity;
+    int bt_stride, B, T, H, groups, layer, num_pages, P, latent, rope, nch, stages, capacity, ctas;
     float scale_log2;
 };
 
@@ -93,26 +91,6 @@ __device__ __forceinline__ int ld_len(const LdParams& p, int b) {
     const int len = __ldg(p.lens + b);
     return len < 0 || len > p.capacity ? 0 : len;
 }
-
-// n CTAs share `total`: the first `rem` take q + 1, the others q.  (64-bit
-// divisions cost hundreds of cycles of every launch; totals below 2^32 need none.)
-struct LdDeal {
-    int64_t q, rem;
-    int n;
-    __device__ __forceinline__ LdDeal(int64_t total, int ctas) {
-        n = static_cast<int>(min(static_cast<int64_t>(ctas), (total + kLdMinRange - 1) / kLdMinRange));
-        q = div(total, n);
-        rem = total - q * n;
-    }
-    static __device__ __forceinline__ int64_t div(int64_t a, int64_t b) {
-        return (a | b) >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
-    }
-    __device__ __forceinline__ int64_t start(int c) const { return c * q + min(static_cast<int64_t>(c), rem); }
-    __device__ __forceinline__ int owner(int64_t v) const {  // the CTA whose range holds v
-        const int64_t head = rem * (q + 1);
-        return static_cast<int>(v < head ? div(v, q + 1) : rem + div(v - head, q));
-    }
-};
 
 struct LdPiece {
     int b, g, t0, t1, tiles, len;
@@ -702,7 +680,7 @@ __global__ void __launch_bounds__(D * KG) latent_merge_kernel(const __grid_const
     if (row_in >= rows) return;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int2 u = p.ws_unit[unit];
-    if (u.x < 0) return;
+    if (!ld_joinable(u.x, u.y, p.ctas)) return;
     // piece i of CTA u.x + i: the first tile's piece in the odd slot, the others in even ones
     auto slot_of = [&](int i) { return 2 * (u.x + i) + (i == 0 ? 1 : 0); };
     const int pieces = u.y - u.x + 1;
@@ -819,7 +797,7 @@ static vk_status launch_latent_decode(vk_pool* pool, const LdParams& p, cudaStre
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(latent_decode)");
         attr_set |= bit;
     }
-    latent_decode_kernel<T, LCH><<<min(pool->num_sms, kLdMaxPieces), kLdThreads, smem, st>>>(pool->tmap16, p);
+    latent_decode_kernel<T, LCH><<<p.ctas, kLdThreads, smem, st>>>(pool->tmap16, p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "latent_decode_kernel launch");
     const int64_t units = static_cast<int64_t>(p.B) * p.groups;
@@ -905,6 +883,7 @@ extern "C" vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* 
     p.layer = layer;
     p.num_pages = pool->num_pages;
     p.P = pool->cfg.page_tokens;
+    p.ctas = min(pool->num_sms, kLdMaxPieces);
     const int64_t capacity = static_cast<int64_t>(bt_stride) * p.P;
     p.capacity = static_cast<int>(capacity < 0x7fffff00 ? capacity : 0x7fffff00);  // (rounded up to tiles in int32)
     p.latent = pool->latent_dim;
