@@ -150,8 +150,10 @@ static vk_status rotary_frequencies(const vk_rotary_cfg& c, double* f, double* m
         auto pair_of = [&](double turns) {
             return c.rotary_dim * std::log(c.original_len / (turns * two_pi)) / (2.0 * std::log(c.theta_base));
         };
-        const double first = std::max(std::floor(pair_of(c.high)), 0.0);
-        const double last = std::min(std::ceil(pair_of(c.low)), static_cast<double>(n - 1));
+        // the ramp may end behind the last pair: cut there, it would give pairs that make
+        // more than `low` turns the whole factor
+        const double last = std::min(std::ceil(pair_of(c.low)), static_cast<double>(c.rotary_dim - 1));
+        const double first = std::min(std::max(std::floor(pair_of(c.high)), 0.0), last);
         for (int i = 0; i < n; ++i) {
             const double ramp = std::min(std::max((i - first) / std::max(last - first, 0.001), 0.0), 1.0);
             f[i] = f[i] * (1.0 - ramp) + f[i] / c.factor * ramp;
