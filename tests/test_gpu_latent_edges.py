@@ -1,0 +1,71 @@
+"""GPU tests of the latent cache's attention where its arithmetic is tight, against 64 bits.
+
+Tolerances as in test_gpu_latent.py, and for fp16 weights one more term: a weight is
+stored as 2^11 (up to 2^15) times its share of the row's largest, so that one below 2^-25
+of the largest lies among fp16's subnormals and is off by up to 2^-25 / 2^11 = 2^-36 of the
+largest weight p_max: p_max 2^-36 sum_j |v_j| in all."""
+import math
+
+import pytest
+import torch
+
+from .test_gpu_latent import Cache, gen, rnd
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def vk(cuda_ok):
+    import vulcan_b200
+    vulcan_b200.load()
+    return vulcan_b200
+
+
+# ------------------------------------------------------------------ one dominant key
+
+BITS = [0.0, 12.0, 20.0, 24.0, 25.0, 26.0, 28.0, 34.0]  # binary orders between the dominant key and the others
+KEYS = 131072
+
+
+def sink(vk, at, dtype=torch.float16):
+    """A sequence whose key `at` is the only one with a score, the others hold the values."""
+    g = gen(at)
+    c = Cache(vk, [KEYS], 128, 16, 64, layers=1, layer=0, dtype=dtype)
+    rows = torch.cat([0.5 + torch.rand(KEYS, 128, generator=g, device="cuda"), torch.zeros(KEYS, 16, device="cuda")], -1).to(dtype)
+    rows[:, 0] = 0
+    rows[at] = 0
+    rows[at, 0] = 16
+    c.pool.latent_view()[0, c.tables[0].long()] = rows.view(-1, 64, 144)
+    return c, rows
+
+
+def weak_weight_bound(p, v, e, share):
+    """Bound of sum_j p_j v_j without the output's own rounding; `share`: roundings of a product's factors."""
+    return p @ v.abs() * share + p.amax(-1, keepdim=True) * 2.0 ** -36 * v.abs().sum(0) * (e < 2.0 ** -9)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("at,sequences", [(5, 1), (KEYS - 70, 1), (5, 200)])
+def test_decode_one_dominant_key(vk, dtype, at, sequences):
+    """Many keys of little weight each keep their part of the output.  200 sequences that share their pages: a CTA has
+    whole sequences to itself, and the dominant key stands against all the others in it."""
+    c, rows = sink(vk, at, dtype)
+    scale, e = 0.07, torch.finfo(dtype).eps / 2
+    ql = torch.zeros(sequences, len(BITS), 128, device="cuda")
+    ql[..., 0] = torch.tensor(BITS, device="cuda") * math.log(2) / (16 * scale)
+    ql = ql.to(dtype)
+    qr = torch.zeros(sequences, len(BITS), 16, device="cuda").to(dtype)
+    tables = c.tables.expand(sequences, -1).contiguous()
+    lens = torch.full((sequences,), KEYS, dtype=torch.int32, device="cuda")
+    out, lse = c.pool.decode(0, ql, qr, tables, lens, scale, return_lse=True)
+    assert c.check() == 0
+    x = rows.double()
+    a = scale * ql[0].double() @ x[:, :128].t()
+    want_lse = torch.logsumexp(a, -1)
+    p = torch.exp(a - want_lse[:, None])
+    want = p @ x[:, :128]
+    ds = a.abs().amax(-1, keepdim=True) * 144 * 2.0 ** -24
+    bound = weak_weight_bound(p, x[:, :128], e, e + 4 * ds + 2.0 ** -18) + e * want.abs() + 2.0 ** -25
+    err = (out.double() - want).abs()
+    assert (err <= bound).all(), "rows' worst %s of the bound" % (err / bound).amax((0, 2)).tolist()
+    assert ((lse.double() - want_lse).abs() <= ds[:, 0] + 2.0 ** -20 + want_lse.abs() * 2.0 ** -22).all()

@@ -36,6 +36,26 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
     return r;
 }
 
+// The unnormalised weights of both attentions are 2^(s - m) (s: scores in the log2
+// domain), with m a reference below the row's running maximum by kMargin or, while the
+// maximum has grown since m was taken, by up to kMargin + kLag: a growth by more than
+// kLag moves m and rescales O.  The weights are rounded to the cache's type for the
+// second product.  fp16 has normal numbers from 2^-14 to 2^16 only: with m at the maximum
+// itself, the weights of keys 2^-25 below it became 0 there and still counted in full in
+// the fp32 sum, and 131,072 such keys lost 0.4% of the mass to one dominant key.  Weights up to
+// 2^(kMargin + kLag) = 2^15 use the range above 1: relative 2^-11 down to 2^-25 of the
+// maximum, absolute 2^-36 of it below.  bf16 has fp32's range and needs no margin.
+template <typename T>
+struct Weights {
+    static constexpr float kMargin = Elem<T>::kBf16 ? 0.f : 11.f;
+    static constexpr float kLag = Elem<T>::kBf16 ? 8.f : 4.f;
+    // log2 of the sum of 2^s from the reference and the sum of the weights
+    static __device__ __forceinline__ float log2_sum(float m, float l) {
+        constexpr float unit = Elem<T>::kBf16 ? 1.f : 0x1p-11f;
+        return (m + kMargin) + log2f(l * unit);
+    }
+};
+
 // 0 in the place of each non-finite 16-bit element of a word.
 template <typename T>
 __device__ __forceinline__ uint32_t finite_word(uint32_t w) {

@@ -28,11 +28,13 @@
 //    (r/16)*32 + r%16 of TMEM (M = 64 fills 16 lanes of each warp's quarter); the
 //    matrix-fragment load spreads them over all 32 threads (2 rows x 16 keys
 //    each), and P goes to shared memory by stmatrix.  O is rescaled only when a
-//    row's maximum grows by more than 2^8 (all warps vote).
+//    row's maximum grows by more than 2^8 (bf16) or 2^4 (fp16; all warps vote).
 //
-// P is rounded to the cache's 16-bit type for the second product: relative
-// error 2^-9 (bf16) or 2^-12 (fp16) a weight, below the output's own rounding;
-// the sum of the weights is taken from the unrounded fp32 values.
+// P is rounded to the cache's 16-bit type for the second product, the type that
+// the tensor core takes beside it: relative 2^-8 (bf16) or 2^-11 (fp16) a weight at
+// most, the same step as the output's own rounding, absolute 2^-36 of the row's
+// largest weight among fp16's subnormals (struct Weights); the sum of the weights is
+// taken from the unrounded fp32 values.
 //
 // Measured, 512 + 64, 64 rows: 24 sequences of ~16k tokens 89 us, 0.75 of the
 // measured copy rate (under the 1000 W cap in a long run, at 1.70 GHz, 100 us); in
@@ -81,7 +83,7 @@ struct LdParams {
     const int32_t* lens;
     uint32_t* err;
     float4* ws_o;    // partial O: ld_part()
-    float2* ws_ml;   // [2 * CTAs][64]: maximum (log2 domain), sum
+    float2* ws_ml;   // [2 * CTAs][64]: reference of the weights (log2 domain), sum
     int2* ws_unit;   // [units]: first and last CTA of a split unit, or (-1, -1)
     int bt_stride, B, T, H, groups, layer, num_pages, P, latent, rope, nch, stages, capacity, ctas;
     float scale_log2;
@@ -489,8 +491,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     al[u] = 1.f;
-                    if (top > m[u] + 8.f || m[u] == -INFINITY) {
-                        const float mn = fmaxf(m[u], top);
+                    if (top > m[u] + (Weights<T>::kMargin + Weights<T>::kLag) || m[u] == -INFINITY) {
+                        const float mn = fmaxf(m[u], top - Weights<T>::kMargin);
                         al[u] = m[u] == -INFINITY ? 0.f : ex2(m[u] - mn);
                         m[u] = mn;
                         resc = resc || live_row[u];
@@ -579,7 +581,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                     inv_l[rr] = l[u] > 0.f || l[u] != l[u] ? 1.f / l[u] : 0.f;
                     if (!whole) p.ws_ml[slot * 64 + rr] = make_float2(m[u], l[u]);
                     else if (p.lse && live_row[u])
-                        p.lse[row0 + rr] = l[u] == 0.f ? -INFINITY : (m[u] + log2f(l[u])) * 0.69314718055994531f;
+                        p.lse[row0 + rr] = l[u] == 0.f ? -INFINITY : Weights<T>::log2_sum(m[u], l[u]) * 0.69314718055994531f;
                 }
             }
             if (threadIdx.x == 0 && c.t0 == 0) {
@@ -780,7 +782,7 @@ __global__ void __launch_bounds__(D * KG) latent_merge_kernel(const __grid_const
             reinterpret_cast<T*>(p.out)[(row + r) * (LCH * 64) + k * 128 + e0] = Elem<T>::down(inv == 0.f ? 0.f : a * inv);
         }
         if (p.lse && blockIdx.y % kSplit == 0 && threadIdx.x == 0)
-            p.lse[row + r] = lv[r] == 0.f ? -INFINITY : (mv[r] + log2f(lv[r])) * 0.69314718055994531f;
+            p.lse[row + r] = lv[r] == 0.f ? -INFINITY : Weights<T>::log2_sum(mv[r], lv[r]) * 0.69314718055994531f;
     }
 }
 
