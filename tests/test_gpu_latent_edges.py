@@ -69,3 +69,30 @@ def test_decode_one_dominant_key(vk, dtype, at, sequences):
     err = (out.double() - want).abs()
     assert (err <= bound).all(), "rows' worst %s of the bound" % (err / bound).amax((0, 2)).tolist()
     assert ((lse.double() - want_lse).abs() <= ds[:, 0] + 2.0 ** -20 + want_lse.abs() * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("at,heads", [(5, 2), (KEYS - 70, 2), (5, 40)])
+def test_prefill_one_dominant_key(vk, dtype, at, heads):
+    """As above in the expanded form: keys [c_0, 0, ...] (exact in 16 bits), values c; few heads cut along the keys, and many."""
+    c, rows = sink(vk, at, dtype)
+    scale, e, new = 0.07, torch.finfo(dtype).eps / 2, len(BITS)
+    w = torch.zeros(heads, 256, 128, device="cuda")
+    w[:, 0, 0] = 1
+    w[:, 128:] = torch.eye(128, device="cuda")
+    w = w.view(heads * 256, 128).to(dtype)
+    q = torch.zeros(new, heads, 144, device="cuda")
+    q[..., 0] = (torch.tensor(BITS, device="cuda") * math.log(2) / (16 * scale))[:, None]
+    q = q.to(dtype)
+    out = c.pool.prefill(0, q, w, c.tables, c.seq_lens - new, scale=scale)
+    assert c.check() == 0
+    x = rows[:, :128].double()
+    hidden = torch.arange(KEYS, device="cuda")[None] > torch.arange(KEYS - new, KEYS, device="cuda")[:, None]
+    a = scale * q[:, 0, :1].double() @ x[:, :1].t()
+    p = torch.softmax(a.masked_fill(hidden, -math.inf), -1)
+    want = p @ x
+    ds = a.abs().amax(-1, keepdim=True) * (144 + 128) * 2.0 ** -24
+    # values are exact: c times one
+    bound = weak_weight_bound(p, x, e, e + 4 * ds + 2.0 ** -18) + e * want.abs() + 2.0 ** -25
+    err = (out.double() - want[:, None]).abs()
+    assert (err <= bound[:, None]).all(), "rows' worst %s of the bound" % (err / bound[:, None]).amax((1, 2)).tolist()

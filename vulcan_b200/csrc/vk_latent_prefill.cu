@@ -16,13 +16,15 @@
 //    memory (128 KiB at 512), row tile 1 in TMEM (256 columns), as the A operands of
 //    its MMAs.  With one row tile a CTA the same GEMM took 150 us at 8 x 2048 tokens
 //    and 32 heads, with two 141.  Output rows [token][head][128 K | 128 V] in the
-//    workspace, rounded to the cache's 16-bit type (relative 2^-9 or 2^-12 of
-//    each element, as a cache of keys and values holds them); rows behind the
+//    workspace, rounded to the cache's 16-bit type (relative 2^-8 in bf16 and 2^-11
+//    in fp16 at most, as a cache of keys and values holds them: in fp32 they would
+//    be twice the workspace and its traffic, and no operand of kind::f16); rows behind the
 //    sequence are stored as zeros, so the attention reads no stale bytes.
 //  * latent_prefill_kernel: causal attention, one CTA per (256 query rows, head,
 //    sequence): the rows are two 128-row tiles whose softmax steps alternate on
 //    one tensor core (S_A, S_B, then P V of one tile while the other's softmax
-//    runs), P in TMEM as the A operand.  K and V move through one ring of eight
+//    runs), P in TMEM as the A operand, rounded to the cache's type (vk_latent.cuh,
+//    struct Weights), its sum kept in fp32 unrounded.  K and V move through one ring of eight
 //    16 KiB units (128 keys x 64 elements): a key tile takes three for K (two of
 //    W_k c from the workspace, one of r from the pages) and two for V.  K and V
 //    of whole 32 + 16 KiB tiles would not fit twice beside 96 KiB of queries;
@@ -62,7 +64,7 @@ struct LpParams {
     int bt_stride, B, tokens, H, heads, h0, layer, num_pages, P, latent, rope, lpad, max_tokens, max_len, stages, per_cta;
     int q_tiles, splits;   // attention: 256-row tiles of the longest chunk, key ranges a CTA's tile is cut into
     float* part_o;         // splits > 1: [q tile of (b, head)][split][256][128] unnormalised O
-    float2* part_ml;       // and its (maximum, sum) [..][256]
+    float2* part_ml;       // and its (reference of the weights, their sum) [..][256]
     float scale_log2;
 };
 
@@ -593,8 +595,8 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
                 }
             const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
             float alpha = 1.f;
-            if (mx > m_ref + 8.f || m_ref == -INFINITY) {
-                const float m_new = fmaxf(m_ref, mx);
+            if (mx > m_ref + (Weights<T>::kMargin + Weights<T>::kLag) || m_ref == -INFINITY) {
+                const float m_new = fmaxf(m_ref, mx - Weights<T>::kMargin);
                 alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - m_new);
                 m_ref = m_new;
             }
