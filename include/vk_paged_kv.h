@@ -474,6 +474,10 @@ vk_status vk_latent_append(vk_pool* pool, int32_t layer, const void* latent, int
  * Query token t of tokens_per_seq (T) sees the first seq_lens[b] - (T-1-t)
  * rows: seq_lens (device) counts all T tokens, appended before the call.  A row
  * that sees nothing gives zeros and an lse of -inf.
+ * NaN and infinities of a cached row reach the query rows that see it, as the
+ * formula has it, and no others: a score of +inf or NaN makes the whole row NaN,
+ * one of -inf is a weight of 0, NaN only in elements where the latent is not
+ * finite; a row whose every score is -inf is NaN.
  * Element (b, t, h, d) of q_latent: [(b*T + t)*ql_token_stride +
  * h*ql_head_stride + d], q_rope (rotated already) likewise; out: [batch, T,
  * num_heads, latent_dim], lse (optional): [batch, T, num_heads] fp32, the natural

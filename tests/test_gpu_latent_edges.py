@@ -96,3 +96,98 @@ def test_prefill_one_dominant_key(vk, dtype, at, heads):
     bound = weak_weight_bound(p, x, e, e + 4 * ds + 2.0 ** -18) + e * want.abs() + 2.0 ** -25
     err = (out.double() - want[:, None]).abs()
     assert (err <= bound[:, None]).all(), "rows' worst %s of the bound" % (err / bound[:, None]).amax((1, 2)).tolist()
+
+
+# ------------------------------------------------------------------ infinite and NaN latents
+
+
+def decode_pattern_check(c, rows, ql, qr, out, lse, scale):
+    """Every row against the formula in 64 bits: a weight of zero times an infinite element is NaN in that element, an
+    infinite or NaN score makes the row NaN; finite elements are held to the usual bound."""
+    e, tokens = torch.finfo(c.dtype).eps / 2, ql.shape[1]
+    kinds = set()
+    for b, n in enumerate(c.lens):
+        x = rows[b].double()
+        size_x = torch.where(torch.isfinite(x), x, 0.0).abs()
+        for t in range(tokens):
+            k = max(0, n - (tokens - 1 - t))
+            o, s = out[b, t].double(), lse[b, t].double()
+            if not k:
+                assert (o == 0).all() and (s == -math.inf).all()
+                continue
+            q = torch.cat([ql[b, t], qr[b, t]], -1).double()
+            a = scale * q @ x[:k].t()
+            p = torch.softmax(a, -1)
+            want = p @ x[:k, :c.latent]
+            bad = torch.isnan(want)
+            assert torch.equal(torch.isnan(o), bad), "sequence %d token %d: NaN where none belongs, or none where one does" % (b, t)
+            kinds |= {"row" if r.all() else "some" if r.any() else "none" for r in bad}
+            ds = float((scale * q.abs() @ size_x[:k].t()).max()) * (c.latent + c.rope) * 2.0 ** -24
+            pf = torch.where(torch.isnan(p), 0.0, p)
+            bound = pf @ size_x[:k, :c.latent] * (e + 4 * ds + 2.0 ** -18) + e * want.abs() + 2.0 ** -25
+            assert ((o - want).abs() <= bound)[~bad].all(), (b, t)
+            whole = ~torch.isnan(p).any(-1)
+            want_lse = torch.logsumexp(a, -1)
+            assert ((s - want_lse).abs() <= ds + 2.0 ** -20 + want_lse.abs() * 2.0 ** -22)[whole].all()
+            assert not torch.isfinite(s[~whole]).any()
+    return kinds
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("lens,heads", [([65, 130, 64, 2, 1], 4), ([65, 300, 3], 40), ([20000], 30)])
+def test_decode_broken_latents(vk, dtype, bad, lens, heads):
+    """Broken latents among the drafted rows and before them, in sequences that one CTA has and that all share."""
+    g, tokens, scale = gen(len(lens) + heads), 3, 0.07
+    c = Cache(vk, lens, 256, 32, 32, layers=2, layer=1, dtype=dtype)
+    ql, qr = rnd(g, len(lens), tokens, heads, 256, dtype=dtype, std=0.5), rnd(g, len(lens), tokens, heads, 32, dtype=dtype)
+    view = c.pool.latent_view()
+
+    def spoil(b, key, element, value):
+        if key >= 0:
+            c.rows[b][key, element] = value
+            view[1, int(c.tables[b, key // 32]), key % 32, element] = value
+
+    for b, n in enumerate(lens):
+        spoil(b, n - 1, 100, bad)  # token 2 sees it
+        spoil(b, n - 2, 7, -bad)   # tokens 1 and 2
+    out, lse = c.pool.decode(1, ql, qr, c.tables, c.seq_lens, scale, return_lse=True)
+    assert c.check() == 0
+    kinds = decode_pattern_check(c, c.rows, ql, qr, out, lse, scale)
+    assert kinds >= ({"row", "none"} if bad != bad else {"row", "some", "none"})
+    again, lse2 = c.pool.decode(1, ql, qr, c.tables, c.seq_lens, scale, return_lse=True)
+    assert torch.equal(out.view(torch.int16), again.view(torch.int16)) and torch.equal(lse.view(torch.int32), lse2.view(torch.int32))
+    for b, n in enumerate(lens):
+        if n > 60:
+            spoil(b, 5, 200, bad)  # all tokens see it
+    out, lse = c.pool.decode(1, ql, qr, c.tables, c.seq_lens, scale, return_lse=True)
+    assert c.check() == 0
+    decode_pattern_check(c, c.rows, ql, qr, out, lse, scale)
+    # an infinite rotary part: a score of -inf weighs nothing and leaves no element, one of +inf makes the row NaN
+    for b, n in enumerate(lens):
+        spoil(b, n - 1, 100, 0.5)
+        spoil(b, n - 2, 7, 0.5)
+        spoil(b, 5 if n > 60 else -1, 200, 0.5)
+        spoil(b, n - 1, 256 + 3, bad)
+    out, lse = c.pool.decode(1, ql, qr, c.tables, c.seq_lens, scale, return_lse=True)
+    assert c.check() == 0
+    decode_pattern_check(c, c.rows, ql, qr, out, lse, scale)
+
+
+def test_decode_rows_that_see_only_infinite_scores(vk):
+    """One cached row whose score is -inf: 0/0 by the formula, not the zeros of a row that sees nothing; alone and in
+    sequences that several CTAs share."""
+    g, scale = gen(77), 0.07
+    c = Cache(vk, [1, 0, 1, 4000], 128, 16, 16, layers=1, layer=0)
+    ql, qr = rnd(g, 4, 1, 3, 128, std=0.5), rnd(g, 4, 1, 3, 16)
+    ql[..., 9] = ql[..., 9].abs() + 0.5
+    view = c.pool.latent_view()
+    for b, n in enumerate(c.lens):
+        c.rows[b][:, 9] = -math.inf
+        ids = c.tables[b].repeat_interleave(16)[:n].long()
+        view[0, ids, torch.arange(n, device="cuda") % 16, 9] = -math.inf
+    out, lse = c.pool.decode(0, ql, qr, c.tables, c.seq_lens, scale, return_lse=True)
+    assert c.check() == 0
+    for b in (0, 2, 3):
+        assert torch.isnan(out[b]).all() and (lse[b] == -math.inf).all()
+    assert (out[1] == 0).all() and (lse[1] == -math.inf).all()

@@ -51,8 +51,10 @@
 //
 // Rows of the last tile behind the sequence are zeroed in shared memory before
 // the second product (0 * NaN is NaN), and keys that only some of the T tokens
-// may see have non-finite elements cleared there: a row that does see such a
-// key gets its NaN through S.
+// may see have non-finite elements cleared there.  A row that does see such a
+// key gets its NaN through S where the score is +inf or NaN; a score of -inf is a
+// weight of 0, and 0 * inf is NaN in the infinite element alone, as in a tile that all
+// rows see: those elements are written behind the output (ld_broken_keys).
 #include "vk_internal.h"
 #include "vk_latent.cuh"
 #include "vk_latent_deal.h"
@@ -74,6 +76,7 @@ constexpr int kLdSmemMax = 232448;
 constexpr int kLdUnitCost = 3;
 
 struct LdParams {
+    const char* base;  // the layer's region
     const char* ql;
     const char* qr;
     int64_t ql_token, ql_head, qr_token, qr_head;  // strides in elements
@@ -92,6 +95,12 @@ struct LdParams {
 __device__ __forceinline__ int ld_len(const LdParams& p, int b) {
     const int len = __ldg(p.lens + b);
     return len < 0 || len > p.capacity ? 0 : len;
+}
+
+// 1 / l of a row.  A row that sees no key has l = 0 and gives zeros; one whose every
+// score is -inf has l = 0 too, and 0 / 0 of the formula is NaN.
+__device__ __forceinline__ float ld_inverse(float l, bool sees) {
+    return l != 0.f ? 1.f / l : sees ? __uint_as_float(0x7fffffffu) : 0.f;
 }
 
 struct LdPiece {
@@ -160,6 +169,35 @@ __device__ __forceinline__ bool bar_softmax_or(bool x) {
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+// NaN in the output (or partial output) elements that a non-finite element of a key
+// reaches: of the keys of the piece that only some tokens may see, in the rows that see
+// them.  Called by the 128 softmax threads, behind the piece's output, when one of them
+// cleared such an element.
+template <typename T, int LCH>
+__device__ __forceinline__ void ld_broken_keys(const LdParams& p, const LdPiece& c, int slot, int live) {
+    bar_softmax();  // behind the stores of the other threads
+    const int first = max(max(c.len - (p.T - 1), 0), c.t0 * kLdKeys), end = min(c.len, c.t1 * kLdKeys);
+    const int64_t row0 = static_cast<int64_t>(c.b) * p.T * p.H + c.g * 64;
+    constexpr uint32_t e = Elem<T>::kBf16 ? 0x7f80u : 0x7c00u;
+#pragma unroll 1
+    for (int key = first; key < end; ++key) {
+        int page = __ldg(p.bt + static_cast<int64_t>(c.b) * p.bt_stride + key / p.P);
+        if (page < 0 || page >= p.num_pages) page = 0;  // as the tile had it
+        const uint16_t* x = reinterpret_cast<const uint16_t*>(p.base) +
+                            (static_cast<int64_t>(page) * p.P + key % p.P) * (p.latent + p.rope);
+        // rows from this one on see the key
+        const int64_t from = (static_cast<int64_t>(key) - c.len + p.T) * p.H - c.g * 64;
+#pragma unroll 1
+        for (int d = threadIdx.x; d < LCH * 64; d += 128) {
+            if ((__ldg(x + d) & e) != e) continue;
+            for (int r = static_cast<int>(max(from, static_cast<int64_t>(0))); r < live; ++r) {
+                if (c.whole()) reinterpret_cast<uint16_t*>(p.out)[(row0 + r) * (LCH * 64) + d] = 0x7fff;
+                else reinterpret_cast<float*>(p.ws_o + ld_part<LCH>(slot, r >> 2, d >> 7, d & 127))[r & 3] = __uint_as_float(0x7fffffffu);
+            }
+        }
+    }
 }
 
 template <typename T, int LCH>  // LCH: latent_dim / 64
@@ -464,6 +502,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                 lim[u] = c.len - (p.T - 1 - (live_row[u] ? row / p.H : p.T - 1));
             }
             const int lim0 = c.len - (p.T - 1);  // keys that every token sees
+            bool broken = false;                 // this thread cleared a non-finite element
             for (int t = c.t0; t < c.t1; ++t, ++it) {
                 const int key0 = t * kLdKeys;
                 fail = !wait_all(smem_u32(&s_full[it & 1]), (it >> 1) & 1, p.err) || fail;
@@ -526,7 +565,9 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                                          : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
                                          : "r"(addr));
+                            const uint4 y = x;
                             x = make_uint4(finite_word<T>(x.x), finite_word<T>(x.y), finite_word<T>(x.z), finite_word<T>(x.w));
+                            broken = broken || ((x.x ^ y.x) | (x.y ^ y.y) | (x.z ^ y.z) | (x.w ^ y.w));
                         }
                         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
                                      : "memory");
@@ -578,7 +619,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                 l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
                 if ((lane & 3) == 0) {
                     const int rr = r + 8 * u;
-                    inv_l[rr] = l[u] > 0.f || l[u] != l[u] ? 1.f / l[u] : 0.f;
+                    inv_l[rr] = ld_inverse(l[u], lim[u] > 0);
                     if (!whole) p.ws_ml[slot * 64 + rr] = make_float2(m[u], l[u]);
                     else if (p.lse && live_row[u])
                         p.lse[row0 + rr] = l[u] == 0.f ? -INFINITY : Weights<T>::log2_sum(m[u], l[u]) * 0.69314718055994531f;
@@ -591,7 +632,8 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                 p.ws_unit[static_cast<int64_t>(c.b) * p.groups + c.g] = u;
             }
             fail = !wait_all(smem_u32(pv_done), (it - 1) & 1, p.err) || fail;
-            if (bar_softmax_or(fail)) goto done;
+            const bool odd = bar_softmax_or(fail || broken);
+            if (odd && bar_softmax_or(fail)) goto done;
             tc_fence_after();
             const int live = min(64, rows - c.g * 64);
             // rolled loops: a CTA runs this once or twice, and unrolled code would arrive
@@ -648,6 +690,7 @@ __global__ void __launch_bounds__(kLdThreads, 1) latent_decode_kernel(const __gr
                 }
             }
             tc_fence_before();
+            if (odd) ld_broken_keys<T, LCH>(p, c, slot, live);
             c = nx;
         }
     done:;
@@ -680,6 +723,7 @@ __global__ void __launch_bounds__(D * KG) latent_merge_kernel(const __grid_const
     const int b = static_cast<int>(unit / p.groups), g = static_cast<int>(unit % p.groups);
     const int rows = p.T * p.H, row_in = g * 64 + quad * 4;
     if (row_in >= rows) return;
+    const int len = ld_len(p, b);  // an input of the launch before: no need to wait for it
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int2 u = p.ws_unit[unit];
     if (!ld_joinable(u.x, u.y, p.ctas)) return;
@@ -775,7 +819,7 @@ __global__ void __launch_bounds__(D * KG) latent_merge_kernel(const __grid_const
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         if (row_in + r >= rows) break;
-        const float inv = lv[r] > 0.f || lv[r] != lv[r] ? 1.f / lv[r] : 0.f;
+        const float inv = ld_inverse(lv[r], len - (p.T - 1 - (row_in + r) / p.H) > 0);
 #pragma unroll
         for (int k = 0; k < MBS; ++k) {
             const float a = r == 0 ? acc[k].x : r == 1 ? acc[k].y : r == 2 ? acc[k].z : acc[k].w;
@@ -866,6 +910,7 @@ extern "C" vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* 
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return fail(VK_INVALID_ARG, "workspace missing, too small or not 16-byte aligned");
     LdParams p;
+    p.base = pool->base + static_cast<uint64_t>(layer) * pool->seg_stride;
     p.ql = static_cast<const char*>(q_latent);
     p.qr = static_cast<const char*>(q_rope);
     p.ql_token = ql_token_stride;
