@@ -512,9 +512,11 @@ vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* q_latent, i
  * max_tokens and max_seq_len bound the longest chunk and the longest sequence
  * after it, on the host (they size the launches and the workspace); a sequence
  * beyond them, or beyond its table, records VK_ERR_SEQ_LEN and is left out.
- * workspace: vk_latent_prefill_workspace_size() bytes (512 a token and head, in
- * groups of heads of up to 1 GiB), 128-byte aligned; calls that may overlap on
- * the GPU need one each.  From ~170 new tokens a sequence on this does less work
+ * workspace: vk_latent_prefill_workspace_size() bytes, 128-byte aligned; calls
+ * that may overlap on the GPU need one each.  It holds 512 bytes a row of
+ * max_seq_len (rounded up to 128), sequence and head, for as many heads, or
+ * sequences of one head, as fit 1 GiB (one sequence's head at least), which then
+ * take turns, and 20 MB of partial results.  From ~170 new tokens a sequence on this does less work
  * than vk_latent_decode at latent_dim 512. */
 size_t    vk_latent_prefill_workspace_size(const vk_pool* pool, int32_t batch, int32_t max_seq_len, int32_t num_heads);
 vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void* q, int64_t q_token_stride,

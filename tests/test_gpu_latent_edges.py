@@ -9,7 +9,7 @@ import math
 import pytest
 import torch
 
-from .test_gpu_latent import Cache, gen, rnd
+from .test_gpu_latent import Cache, gen, prefill_check, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -191,3 +191,24 @@ def test_decode_rows_that_see_only_infinite_scores(vk):
     for b in (0, 2, 3):
         assert torch.isnan(out[b]).all() and (lse[b] == -math.inf).all()
     assert (out[1] == 0).all() and (lse[1] == -math.inf).all()
+
+
+# ------------------------------------------------------------------ groups of sequences
+
+
+def test_prefill_workspace_bound_and_groups_of_sequences(vk):
+    """Bounds so wide that one head of all sequences takes more than the workspace's 1 GiB: sequences go in groups."""
+    g = gen(91)
+    lens = torch.randint(1, 200, (37,), generator=g, device="cuda").tolist()
+    lens[3], lens[20] = 0, 300
+    new = [min(n, 1 + 7 * i % 150) for i, n in enumerate(lens)]
+    c = Cache(vk, lens, 128, 16, 64, layers=1, layer=0)
+    bound = 65536  # 37 * 65536 rows of 512 bytes: 1.16 GiB a head
+    c.tables = torch.cat([c.tables, torch.full((37, bound // 64 - c.tables.shape[1]), -1, dtype=torch.int32, device="cuda")], 1)
+    parts = c.pool.prefill_workspace_size(1, 1, 1) - 128 * 512
+    for batch, longest, heads in ((37, bound, 3), (37, bound, 1), (32, 131072, 40), (1000, 8192, 5), (65535, 128, 9), (4000, 1 << 20, 2)):
+        size = c.pool.prefill_workspace_size(batch, longest, heads)
+        assert 0 < size <= max(1 << 30, -(-longest // 128) * 128 * 512) + parts, (batch, longest, heads)
+    prefill_check(c, g, new, 3, max_tokens=150, max_seq_len=bound)
+    # without bounds: what the tables hold
+    prefill_check(c, g, new, 2)

@@ -59,9 +59,9 @@ struct LpParams {
     const int32_t* pos;
     const int32_t* offsets;  // NULL: tokens / B each
     uint32_t* err;
-    char* ws;     // [B * lpad][heads][256]
+    char* ws;     // [nb * lpad][heads][256]
     char* out;    // [tokens][H][128]
-    int bt_stride, B, tokens, H, heads, h0, layer, num_pages, P, latent, rope, lpad, max_tokens, max_len, stages, per_cta;
+    int bt_stride, B, b0, nb, tokens, H, heads, h0, layer, num_pages, P, latent, rope, lpad, max_tokens, max_len, stages, per_cta;
     int q_tiles, splits;   // attention: 256-row tiles of the longest chunk, key ranges a CTA's tile is cut into
     float* part_o;         // splits > 1: [q tile of (b, head)][split][256][128] unnormalised O
     float2* part_ml;       // and its (reference of the weights, their sum) [..][256]
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
     // the attention may start its launch: it reads what this kernel writes only behind
     // griddepcontrol.wait
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int b = blockIdx.z, key0 = blockIdx.y * kLeTokens;
+    const int bl = blockIdx.z, b = p.b0 + bl, key0 = blockIdx.y * kLeTokens;
     const LpSeq sq = lp_seq(p, b, threadIdx.x == 0 && blockIdx.x == 0 && key0 == 0 && p.h0 == 0);
     const int len = sq.pos + sq.n;
     if (sq.n == 0 || key0 >= len) return;
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kLeThreads, 1) latent_expand_kernel(const __gr
                 fence_async_smem();
                 asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + tile) : "memory");
                 if (r == 0 && ok) {
-                    tma_store_2d(&tmapkv, stage, hfirst * 256 + hh * 128 + c * 64, b * p.lpad + key0 + tile * kLpKeys);
+                    tma_store_2d(&tmapkv, stage, hfirst * 256 + hh * 128 + c * 64, bl * p.lpad + key0 + tile * kLpKeys);
                     bulk_commit();
                 }
             }
@@ -356,7 +356,8 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = SPLIT ? blockIdx.z / p.splits : blockIdx.z, split = SPLIT ? blockIdx.z % p.splits : 0, hl = blockIdx.y, h = p.h0 + hl;
+    const int bl = SPLIT ? blockIdx.z / p.splits : blockIdx.z, split = SPLIT ? blockIdx.z % p.splits : 0, hl = blockIdx.y;
+    const int b = p.b0 + bl, h = p.h0 + hl;
     const LpSeq sq = lp_seq(p, b, false);
     const int qt = p.q_tiles - 1 - static_cast<int>(blockIdx.x), q0 = qt * 2 * kLpRows;  // most keys first
     if (q0 >= sq.n) {  // (this grid must not end before the expansion does)
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
         // units 5j+3, 5j+4 those of tile j-1's first two K units
         if (lane == 0) {
             const uint64_t pol = l2_evict_last_policy();  // other row tiles read the same K and V
-            const int wrow = b * p.lpad + kt0 * kLpKeys, u = warp == 8 ? 0 : 1;
+            const int wrow = bl * p.lpad + kt0 * kLpKeys, u = warp == 8 ? 0 : 1;
             int landed = -1;  // the last tile whose K and V are on their way
             bool ok = true;
             asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -642,7 +643,7 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
                 l = l * alpha + (s0 + s1);
             }
         }
-        const int64_t part = SPLIT ? ((((static_cast<int64_t>(b) * p.heads + hl) * p.q_tiles + qt) * p.splits + split) * 256 + t * kLpRows + r) : 0;
+        const int64_t part = SPLIT ? ((((static_cast<int64_t>(bl) * p.heads + hl) * p.q_tiles + qt) * p.splits + split) * 256 + t * kLpRows + r) : 0;
         if (SPLIT) p.part_ml[part] = make_float2(m_ref, l);  // (-inf, 0) where no key is seen
         if (alive && ntt > 0 && wait_all(smem_u32(&o_full[t]), 0, p.err)) {
             tc_fence_after();
@@ -680,10 +681,10 @@ __global__ void __launch_bounds__(kLaThreads, 1) latent_prefill_kernel(const __g
 // Joins the key ranges of a query row: a warp per (row, head), four elements a lane.
 template <typename T>
 __global__ void __launch_bounds__(128) latent_prefill_merge_kernel(const __grid_constant__ LpParams p) {
-    const int lane = threadIdx.x & 31, b = blockIdx.z, hl = blockIdx.y, qrow = blockIdx.x * 4 + (threadIdx.x >> 5);
-    const LpSeq sq = lp_seq(p, b, false);
+    const int lane = threadIdx.x & 31, bl = blockIdx.z, hl = blockIdx.y, qrow = blockIdx.x * 4 + (threadIdx.x >> 5);
+    const LpSeq sq = lp_seq(p, p.b0 + bl, false);
     if (qrow >= sq.n) return;
-    const int64_t part0 = ((static_cast<int64_t>(b) * p.heads + hl) * p.q_tiles + (qrow >> 8)) * p.splits;
+    const int64_t part0 = ((static_cast<int64_t>(bl) * p.heads + hl) * p.q_tiles + (qrow >> 8)) * p.splits;
     float2 ml = make_float2(-INFINITY, 0.f);  // lane s: split s (at most 16)
     if (lane < p.splits) ml = p.part_ml[(part0 + lane) * 256 + (qrow & 255)];
     float m = ml.x;
@@ -707,17 +708,24 @@ __global__ void __launch_bounds__(128) latent_prefill_merge_kernel(const __grid_
     *reinterpret_cast<uint2*>(dst + lane * 8) = make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
 }
 
-// Heads whose keys and values the workspace holds at once: all, up to 1 GiB.
-constexpr uint64_t kLpWorkspace = 1ull << 30;
-constexpr int kLpMaxSplits = 16;
 // Partials of split query tiles: at most one CTA per SM.
+constexpr int kLpMaxSplits = 16;
 static size_t lp_part_bytes(const vk_pool* pool) { return static_cast<size_t>(pool->num_sms) * 256 * (kLpHead * 4 + 8); }
-static int lp_heads(int64_t rows, int H) {
-    const uint64_t per_head = static_cast<uint64_t>(rows) * 512;
-    const int64_t fit = static_cast<int64_t>(kLpWorkspace / per_head);
-    const int most = static_cast<int>(fit < 1 ? 1 : fit > H ? H : fit);
-    const int groups = (H + most - 1) / most;
-    return (H + groups - 1) / groups;  // even groups
+
+// What the workspace holds the keys and values of at once: as many heads of all
+// sequences as fit 1 GiB, else as many sequences' one head, one at least; in even groups.
+constexpr int64_t kLpWorkspace = 1ll << 30;
+struct LpGroup {
+    int heads, seqs;
+};
+static int64_t lp_pad(int32_t max_seq_len) { return (static_cast<int64_t>(max_seq_len) + kLpKeys - 1) / kLpKeys * kLpKeys; }
+static LpGroup lp_group(int64_t lpad, int B, int H) {
+    auto even = [](int n, int64_t most) {
+        const int groups = static_cast<int>((n + most - 1) / most);
+        return (n + groups - 1) / groups;
+    };
+    const int64_t fit = max(kLpWorkspace / (lpad * 512), static_cast<int64_t>(1));  // (sequence, head) pairs
+    return {even(H, max(fit / B, static_cast<int64_t>(1))), even(B, fit)};
 }
 
 template <typename T>
@@ -743,24 +751,24 @@ static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensor
     int64_t best = 0;
     p.per_cta = 1;
     for (int n = 1; n <= p.heads; ++n) {
-        const int64_t ctas = static_cast<int64_t>(p.B) * row_tiles * ((p.heads + n - 1) / n);
+        const int64_t ctas = static_cast<int64_t>(p.nb) * row_tiles * ((p.heads + n - 1) / n);
         const int64_t cost = (ctas + pool->num_sms - 1) / pool->num_sms * (10 * n + 6);
         if (n == 1 || cost < best) {
             best = cost;
             p.per_cta = n;
         }
     }
-    latent_expand_kernel<T><<<dim3((p.heads + p.per_cta - 1) / p.per_cta, row_tiles, p.B), kLeThreads, smem, st>>>(pool->tmap16, tw, tkv, p);
+    latent_expand_kernel<T><<<dim3((p.heads + p.per_cta - 1) / p.per_cta, row_tiles, p.nb), kLeThreads, smem, st>>>(pool->tmap16, tw, tkv, p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "latent_expand_kernel launch");
     // Too few CTAs for the GPU: each (query tile, head, sequence) is cut along its keys,
     // into ranges of six key tiles or more (200 new tokens behind 30k, 8 heads: 598 us
     // without, 134 with; 1,030 behind none in two ranges: 44 instead of 35).
     p.q_tiles = (p.max_tokens + 2 * kLpRows - 1) / (2 * kLpRows);
-    const int64_t base = static_cast<int64_t>(p.q_tiles) * p.heads * p.B;
+    const int64_t base = static_cast<int64_t>(p.q_tiles) * p.heads * p.nb;
     p.splits = static_cast<int>(max(static_cast<int64_t>(1), min(min(static_cast<int64_t>(kLpMaxSplits), pool->num_sms / base),
                                                                   static_cast<int64_t>(p.max_len / (6 * kLpKeys)))));
-    const dim3 grid(p.q_tiles, p.heads, p.B * p.splits);
+    const dim3 grid(p.q_tiles, p.heads, p.nb * p.splits);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -775,7 +783,7 @@ static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensor
                      : cudaLaunchKernelEx(&cfg, latent_prefill_kernel<T, false>, pool->tmap16, tq, tkv, p);
     if (e != cudaSuccess) return cuda_fail(e, "latent_prefill_kernel launch");
     if (p.splits > 1) {
-        latent_prefill_merge_kernel<T><<<dim3((p.max_tokens + 3) / 4, p.heads, p.B), 128, 0, st>>>(p);
+        latent_prefill_merge_kernel<T><<<dim3((p.max_tokens + 3) / 4, p.heads, p.nb), 128, 0, st>>>(p);
         e = cudaGetLastError();
         if (e != cudaSuccess) return cuda_fail(e, "latent_prefill_merge_kernel launch");
     }
@@ -788,9 +796,9 @@ using namespace vk;
 
 extern "C" size_t vk_latent_prefill_workspace_size(const vk_pool* pool, int32_t batch, int32_t max_seq_len, int32_t num_heads) {
     if (!pool || !is_latent(pool) || batch <= 0 || max_seq_len <= 0 || num_heads <= 0) return 0;
-    const int64_t rows = static_cast<int64_t>(batch) * ((static_cast<int64_t>(max_seq_len) + kLpKeys - 1) / kLpKeys * kLpKeys);
-    if (rows >= (1ll << 31)) return 0;
-    return static_cast<size_t>(rows) * 512 * lp_heads(rows, num_heads) + lp_part_bytes(pool);
+    const int64_t lpad = lp_pad(max_seq_len);
+    const LpGroup group = lp_group(lpad, batch, num_heads);
+    return static_cast<size_t>(lpad) * group.seqs * 512 * group.heads + lp_part_bytes(pool);
 }
 
 extern "C" vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -818,8 +826,8 @@ extern "C" vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void*
         return fail(VK_INVALID_ARG, "q, w_kv and out must be 16-byte aligned, strides multiples of 8");
     if (q_token_stride < 0 || q_head_stride < 0 || w_stride < pool->latent_dim)
         return fail(VK_INVALID_ARG, "q strides must be >= 0, w_stride >= latent_dim");
+    if (max_seq_len > 65535 * kLpKeys) return fail(VK_INVALID_ARG, "max_seq_len too large");
     const size_t need = vk_latent_prefill_workspace_size(pool, batch, max_seq_len, num_heads);
-    if (need == 0 || max_seq_len > 65535 * kLpKeys) return fail(VK_INVALID_ARG, "batch * max_seq_len too large");
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 127))
         return fail(VK_INVALID_ARG, "workspace missing, too small or not 128-byte aligned");
     LpParams p{};
@@ -838,14 +846,13 @@ extern "C" vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void*
     p.P = pool->cfg.page_tokens;
     p.latent = pool->latent_dim;
     p.rope = pool->rope_dim;
-    p.lpad = (max_seq_len + kLpKeys - 1) / kLpKeys * kLpKeys;
+    p.lpad = static_cast<int>(lp_pad(max_seq_len));
     p.max_tokens = max_tokens;
     p.max_len = max_seq_len;
     const int width = kLpHead + p.rope;
     p.scale_log2 = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(width))) * 1.4426950408889634f;
-    const int64_t rows = static_cast<int64_t>(batch) * p.lpad;
-    const int group = lp_heads(rows, num_heads);
-    p.part_o = reinterpret_cast<float*>(p.ws + static_cast<size_t>(rows) * 512 * group);
+    const LpGroup group = lp_group(p.lpad, batch, num_heads);
+    p.part_o = reinterpret_cast<float*>(p.ws + static_cast<size_t>(p.lpad) * group.seqs * 512 * group.heads);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(pool->num_sms) * 256 * kLpHead);
 
     const CUtensorMapDataType type = pool->kv_format == VK_KV_LATENT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -873,20 +880,23 @@ extern "C" vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void*
             return fail(VK_INVALID_ARG, "w_kv's shape or stride cannot be addressed by TMA");
     }
     DeviceGuard g(pool->device);
-    // the last group may have fewer heads; its rows keep its own pitch, so it has its own map
-    for (int h0 = 0; h0 < num_heads; h0 += group) {
-        p.h0 = h0;
-        p.heads = min(group, num_heads - h0);
-        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.heads) * 256, static_cast<cuuint64_t>(rows)};
-        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.heads) * 512};
-        const cuuint32_t box[2] = {64, kLpKeys};
-        if (encode(&tkv, type, 2, workspace, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-            return fail(VK_CUDA_ERROR, "cuTensorMapEncodeTiled failed for the workspace");
-        const vk_status s = pool->kv_format == VK_KV_LATENT_BF16
-                                ? launch_latent_prefill<__nv_bfloat16>(pool, p, tq, tw, tkv, as_stream(stream))
-                                : launch_latent_prefill<__half>(pool, p, tq, tw, tkv, as_stream(stream));
-        if (s != VK_OK) return s;
-    }
+    // the last groups may have fewer heads or sequences; rows keep their own pitch, so each has its own map
+    for (int b0 = 0; b0 < batch; b0 += group.seqs)
+        for (int h0 = 0; h0 < num_heads; h0 += group.heads) {
+            p.b0 = b0;
+            p.nb = min(group.seqs, batch - b0);
+            p.h0 = h0;
+            p.heads = min(group.heads, num_heads - h0);
+            const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.heads) * 256, static_cast<cuuint64_t>(p.nb) * p.lpad};
+            const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.heads) * 512};
+            const cuuint32_t box[2] = {64, kLpKeys};
+            if (encode(&tkv, type, 2, workspace, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+                return fail(VK_CUDA_ERROR, "cuTensorMapEncodeTiled failed for the workspace");
+            const vk_status s = pool->kv_format == VK_KV_LATENT_BF16
+                                    ? launch_latent_prefill<__nv_bfloat16>(pool, p, tq, tw, tkv, as_stream(stream))
+                                    : launch_latent_prefill<__half>(pool, p, tq, tw, tkv, as_stream(stream));
+            if (s != VK_OK) return s;
+        }
     return VK_OK;
 }
