@@ -388,7 +388,8 @@ vk_status vk_oproj_pack_weight_t16(const void* w_t, int32_t ldw, int32_t n, int3
  *   VK_ROTARY_BY_WAVELENGTH  the same two ends with
  *       t = original_len * f_i / (2 pi) turns: a blend (t - low) / (high - low)
  * magnitude > 0 replaces the factor on cos and sin (0: the scaling's own, 1
- * unless said above).  Angles are exact to fp32 at any int32 position. */
+ * unless said above).  At any int32 position an angle, less its whole turns, is off by
+ * at most 2^-29 rad before its rounding to fp32 (relative 2^-23). */
 #define VK_ROTARY_INTERLEAVED 0
 #define VK_ROTARY_HALF        1
 #define VK_ROTARY_PLAIN         0

@@ -137,37 +137,38 @@ static vk_status launch_rotary(const vk_rotary* r, const RotaryParams& p, bool v
     return e == cudaSuccess ? VK_OK : cuda_fail(e, "rotary_kernel launch");
 }
 
-// Angle per position of each pair, scaled for long contexts.
-static vk_status rotary_frequencies(const vk_rotary_cfg& c, double* f, double* magnitude) {
-    const double two_pi = 6.283185307179586476925286766559;
+// Angle per position of each pair, scaled for long contexts.  In long double (64 bits
+// of mantissa or more): at position 2^31 the 2^-53 of a double is 2^-22 rad.
+constexpr long double kTwoPi = 6.283185307179586476925286766559005768L;
+static vk_status rotary_frequencies(const vk_rotary_cfg& c, long double* f, double* magnitude) {
     const int n = c.rotary_dim / 2;
-    for (int i = 0; i < n; ++i) f[i] = std::pow(c.theta_base, -2.0 * i / c.rotary_dim);
+    const long double theta = c.theta_base, factor = c.factor, original_len = c.original_len, low = c.low, high = c.high;
+    for (int i = 0; i < n; ++i) f[i] = std::pow(theta, -2.0L * i / c.rotary_dim);
     *magnitude = c.magnitude > 0 ? c.magnitude : 1.0;
     if (c.scaling == VK_ROTARY_LINEAR) {
-        for (int i = 0; i < n; ++i) f[i] /= c.factor;
+        for (int i = 0; i < n; ++i) f[i] /= factor;
     } else if (c.scaling == VK_ROTARY_BY_PARTS) {
         // the pair that makes `turns` turns within original_len positions
-        auto pair_of = [&](double turns) {
-            return c.rotary_dim * std::log(c.original_len / (turns * two_pi)) / (2.0 * std::log(c.theta_base));
+        auto pair_of = [&](long double turns) {
+            return c.rotary_dim * std::log(original_len / (turns * kTwoPi)) / (2.0L * std::log(theta));
         };
         // the ramp may end behind the last pair: cut there, it would give pairs that make
         // more than `low` turns the whole factor
-        const double last = std::min(std::ceil(pair_of(c.low)), static_cast<double>(c.rotary_dim - 1));
-        const double first = std::min(std::max(std::floor(pair_of(c.high)), 0.0), last);
+        const long double last = std::min(std::ceil(pair_of(low)), static_cast<long double>(c.rotary_dim - 1));
+        const long double first = std::min(std::max(std::floor(pair_of(high)), 0.0L), last);
         for (int i = 0; i < n; ++i) {
-            const double ramp = std::min(std::max((i - first) / std::max(last - first, 0.001), 0.0), 1.0);
-            f[i] = f[i] * (1.0 - ramp) + f[i] / c.factor * ramp;
+            const long double ramp = std::min(std::max((i - first) / std::max(last - first, 0.001L), 0.0L), 1.0L);
+            f[i] = f[i] * (1.0L - ramp) + f[i] / factor * ramp;
         }
         if (!(c.magnitude > 0)) *magnitude = c.factor > 1.0 ? 0.1 * std::log(c.factor) + 1.0 : 1.0;
     } else if (c.scaling == VK_ROTARY_BY_WAVELENGTH) {
         for (int i = 0; i < n; ++i) {
-            const double blend =
-                std::min(std::max((c.original_len * f[i] / two_pi - c.low) / (c.high - c.low), 0.0), 1.0);
-            f[i] = (1.0 - blend) * f[i] / c.factor + blend * f[i];
+            const long double blend = std::min(std::max((original_len * f[i] / kTwoPi - low) / (high - low), 0.0L), 1.0L);
+            f[i] = (1.0L - blend) * f[i] / factor + blend * f[i];
         }
     }
     for (int i = 0; i < n; ++i)
-        if (!(f[i] >= 0.0) || f[i] >= 3.0) return fail(VK_INVALID_ARG, "rotary: a frequency is outside [0, 3) rad per position");
+        if (!(f[i] >= 0.0L) || f[i] >= 3.0L) return fail(VK_INVALID_ARG, "rotary: a frequency is outside [0, 3) rad per position");
     return VK_OK;
 }
 
@@ -207,7 +208,8 @@ extern "C" vk_status vk_rotary_create(const vk_rotary_cfg* cfg, vk_rotary** out)
     *out = nullptr;
     vk_status s = check_rotary_cfg(cfg);
     if (s != VK_OK) return s;
-    double f[kRotaryMaxPairs], magnitude = 1.0;
+    long double f[kRotaryMaxPairs];
+    double magnitude = 1.0;
     s = rotary_frequencies(*cfg, f, &magnitude);
     if (s != VK_OK) return s;
     auto* r = new (std::nothrow) vk_rotary();
@@ -217,7 +219,7 @@ extern "C" vk_status vk_rotary_create(const vk_rotary_cfg* cfg, vk_rotary** out)
     r->table.half = cfg->layout == VK_ROTARY_HALF;
     r->table.magnitude = static_cast<float>(magnitude);
     for (int i = 0; i < r->table.pairs; ++i)  // f / (2 pi) < 1/2: the scaled value fits 63 bits
-        r->table.turn[i] = static_cast<uint64_t>(std::llround(std::ldexp(f[i] / 6.283185307179586476925286766559, 64)));
+        r->table.turn[i] = static_cast<uint64_t>(std::llround(std::ldexp(f[i] / kTwoPi, 64)));
     *out = r;
     return VK_OK;
 }
@@ -231,7 +233,11 @@ extern "C" vk_status vk_rotary_frequencies(const vk_rotary_cfg* cfg, double* out
     vk_status s = check_rotary_cfg(cfg);
     if (s != VK_OK) return s;
     if (!out || !magnitude) return fail(VK_INVALID_ARG, "NULL array");
-    return rotary_frequencies(*cfg, out, magnitude);
+    long double f[kRotaryMaxPairs];
+    s = rotary_frequencies(*cfg, f, magnitude);
+    if (s != VK_OK) return s;
+    for (int i = 0; i < cfg->rotary_dim / 2; ++i) out[i] = static_cast<double>(f[i]);
+    return VK_OK;
 }
 
 extern "C" vk_status vk_rotary_apply(const vk_rotary* r, int32_t dtype, const vk_rotary_view* q, const vk_rotary_view* k,
