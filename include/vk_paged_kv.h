@@ -453,7 +453,8 @@ vk_status vk_latent_pool_create(const vk_latent_cfg* cfg, void* device_mem, size
 
 /* Appends `tokens` new tokens of `batch` sequences.  Token rows come
  * concatenated; offsets (int32 [batch+1], device) gives sequence b the rows
- * offsets[b]..offsets[b+1]-1 (rows behind offsets[batch] are ignored); NULL:
+ * offsets[b]..offsets[b+1]-1 (rows before offsets[0] and behind offsets[batch]
+ * are ignored); NULL:
  * tokens / batch rows each.  Row offsets[b]+i is written to position
  * positions[b]+i of sequence b.
  * latent, k_rope: the pool's type, row strides in elements (two views of one
@@ -502,7 +503,7 @@ vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* q_latent, i
  * token i of sequence b sits at positions[b]+i and sees rows 0..positions[b]+i.
  *   out = sum_j softmax_j(scale * q . k_j) v_j,   scale 0: 1/sqrt(128 + rope_dim)
  * Token rows come concatenated, with offsets as in vk_latent_append; rows
- * behind offsets[batch] are left as they were.  q: [tokens, num_heads, 128 +
+ * of no sequence are left as they were.  q: [tokens, num_heads, 128 +
  * rope_dim] by strides in elements, its last rope_dim elements rotated already;
  * w_kv: [num_heads * 256, latent_dim], row stride w_stride, per head the 128
  * rows of W_k,h, then the 128 of W_v,h (an [out, in] projection weight as it

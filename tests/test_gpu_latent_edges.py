@@ -212,3 +212,33 @@ def test_prefill_workspace_bound_and_groups_of_sequences(vk):
     prefill_check(c, g, new, 3, max_tokens=150, max_seq_len=bound)
     # without bounds: what the tables hold
     prefill_check(c, g, new, 2)
+
+
+# ------------------------------------------------------------------ offsets of a part of a batch
+
+
+def test_offsets_of_a_part_of_a_batch(vk):
+    """offsets[k:k+n+1] of a larger batch: the rows of the sequences before and behind are ignored, by the append and by
+    the prefill, and nothing is recorded."""
+    g = gen(95)
+    c = Cache(vk, [40, 30, 70], layers=1, layer=0)
+    new = [3, 20, 5]
+    cu = torch.tensor([0, 7, 10, 30, 35, 36], dtype=torch.int32, device="cuda")  # sequences 1..3 of 5
+    start = c.seq_lens - torch.tensor(new, dtype=torch.int32, device="cuda")
+    kv = rnd(g, 36, 576)
+    before = c.pool.latent_view().clone()
+    c.pool.append(0, kv[:, :512], kv[:, 512:], c.tables, start, offsets=cu[1:5])
+    assert c.check() == 0
+    for b in range(3):
+        rows = kv[int(cu[b + 1]):int(cu[b + 2])]
+        for i in range(new[b]):
+            pos = int(start[b]) + i
+            before[0, int(c.tables[b, pos // 16]), pos % 16] = rows[i]
+    assert torch.equal(c.pool.latent_view().view(torch.int16), before.view(torch.int16))
+    q, w = rnd(g, 36, 2, 192), rnd(g, 512, 512, std=512 ** -0.5)
+    out = torch.full((36, 2, 128), 9.0, device="cuda").half()
+    c.pool.prefill(0, q, w, c.tables, start, offsets=cu[1:5], max_tokens=20, max_seq_len=70, out=out)
+    assert c.check() == 0
+    assert (out[:7] == 9).all() and (out[35:] == 9).all()
+    want = c.pool.prefill(0, q[7:35].contiguous(), w, c.tables, start, offsets=cu[1:5] - 7, max_tokens=20, max_seq_len=70)
+    assert torch.equal(out[7:35], want)

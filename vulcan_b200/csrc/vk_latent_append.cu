@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kLaWarps * 32, 64 / kLaWarps) latent_append_ke
     int b, first, start;
     if (p.offsets) {
         b = sequence_of(p.offsets, p.pos, p.B, static_cast<int>(row), lane, &first, &start);
-        if (b < 0) return;
+        if (b < 0 || (b == 0 && row < first)) return;  // a row of no sequence
     } else {
         const int per = p.tokens / p.B;
         b = static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(per));
