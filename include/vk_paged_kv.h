@@ -409,7 +409,8 @@ typedef struct vk_rotary_cfg {
 /* One tensor: element (token, head, d) is x[token*x_token + head*x_head + d]
  * (strides in elements); the result goes to y likewise.  y may be x with equal
  * strides (in place), and may not overlap x otherwise; rows of y may not share
- * elements (a broadcast tensor is not rotated in place). */
+ * elements (a broadcast tensor is not rotated in place), nor may y of one of q
+ * and k overlap x or y of the other. */
 typedef struct vk_rotary_view {
     const void* x;
     void*       y;

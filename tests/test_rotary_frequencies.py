@@ -1,4 +1,5 @@
-"""CPU tests of vk_rotary_frequencies against formulas written apart from the library."""
+"""CPU tests of the rotary entry points: frequencies against formulas written apart from the library, and calls whose
+tensors coincide."""
 import ctypes
 import math
 
@@ -51,3 +52,24 @@ def test_by_parts_ends_outside_the_pairs(lib, original, share):
     for i, f in enumerate(got):
         plain = 1e4 ** (-2.0 * i / 64)
         assert abs(f / (plain / 8.0 if share else plain) - 1) < 1e-13, i
+
+
+def test_one_tensor_as_q_and_k_is_refused_as_an_output(lib):
+    """Where one view's output is the other's input or output, both rotate the same elements."""
+    out = ctypes.c_void_p()
+    cfg = _lib.VkRotaryCfg(64, 0, 0, 0, 10000.0, 1.0, 0.0, 1.0, 32.0, 0.0)
+    assert lib.vk_rotary_create(ctypes.byref(cfg), ctypes.byref(out)) == _lib.VK_OK
+    a, b, c, d = 0x10000, 0x20000, 0x30000, 0x40000  # addresses that no refused call touches
+
+    def refused(q, k, heads=2, tokens=3):
+        views = [_lib.VkRotaryView(x, y, 128, 64, 128, 64, heads) for x, y in (q, k)]
+        # without positions a call that passes is refused for that instead
+        status = lib.vk_rotary_apply(out, 0, views[0], views[1], 64, None, tokens, None)
+        assert status == (_lib.VK_INVALID_ARG if tokens and heads else _lib.VK_OK)
+        return b"q and k" in lib.vk_last_error_string()
+
+    for q, k in (((a, a), (a, a)), ((a, c), (b, c)), ((a, b), (b, d)), ((a, c), (b, a)), ((a, a), (a, c)), ((a, b), (b, b)), ((a, b), (b, a))):
+        assert refused(q, k), (q, k)
+    for q, k in (((a, a), (b, b)), ((a, c), (b, d)), ((a, c), (a, d)), ((a, a), (b, d))):
+        assert not refused(q, k), (q, k)
+    lib.vk_rotary_destroy(out)

@@ -273,6 +273,8 @@ extern "C" vk_status vk_rotary_apply(const vk_rotary* r, int32_t dtype, const vk
         heads += v->heads;
     }
     if (tokens == 0 || heads == 0) return VK_OK;
+    if (p.v[0].heads && p.v[1].heads && (p.v[0].y == p.v[1].y || p.v[0].y == p.v[1].x || p.v[1].y == p.v[0].x))
+        return fail(VK_INVALID_ARG, "an output may not be a tensor of the other of q and k");
     if (!positions) return fail(VK_INVALID_ARG, "NULL array");
     if (vec) {
         p.rotated = rotary_dim / n / (r->table.half ? 2 : 1);
