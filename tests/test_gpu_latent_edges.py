@@ -242,3 +242,42 @@ def test_offsets_of_a_part_of_a_batch(vk):
     assert (out[:7] == 9).all() and (out[35:] == 9).all()
     want = c.pool.prefill(0, q[7:35].contiguous(), w, c.tables, start, offsets=cu[1:5] - 7, max_tokens=20, max_seq_len=70)
     assert torch.equal(out[7:35], want)
+
+
+# ------------------------------------------------------------------ host threads
+
+
+def test_calls_from_host_threads(vk):
+    """Four host threads, a stream each, call every entry point of one pool at once."""
+    import threading
+    g = gen(97)
+    c = Cache(vk, [300, 70], 384, 48, 32, layers=5, layer=0)
+    view = c.pool.latent_view()
+    view[1:] = 0
+    ql, qr = rnd(g, 2, 1, 8, 384, std=0.5), rnd(g, 2, 1, 8, 48)
+    q, w, kv = rnd(g, 2, 20, 3, 176), rnd(g, 3 * 256, 384, std=384 ** -0.5), rnd(g, 40, 432)
+    rope = vk.RotaryEmbedding(48, layout="half")
+    want = c.pool.decode(0, ql, qr, c.tables, c.seq_lens, 0.07), c.pool.prefill(0, q, w, c.tables, c.seq_lens - 20)
+    torch.cuda.synchronize()
+    got, failed = [], []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            for _ in range(5):
+                c.pool.append(1 + i, kv[:, :384], kv[:, 384:], c.tables, c.seq_lens - 20, rope=rope, stream=s)
+                got.append((c.pool.decode(0, ql, qr, c.tables, c.seq_lens, 0.07, stream=s),
+                            c.pool.prefill(0, q, w, c.tables, c.seq_lens - 20, stream=s)))
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001 - reported below
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and c.check() == 0
+    assert all(torch.equal(a, want[0]) and torch.equal(b, want[1]) for a, b in got)
+    for i in range(1, 4):
+        assert torch.equal(view[1].view(torch.int16), view[1 + i].view(torch.int16))

@@ -55,6 +55,8 @@
 // key gets its NaN through S where the score is +inf or NaN; a score of -inf is a
 // weight of 0, and 0 * inf is NaN in the infinite element alone, as in a tile that all
 // rows see: those elements are written behind the output (ld_broken_keys).
+#include <atomic>
+
 #include "vk_internal.h"
 #include "vk_latent.cuh"
 #include "vk_latent_deal.h"
@@ -834,14 +836,14 @@ static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 template <typename T, int LCH>
 static vk_status launch_latent_decode(vk_pool* pool, const LdParams& p, cudaStream_t st) {
-    static uint64_t attr_set = 0;
+    static std::atomic<uint64_t> attr_set{0};  // a bit per device; host threads may call at once
     const uint64_t bit = 1ull << (pool->device & 63);
     const size_t smem = static_cast<size_t>(p.stages + 1) * p.nch * kLdChunk + kLdChunk + kLdAux + 1024;
     cudaError_t e = cudaSuccess;
-    if (!(attr_set & bit)) {
+    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
         e = cudaFuncSetAttribute(latent_decode_kernel<T, LCH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLdSmemMax);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(latent_decode)");
-        attr_set |= bit;
+        attr_set.fetch_or(bit, std::memory_order_release);
     }
     latent_decode_kernel<T, LCH><<<p.ctas, kLdThreads, smem, st>>>(pool->tmap16, p);
     e = cudaGetLastError();

@@ -40,6 +40,8 @@
 // every barrier and commit between them.  Not kept: a share of the exponentials by a
 // polynomial on the FMA pipe (no gain), two issuing threads (16% slower), waiting for
 // the next tile's loads between the halves of P V (3% slower).
+#include <atomic>
+
 #include "vk_internal.h"
 #include "vk_latent.cuh"
 #include "vk_ptx.cuh"
@@ -731,16 +733,16 @@ static LpGroup lp_group(int64_t lpad, int B, int H) {
 template <typename T>
 static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensorMap& tq, const CUtensorMap& tw, const CUtensorMap& tkv,
                                        cudaStream_t st) {
-    static uint64_t attr_set = 0;
+    static std::atomic<uint64_t> attr_set{0};  // a bit per device; host threads may call at once
     const uint64_t bit = 1ull << (pool->device & 63);
-    if (!(attr_set & bit)) {
+    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
         cudaError_t e = cudaFuncSetAttribute(latent_expand_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLpSmemMax);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(latent_prefill_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLaSmem);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(latent_prefill_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLaSmem);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(latent prefill)");
-        attr_set |= bit;
+        attr_set.fetch_or(bit, std::memory_order_release);
     }
     const int lch = p.latent / 64;
     p.stages = min(kLeMaxStages, (kLpSmemMax - 2048 - lch * kLpUnit) / kLeStage - 2);  // 4, 6, 8, 10 at 512 .. 128
