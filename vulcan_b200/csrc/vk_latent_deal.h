@@ -13,18 +13,15 @@
 
 namespace vk {
 
-// Least cost of a CTA's range (1 x 200 tokens: 12.5 us with 1, 14.7 with 4: tiles in
-// parallel and a merge beat tiles in turn)
-constexpr int kLdMinRange = 1;
-
-// n CTAs share `total`: the first `rem` take q + 1, the others q.  (64-bit
-// divisions cost hundreds of cycles of every launch; totals below 2^32 need none.)
+// n CTAs share `total`: the first `rem` take q + 1, the others q; a range may be a
+// single tile (1 x 200 tokens: 12.5 us so, 14.7 with four at least: tiles in parallel
+// and a merge beat tiles in turn).  (64-bit divisions cost hundreds of cycles of every
+// launch; totals below 2^32 need none.)
 struct LdDeal {
     int64_t q, rem;
     int n;
     VK_HD LdDeal(int64_t total, int ctas) {
-        const int64_t most = (total + kLdMinRange - 1) / kLdMinRange;
-        n = static_cast<int>(ctas < most ? ctas : most);
+        n = static_cast<int>(ctas < total ? ctas : total);
         q = div(total, n);
         rem = total - q * n;
     }

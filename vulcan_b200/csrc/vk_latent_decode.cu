@@ -939,7 +939,7 @@ extern "C" vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* 
     p.rope = pool->rope_dim;
     p.nch = p.latent / 64 + 1;
     const int stage = p.nch * kLdChunk;
-    p.stages = (kLdSmemMax - 1024 - kLdAux - kLdChunk - stage) / stage;  // 2, 2, 4, 7 at 512, 384, 256, 128
+    p.stages = (kLdSmemMax - 1024 - kLdAux - kLdChunk - stage) / stage;  // 2, 2, 4, 8 at 512, 384, 256, 128
     if (p.stages > kLdMaxStages) p.stages = kLdMaxStages;
     p.scale_log2 = scale * 1.4426950408889634f;
     const size_t slots = 2 * static_cast<size_t>(pool->num_sms);
