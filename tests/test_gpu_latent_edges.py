@@ -9,7 +9,7 @@ import math
 import pytest
 import torch
 
-from .test_gpu_latent import Cache, gen, prefill_check, rnd
+from .test_gpu_latent import Cache, decode_bound_check, gen, prefill_check, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -281,3 +281,18 @@ def test_calls_from_host_threads(vk):
     assert all(torch.equal(a, want[0]) and torch.equal(b, want[1]) for a, b in got)
     for i in range(1, 4):
         assert torch.equal(view[1].view(torch.int16), view[1 + i].view(torch.int16))
+
+
+# ------------------------------------------------------------------ more heads than a unit's rows
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,tokens", [([30000], 1), ([9000, 20011, 64, 1, 12345], 1), ([4000, 7001], 2)])
+def test_decode_128_heads_over_long_contexts(vk, dtype, lens, tokens):
+    g = gen(len(lens) + 200)
+    c = Cache(vk, lens, page=64, layers=1, layer=0, dtype=dtype)
+    n = len(lens)
+    ql, qr = rnd(g, n, tokens, 128, 512, dtype=dtype, std=0.5), rnd(g, n, tokens, 128, 64, dtype=dtype)
+    out, lse = c.pool.decode(0, ql, qr, c.tables, c.seq_lens, scale=0.07, return_lse=True)
+    assert c.check() == 0
+    decode_bound_check(c, ql, qr, out, lse, 0.07, tokens)
