@@ -296,3 +296,30 @@ def test_decode_128_heads_over_long_contexts(vk, dtype, lens, tokens):
     out, lse = c.pool.decode(0, ql, qr, c.tables, c.seq_lens, scale=0.07, return_lse=True)
     assert c.check() == 0
     decode_bound_check(c, ql, qr, out, lse, 0.07, tokens)
+
+
+# ------------------------------------------------------------------ pools, and calls with nothing in them
+
+
+def test_a_new_pool_is_zero_before_any_stream_uses_it(vk):
+    """Memory of the library's own: the zero fill is over when the pool is there, also for a stream that waits for nothing."""
+    g = gen(98)
+    kv = rnd(g, 64, 576)
+    p = torch.zeros(64, dtype=torch.int32, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    pages = (12 << 30) // (16 * 576 * 2)
+    tables = torch.arange(pages - 64, pages, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    ql, qr = rnd(g, 64, 8, 512), rnd(g, 64, 8, 64)
+    torch.cuda.synchronize()
+    small = vk.LatentKVPool(1, 512, 64, 64)
+    small.append(0, kv[:, :512], kv[:, 512:], tables - (pages - 64), p)
+    want = small.decode(0, ql, qr, tables - (pages - 64), p + 1, 0.07)
+    torch.cuda.synchronize()
+    pool = vk.LatentKVPool(1, 512, 64, pages, own_memory=True)
+    pool.append(0, kv[:, :512], kv[:, 512:], tables, p, stream=s)
+    s.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(pool.decode(0, ql, qr, tables, p + 1, 0.07), want)
+    assert pool.check() == 0
+    pool.close()

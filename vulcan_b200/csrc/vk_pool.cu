@@ -211,6 +211,10 @@ static vk_status finish_create(vk_pool* p, vk_pool** out) {
         vk_status s = make_latent_tmap(p);
         if (s != VK_OK) return s;
     }
+    // the fills above are asynchronous: a stream that does not wait for the default one may
+    // use the pool as soon as the caller has it
+    e = cudaStreamSynchronize(cudaStreamLegacy);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaStreamSynchronize(pool)");
     p->alloc.reset(p->num_pages);
     *out = p;
     return VK_OK;
