@@ -323,3 +323,15 @@ def test_a_new_pool_is_zero_before_any_stream_uses_it(vk):
     assert torch.equal(pool.decode(0, ql, qr, tables, p + 1, 0.07), want)
     assert pool.check() == 0
     pool.close()
+
+
+def test_batches_without_tokens(vk):
+    """[batch, 0, heads, d]: nothing to do, in every entry point that takes batches."""
+    c = Cache(vk, [40, 20])
+    empty = lambda heads, d: torch.empty(2, 0, heads, d, device="cuda").half()  # noqa: E731
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    assert vk.RotaryEmbedding(64).apply(empty(3, 64), none).shape == (2, 0, 3, 64)
+    out, lse = c.pool.decode(0, empty(4, 512), empty(4, 64), c.tables, c.seq_lens, 0.1, return_lse=True)
+    assert out.shape == (2, 0, 4, 512) and lse.shape == (2, 0, 4)
+    assert c.pool.prefill(0, empty(3, 192), rnd(gen(1), 768, 512), c.tables, c.seq_lens).shape == (2, 0, 3, 128)
+    assert c.check() == 0

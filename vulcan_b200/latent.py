@@ -93,7 +93,7 @@ def _token_head(t: torch.Tensor, name: str) -> Tuple[int, int]:
         return s[0], s[1]
     if shape[1] == 1:
         return s[0], s[2]
-    if shape[0] > 1 and s[0] != s[1] * shape[1]:
+    if s[0] != s[1] * shape[1] and shape[0] > 1 and shape[1]:
         raise ValueError("%s: the batches of a 4-D view must follow one another (stride 0 = stride 1 * tokens)" % name)
     return s[1], s[2]
 
