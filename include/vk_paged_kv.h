@@ -513,8 +513,10 @@ vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* q_latent, i
  * its range: to its largest number); a NaN or infinite latent reaches the rows that
  * see it, as NaN, and no others.
  * max_tokens and max_seq_len bound the longest chunk and the longest sequence
- * after it, on the host (they size the launches and the workspace); a sequence
- * beyond them, or beyond its table, records VK_ERR_SEQ_LEN and is left out.
+ * after it (8,388,480 at most), on the host; a sequence beyond them, or beyond
+ * its table, records VK_ERR_SEQ_LEN and is left out.  They size the launches and
+ * the workspace, so give tight ones: CTAs, and workspace, are there for chunks and
+ * sequences as long as the bounds say.
  * workspace: vk_latent_prefill_workspace_size() bytes, 128-byte aligned; calls
  * that may overlap on the GPU need one each.  It holds 512 bytes a row of
  * max_seq_len (rounded up to 128), sequence and head, for as many heads, or

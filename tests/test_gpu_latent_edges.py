@@ -335,3 +335,16 @@ def test_batches_without_tokens(vk):
     assert out.shape == (2, 0, 4, 512) and lse.shape == (2, 0, 4)
     assert c.pool.prefill(0, empty(3, 192), rnd(gen(1), 768, 512), c.tables, c.seq_lens).shape == (2, 0, 3, 128)
     assert c.check() == 0
+
+
+def test_bounds_beyond_the_prefill_are_refused_before_memory_is_taken(vk):
+    """Tables wider than the longest sequence that a call takes, without a bound: refused, not an allocation of terabytes."""
+    c = Cache(vk, [40], 128, 16, 64)
+    q, w = rnd(gen(2), 1, 8, 2, 144), rnd(gen(3), 512, 128)
+    wide = torch.full((1, 1 << 22), -1, dtype=torch.int32, device="cuda")
+    wide[0, 0] = c.tables[0, 0]
+    assert c.pool.prefill_workspace_size(1, (1 << 22) * 64, 2) == 0
+    with pytest.raises(vk.VKError, match="max_seq_len"):
+        c.pool.prefill(1, q, w, wide, c.seq_lens - 8)
+    got = c.pool.prefill(1, q, w, wide, c.seq_lens - 8, max_seq_len=40)
+    assert torch.equal(got, c.pool.prefill(1, q, w, c.tables, c.seq_lens - 8, max_seq_len=40)) and c.check() == 0

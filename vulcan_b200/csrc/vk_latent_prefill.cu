@@ -717,6 +717,7 @@ static size_t lp_part_bytes(const vk_pool* pool) { return static_cast<size_t>(po
 // What the workspace holds the keys and values of at once: as many heads of all
 // sequences as fit 1 GiB, else as many sequences' one head, one at least; in even groups.
 constexpr int64_t kLpWorkspace = 1ll << 30;
+constexpr int kLpMaxLen = 65535 * kLpKeys;  // (row tiles are a grid's y)
 struct LpGroup {
     int heads, seqs;
 };
@@ -797,7 +798,7 @@ static vk_status launch_latent_prefill(vk_pool* pool, LpParams p, const CUtensor
 using namespace vk;
 
 extern "C" size_t vk_latent_prefill_workspace_size(const vk_pool* pool, int32_t batch, int32_t max_seq_len, int32_t num_heads) {
-    if (!pool || !is_latent(pool) || batch <= 0 || max_seq_len <= 0 || num_heads <= 0) return 0;
+    if (!pool || !is_latent(pool) || batch <= 0 || max_seq_len <= 0 || max_seq_len > kLpMaxLen || num_heads <= 0) return 0;
     const int64_t lpad = lp_pad(max_seq_len);
     const LpGroup group = lp_group(lpad, batch, num_heads);
     return static_cast<size_t>(lpad) * group.seqs * 512 * group.heads + lp_part_bytes(pool);
@@ -828,7 +829,7 @@ extern "C" vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void*
         return fail(VK_INVALID_ARG, "q, w_kv and out must be 16-byte aligned, strides multiples of 8");
     if (q_token_stride < 0 || q_head_stride < 0 || w_stride < pool->latent_dim)
         return fail(VK_INVALID_ARG, "q strides must be >= 0, w_stride >= latent_dim");
-    if (max_seq_len > 65535 * kLpKeys) return fail(VK_INVALID_ARG, "max_seq_len too large");
+    if (max_seq_len > kLpMaxLen) return fail(VK_INVALID_ARG, "max_seq_len too large");
     const size_t need = vk_latent_prefill_workspace_size(pool, batch, max_seq_len, num_heads);
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 127))
         return fail(VK_INVALID_ARG, "workspace missing, too small or not 128-byte aligned");
