@@ -36,9 +36,10 @@
 // largest weight among fp16's subnormals (struct Weights); the sum of the weights is
 // taken from the unrounded fp32 values.
 //
-// Measured, 512 + 64, 64 rows: 24 sequences of ~16k tokens 89 us, 0.75 of the
-// measured copy rate (under the 1000 W cap in a long run, at 1.70 GHz, 100 us); in
-// between a CTA takes a 64-key tile in 2,980 cycles, which is 7.2 TB/s at 1.965 GHz.
+// Measured, 512 + 64, 64 rows: 24 sequences of ~16k tokens 89 us at 1.965 GHz, 0.75 of
+// the measured copy rate, and 107 us in a long run, where the 1000 W cap leaves 1.62 GHz:
+// the time follows the SM clock.  Between its ends a CTA takes a 64-key tile in 2,980
+// cycles (7.2 TB/s at 1.965 GHz), and those cycles bound it.
 // 64 x ~2k tokens 49 us, 0.53: the merge kernel takes 6-7 us of that, a CTA's start
 // (lengths, queries, first pages, first tile) 12,000 cycles and a change of units
 // 10,500, of which half is the next queries waiting behind the tiles in flight.

@@ -30,8 +30,8 @@
 //    of whole 32 + 16 KiB tiles would not fit twice beside 96 KiB of queries;
 //    units let the next K load while the last V is read.
 //
-// Measured, 512 + 64, 32 heads: 8 chunks of 2048 tokens 498 us (about 600 in a long run
-// under the 1000 W cap), 141 of them the expansion and 357 the attention.  The
+// Measured, 512 + 64, 32 heads: 8 chunks of 2048 tokens 500 us (596 in a long run
+// under the 1000 W cap, at 1.62 GHz), 141 of them the expansion and 359 the attention.  The
 // expansion is bound by shared memory: a stage of 64 latent elements takes 660 cycles,
 // 640 of them reads of operands at 128 bytes a cycle.  A step of the attention (a key
 // tile against two row tiles) takes ~3,700 cycles, 2,300 to 2,560 of them MMAs: each row

@@ -134,7 +134,7 @@ class RotaryEmbedding:
               out: Optional[torch.Tensor] = None, out_k: Optional[torch.Tensor] = None, stream=None):
         """q, k: [tokens, heads, D] (or [batch, tokens, heads, D]) fp16, bf16 or fp32, strided views allowed;
         positions: int32, one per token.  Returns the rotated q, or (q, k).  ``out``/``out_k`` may be q/k
-        themselves: rotated in place."""
+        themselves: rotated in place (``out`` may not be k, nor ``out_k`` q)."""
         dev, index = self.device, self._index
         dtype, shape = q.dtype, q.shape
         if dtype not in DTYPES:
@@ -226,7 +226,8 @@ class LatentKVPool(PagedKVPool):
                positions: torch.Tensor, offsets: Optional[torch.Tensor] = None, norm_weight: Optional[torch.Tensor] = None,
                eps: float = 1e-6, rope: Optional[RotaryEmbedding] = None, stream=None) -> None:
         """latent [tokens, latent_dim], k_rope [tokens, rope_dim] (row-strided views); sequence b takes the rows
-        offsets[b]..offsets[b+1]-1 (None: the same number each) from position positions[b] on.  ``norm_weight``: root
+        offsets[b]..offsets[b+1]-1 (None: the same number each; rows of no sequence are ignored) from position
+        positions[b] on.  ``norm_weight``: root
         mean square norm of the latent first; ``rope``: k_rope rotated at its position."""
         index, dtype = self._index, self.dtype
         batch, width = _tables(block_tables, index)
@@ -305,8 +306,8 @@ class LatentKVPool(PagedKVPool):
         views allowed), w_kv [H*256, latent_dim]: per head 128 rows of the key and 128 of the value up-projection.
         Sequence b's rows are offsets[b]..offsets[b+1]-1 (None: the same number each), from position positions[b] on.
         ``max_tokens`` bounds the longest chunk (default: without offsets the chunk, with them all tokens),
-        ``max_seq_len`` the longest sequence after the chunk (default: what the tables hold).  Returns
-        [..., H, 128]."""
+        ``max_seq_len`` the longest sequence after the chunk (default: what the tables hold).  Launches and
+        workspace are sized by them: give both where the tables are wide.  Returns [..., H, 128]."""
         dev, index = self.device, self._index
         batch, width = _tables(block_tables, index)
         _on(q, self.dtype, "q", index)
