@@ -521,8 +521,8 @@ vk_status vk_latent_decode(vk_pool* pool, int32_t layer, const void* q_latent, i
  * that may overlap on the GPU need one each.  It holds 512 bytes a row of
  * max_seq_len (rounded up to 128), sequence and head, for as many heads, or
  * sequences of one head, as fit 1 GiB (one sequence's head at least), which then
- * take turns, and 20 MB of partial results.  From ~170 new tokens a sequence on this does less work
- * than vk_latent_decode at latent_dim 512. */
+ * take turns, and 20 MB of partial results.  From ~170 new tokens a sequence on
+ * this does less work than vk_latent_decode at latent_dim 512. */
 size_t    vk_latent_prefill_workspace_size(const vk_pool* pool, int32_t batch, int32_t max_seq_len, int32_t num_heads);
 vk_status vk_latent_prefill(vk_pool* pool, int32_t layer, const void* q, int64_t q_token_stride,
                             int64_t q_head_stride, const void* w_kv, int64_t w_stride, void* out,

@@ -28,11 +28,11 @@
 //    (r/16)*32 + r%16 of TMEM (M = 64 fills 16 lanes of each warp's quarter); the
 //    matrix-fragment load spreads them over all 32 threads (2 rows x 16 keys
 //    each), and P goes to shared memory by stmatrix.  O is rescaled only when a
-//    row's maximum grows by more than 2^8 (bf16) or 2^4 (fp16; all warps vote).
+//    row's maximum grows by more than 2^8 (all warps vote).
 //
 // P is rounded to the cache's 16-bit type for the second product, the type that
 // the tensor core takes beside it: relative 2^-8 (bf16) or 2^-11 (fp16) a weight at
-// most, the same step as the output's own rounding, absolute 2^-36 of the row's
+// most, the same step as the output's own rounding, absolute 2^-32 of the row's
 // largest weight among fp16's subnormals (struct Weights); the sum of the weights is
 // taken from the unrounded fp32 values.
 //
